@@ -20,7 +20,7 @@ from torch.utils._device import DeviceContext
 # host-sanitized one that tests/test_host_sanitizers.py runs the ABI checks on).
 LIB_PATH = pathlib.Path(os.environ.get("CAB_HIP_LIB") or
                         pathlib.Path(__file__).resolve().with_name("libcab_hip.so"))
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 CAB_OK, CAB_EINVAL, CAB_EDTYPE, CAB_ESHAPE, CAB_EWORKSPACE, CAB_EHIP = range(6)
 CAB_F32, CAB_F16, CAB_BF16 = 0, 1, 2
@@ -89,6 +89,13 @@ SIGNATURES = {
                                      _i64x4, _i64x4, _i64, _ptr]),
     "cab_key_sums": (ctypes.c_int, [_ptr, ctypes.c_int, _i64, _i64, _i64, _i64, _i64x4, _ptr, _i64,
                                     _ptr, _ptr]),
+    "cab_kv_append_at": (ctypes.c_int, [_ptr, _ptr, _ptr, _ptr, _i32, _i64, _i64, _i64, _i64, _i64,
+                                        _i64x4, _i64x4, _i64x4, _i64x4, _ptr, _ptr, _ptr]),
+    "cab_kv_commit": (ctypes.c_int, [ctypes.POINTER(_ptr), _i32, _i32, _i64, _i64, _i64, _i64,
+                                     _i64x4, _ptr, _i64, _ptr, _i64, _i64, _ptr, _i32, _ptr, _ptr]),
+    "cab_verify_drafts": (ctypes.c_int, [_ptr, _ptr, ctypes.c_int, _i64, _i64, _i64, _i64x4, _i64x4,
+                                         _ptr, _ptr, _i64, _ptr, _ptr, _f32, _ptr, _ptr, _ptr,
+                                         _ptr]),
     "cab_token_frc": (ctypes.c_int, [_ptr, ctypes.c_int, _i64, _i64, _ptr, _ptr, _ptr, _ptr]),
     "cab_attention_symmetrize": (ctypes.c_int, [_ptr, ctypes.c_int, _i64, _i64, _i64, _i64, _i64x4,
                                                 _ptr, _i64, _ptr]),
@@ -229,6 +236,30 @@ def closed(t: torch.Tensor) -> bool:
     """Whether torch refuses in-place writes into ``t`` here (an inference tensor
     outside inference mode)."""
     return t.is_inference() and not torch.is_inference_mode_enabled()
+
+
+def require_plain(fn: str, *tensors: torch.Tensor) -> None:
+    """Raises for what only torch ops can follow: tensor subclasses, transforms,
+    modes, and gradients to record (the operators that call this have none)."""
+    if not addressable(*tensors):
+        raise RuntimeError(f"{fn} takes plain tensors outside transforms, tracing and modes")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise RuntimeError(f"{fn} has no gradient: call it under torch.no_grad() or on "
+                                   "detached tensors")
+
+
+def index32(t: torch.Tensor, name: str, shape: tuple) -> torch.Tensor:
+    """``t`` as a contiguous int32 tensor of ``shape`` (itself where it is one)."""
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}; got {list(t.shape)}")
+    if t.dtype is not torch.int32:
+        if t.dtype is not torch.int64:
+            raise TypeError(f"{name} must be int32 or int64; got {t.dtype}")
+        # (values past 32 bits stay out of range instead of wrapping round)
+        t = t.clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def wrote(*tensors: torch.Tensor) -> None:

@@ -2,9 +2,10 @@
 caches on one device-resident store and eviction core (``store.py``)."""
 
 from .cab_cache import CABCache, CABCacheConfig
+from .drafts import append_drafts, commit_drafts
 from .h2o_cache import H2OCache
 from .prune import gather_into, gather_positions, prune_layers
 from .store import EvictingCache, LayeredKV
 
 __all__ = ["CABCache", "CABCacheConfig", "H2OCache", "EvictingCache", "LayeredKV",
-           "gather_into", "gather_positions", "prune_layers"]
+           "append_drafts", "commit_drafts", "gather_into", "gather_positions", "prune_layers"]

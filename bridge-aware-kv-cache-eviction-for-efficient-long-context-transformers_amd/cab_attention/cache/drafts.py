@@ -1,0 +1,123 @@
+"""Drafted tokens in K/V caches whose sequences have lengths of their own: new
+rows written behind each sequence's length (``cab_kv_append_at``), and after
+verification the accepted ones kept (``cab_kv_commit``). Lengths, counts and
+paths stay on the device, so a decoding loop reads nothing back and can be
+captured into a graph. The reference has neither: its caches hold one length and
+grow by ``torch.cat`` (cache/cab_cache.py:122-175).
+
+One step of a loop over static buffers ``[B, H_kv, N, D]`` per layer::
+
+    for layer: append_drafts(k, v, keys[layer], values[layer], lengths)
+               tree_attention(q, keys[layer], values[layer], parents, lengths)
+    path, counts, token = verify_drafts(logits, tokens, parents, uniforms, noise)
+    lengths = commit_drafts(keys + values, lengths, path, counts)
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Sequence
+
+import torch
+
+from .. import _native as nat
+
+_SIZES = {torch.bfloat16: 2, torch.float16: 2, torch.float32: 4}
+
+
+def _writable(fn: str, *caches: torch.Tensor) -> None:
+    for c in caches:
+        if nat.closed(c):
+            raise RuntimeError(f"{fn}: a cache is an inference tensor; write to it in inference mode")
+
+
+def append_drafts(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                  lengths: torch.Tensor, counts: Optional[torch.Tensor] = None) -> None:
+    """``cache[b, :, lengths[b] + t] = new[b, :, t]`` for ``t < counts[b]``, K and V in
+    one launch.
+
+    k, v: ``[B, H, n, D]``, any strides. k_cache, v_cache: ``[B, H, N, D]`` of the same
+    dtype (bf16, fp16, fp32) with a contiguous last dim. lengths, counts (``None``: n
+    rows of every sequence): int32 ``[B]`` on the device (int64 is converted). Rows that
+    would lie behind the cache's N, and those of a sequence of negative length, are
+    not written. The new rows must not be views of the caches.
+    """
+    if k.dim() != 4 or v.shape != k.shape:
+        raise ValueError("k and v must be two [B, H, n, D] tensors")
+    B, H, n, D = k.shape
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape or shape[:2] != (B, H) or shape[3] != D:
+        raise ValueError(f"k_cache and v_cache must be [{B}, {H}, N, {D}]; got {tuple(shape)} and "
+                         f"{tuple(v_cache.shape)}")
+    dt = k.dtype
+    es = _SIZES.get(dt)
+    if es is None or v.dtype is not dt or k_cache.dtype is not dt or v_cache.dtype is not dt:
+        raise TypeError("k, v and the caches must be of one dtype: bfloat16, float16 or float32")
+    dev = nat.require_device(k, v, k_cache, v_cache, lengths)
+    nat.require_plain("append_drafts", k, v, k_cache, v_cache)
+    _writable("append_drafts", k_cache, v_cache)
+    lengths = nat.index32(lengths, "lengths", (B,))
+    if counts is not None:
+        nat.require_device(k, counts)
+        counts = nat.index32(counts, "counts", (B,))
+    k_st, v_st, kc_st, vc_st = k.stride(), v.stride(), k_cache.stride(), v_cache.stride()
+    ks, kc = nat.I64x4(*k_st), nat.I64x4(*kc_st)
+    with nat.on_device(dev):
+        st = nat.load().cab_kv_append_at(
+            k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), es, B, H, n, D,
+            shape[2], ks, ks if v_st == k_st else nat.I64x4(*v_st), kc,
+            kc if vc_st == kc_st else nat.I64x4(*vc_st), lengths.data_ptr(), nat.ptr(counts),
+            nat.stream_ptr(dev))
+    nat.check("cab_kv_append_at", st)
+    nat.wrote(k_cache, v_cache)
+
+
+def commit_drafts(caches: Sequence[torch.Tensor], lengths: torch.Tensor, path: torch.Tensor,
+                  counts: torch.Tensor) -> torch.Tensor:
+    """Keeps the accepted ones of each sequence's drafted rows, in every cache of the
+    list (all layers' K and V, one launch per 64): row ``lengths[b] + path[b, j]``
+    moves to row ``lengths[b] + j`` for ``j < counts[b]``. Returns the new lengths,
+    int32 ``[B]``: the old ones plus the rows kept. No other row changes.
+
+    caches: distinct ``[B, H, N, D]`` tensors of one shape, dtype (bf16, fp16, fp32)
+    and stride set, with a contiguous last dim. lengths, counts: int32 ``[B]``; path:
+    int32 ``[B, T]``, on the device, as :func:`verify_drafts` gives them (int64 is
+    converted). A path's first ``counts[b]`` entries ascend strictly; the first one
+    that does not, or that lies outside ``[0, T)`` or the cache, ends it.
+    """
+    caches = list(caches)
+    if not caches:
+        raise ValueError("commit_drafts needs at least one cache")
+    ref = caches[0]
+    shape, stride, dt = ref.shape, ref.stride(), ref.dtype
+    es = _SIZES.get(dt)
+    if len(shape) != 4 or path.dim() != 2:
+        raise ValueError("caches must be [B, H, N, D] and path [B, T]")
+    if es is None:
+        raise TypeError(f"unsupported dtype {dt}; expected float32, float16 or bfloat16")
+    for c in caches:
+        if c.shape != shape or c.dtype is not dt or c.stride() != stride:
+            raise ValueError("the caches must share one shape, dtype and stride set")
+    B, H, N, D = shape
+    dev = nat.require_device(lengths, path, counts, *caches)
+    nat.require_plain("commit_drafts", *caches)
+    _writable("commit_drafts", *caches)
+    lengths = nat.index32(lengths, "lengths", (B,))
+    counts = nat.index32(counts, "counts", (B,))
+    path = nat.index32(path, "path", (B, path.shape[1]))
+    new = torch.empty(B, dtype=torch.int32, device=dev)
+    _commit(caches, lengths, 0, path, counts, 0, new, dev, es)
+    return new
+
+
+def _commit(caches, lengths, length, path, counts, count, new, dev, es):
+    B, H, N, D = caches[0].shape
+    n = len(caches)
+    ptrs = (ctypes.c_void_p * n)(*[c.data_ptr() for c in caches])
+    with nat.on_device(dev):
+        st = nat.load().cab_kv_commit(
+            ptrs, n, es, B, H, N, D, nat.strides4(caches[0]), nat.ptr(lengths), length,
+            path.data_ptr(), path.shape[1], path.shape[1] if path.shape[0] == B else 0,
+            nat.ptr(counts), count, nat.ptr(new), nat.stream_ptr(dev))
+    nat.check("cab_kv_commit", st)
+    nat.wrote(*caches)

@@ -55,7 +55,7 @@ enum { CAB_NORM_NONE = 0, CAB_NORM_MINMAX = 1 };
 /* FRC combination (experiments/longbench_qa/config.py:465; test.ipynb:111-145). */
 enum { CAB_FRC_ADDITIVE = 0, CAB_FRC_MULTIPLICATIVE = 1, CAB_FRC_AUGMENTED = 2 };
 
-#define CAB_ABI_VERSION 11
+#define CAB_ABI_VERSION 12
 
 int cab_abi_version(void);
 const char* cab_last_error(void);
@@ -428,6 +428,76 @@ cab_status_t cab_key_sums(const void* attention, cab_dtype_t dtype, int64_t B, i
                           int64_t N_q, int64_t N_k, const int64_t strides[4],
                           const float* old_sums, int64_t n_old, float* sums, void* stream);
 
+/*
+ * Drafted tokens in caches whose sequences have lengths of their own (no
+ * counterpart in the reference, whose caches grow by torch.cat,
+ * cache/cab_cache.py:122-175). lengths, counts, path: int32 device arrays,
+ * read when the work runs, so that no call needs a read-back.
+ *
+ * cab_kv_append_at copies new K and V rows [B,H,n,D] (element strides;
+ * elements of 2 or 4 bytes) into two buffers [B,H,rows,D] (strides each, last
+ * dim 1): sequence b's row r < counts[b] (counts NULL: r < n) goes to row
+ * lengths[b] + r. Rows that would lie outside the buffer, and all rows of a
+ * sequence of negative length, go nowhere. Sources and buffers must not
+ * overlap.
+ *
+ * cab_kv_commit keeps the accepted ones of `nodes` drafted rows in each of
+ * n_tensors buffers (distinct, of one shape and stride set, every layer's K
+ * and V; `tensors` is a host array): with len = lengths[b] (lengths NULL:
+ * length0), row len + path[b][j] moves to row len + j for j < counts[b]
+ * (counts NULL: count0), and new_lengths[b] (may be NULL) = len + rows kept.
+ * Other rows stay as they are. Entries of a path ascend strictly; the first
+ * one that does not, or that is outside [0, nodes) or the buffer, ends it. A
+ * negative length keeps none. path_stride: entries from one sequence's path
+ * to the next's (0: one path for all). new_lengths is another array than
+ * lengths. One launch per 64 tensors.
+ */
+cab_status_t cab_kv_append_at(const void* k, const void* v, void* k_dst, void* v_dst,
+                              int32_t element_bytes, int64_t B, int64_t H, int64_t n, int64_t D,
+                              int64_t rows, const int64_t k_strides[4], const int64_t v_strides[4],
+                              const int64_t k_dst_strides[4], const int64_t v_dst_strides[4],
+                              const int32_t* lengths, const int32_t* counts, void* stream);
+
+cab_status_t cab_kv_commit(void* const* tensors, int32_t n_tensors, int32_t element_bytes,
+                           int64_t B, int64_t H, int64_t rows, int64_t D, const int64_t strides[4],
+                           const int32_t* lengths, int64_t length0, const int32_t* path,
+                           int64_t nodes, int64_t path_stride, const int32_t* counts,
+                           int32_t count0, int32_t* new_lengths, void* stream);
+
+/*
+ * Verification of drafted tokens against the target's logits (no counterpart
+ * in the reference, which decodes one token at a time). B sequences, each with
+ * a tree of T <= 256 nodes: node 0 is the token the model has taken already
+ * (the last one sampled), tokens[b][i] (int64) the draft at node i > 0 and
+ * parents[b][i] < i its parent; nodes with other parents (-1, -2, ..) are
+ * nobody's children. logits[b][i]: the target's logits after node i; draft_logits
+ * (NULL: drafts are taken as certain) those the children of node i were drawn
+ * from, independently. dtype of both; strides in elements {b, node}, last dim
+ * contiguous. From node 0 on, with p = softmax(logits / temperature), q the same
+ * of draft_logits, r = uniforms[b][child], the children in index order:
+ *   temperature 0: a child is accepted if its token is the row's argmax;
+ *   no draft_logits: if r * Z < p(x), Z = 1 - sum of p over the (distinct) tokens
+ *     of siblings rejected before; their weights become 0;
+ *   draft_logits: with w = p at first, if r * q(x) * sum w < w(x); a rejection
+ *     takes q * sum w off w, and what is below 0 is 0.
+ * The walk goes on at the first accepted child. Where none is accepted, the
+ * next token is the argmax (greedy) or argmax_x w(x) / noise[b][x]; noise ~
+ * Exp(1) makes it a sample of w / sum w. Ties go to the lowest index. A NaN
+ * logit weighs 0 as -inf does; entries of +inf share all weight. A draft outside
+ * [0, V) is passed over. With no weight left of w the next token comes from p;
+ * with none in p either it is -1.
+ * uniforms: fp32 [B,T]; noise: fp32 [B,V] (both unused when greedy); parents_stride: 0 for
+ * one tree for all sequences, else entries from one to the next. Out: path int32
+ * [B,T], the accepted nodes ascending (node 0 first), then -1; counts int32 [B],
+ * how many; next_tokens int64 [B]. Arrays are contiguous unless a stride is
+ * given.
+ */
+cab_status_t cab_verify_drafts(const void* logits, const void* draft_logits, cab_dtype_t dtype,
+                               int64_t B, int64_t T, int64_t V, const int64_t logit_strides[2],
+                               const int64_t draft_strides[2], const int64_t* tokens,
+                               const int32_t* parents, int64_t parents_stride,
+                               const float* uniforms, const float* noise, float temperature,
+                               int32_t* path, int32_t* counts, int64_t* next_tokens, void* stream);
 
 /*
  * Token-level Forman-Ricci curvature of a weighted directed graph A [n, n]
