@@ -93,6 +93,11 @@ SIGNATURES = {
                                         _i64x4, _i64x4, _i64x4, _i64x4, _ptr, _ptr, _ptr]),
     "cab_kv_commit": (ctypes.c_int, [ctypes.POINTER(_ptr), _i32, _i32, _i64, _i64, _i64, _i64,
                                      _i64x4, _ptr, _i64, _ptr, _i64, _i64, _ptr, _i32, _ptr, _ptr]),
+    "cab_tree_attn_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, _i64, _i64, _i64, _i64, _i64,
+                                                        _i64]),
+    "cab_tree_attn_fwd": (ctypes.c_int, [_ptr, _ptr, _ptr, ctypes.c_int, _i64, _i64, _i64, _i64, _i64,
+                                         _i64, _i64x4, _i64x4, _i64x4, _i64x4, _ptr, _i64, _ptr, _i64,
+                                         _f32, _ptr, _ptr, _ptr, ctypes.c_size_t, _ptr]),
     "cab_verify_drafts": (ctypes.c_int, [_ptr, _ptr, ctypes.c_int, _i64, _i64, _i64, _i64x4, _i64x4,
                                          _ptr, _ptr, _i64, _ptr, _ptr, _f32, _ptr, _ptr, _ptr,
                                          _ptr]),

@@ -465,6 +465,36 @@ cab_status_t cab_kv_commit(void* const* tensors, int32_t n_tensors, int32_t elem
                            int32_t count0, int32_t* new_lengths, void* stream);
 
 /*
+ * Attention of a tree of drafted tokens over a cache (no counterpart in the
+ * reference, which decodes one token at a time). With len = lengths[b] (lengths
+ * NULL: length0, in [0, N - T]; device values outside are taken as the nearest
+ * inside), rows [0, len) of k and v are sequence b's context and the next T its
+ * drafts. Node i sees the context, itself and its ancestors: parents[b][i] is -1 (a
+ * root), or an earlier node, or anything else (no node: it and its descendants
+ * see nothing and are seen by nobody). out[b,h,i] = softmax_s(q_i . k_s * scale) v_s
+ * over those keys (0 for no node), lse[b,h,i] the natural-log log-sum-exp of the
+ * scaled scores (-inf for no node), lse may be NULL. Keys a node does not see do
+ * not reach it whatever they hold.
+ * q, out: [B,H,T,D]; k, v: [B,H_kv,N,D] (strides); H % H_kv == 0; D == 64 or 128;
+ * T <= 256; bf16, fp16 (products of 16-bit operands, P rounded to 16 bits, sums in
+ * fp32) or fp32 (fp32 throughout). Token strides of k and v in [0, 2^25] bytes.
+ * parents: int32, parents_stride 0 (one tree for all) or entries from one sequence's
+ * to the next's; lse: contiguous fp32 [B,H,T]. workspace:
+ * cab_tree_attn_workspace_bytes() bytes (0 for sizes the call refuses), 16-byte
+ * aligned, overwritten; it depends on the sizes alone, not on the lengths.
+ */
+size_t cab_tree_attn_workspace_bytes(cab_dtype_t dtype, int64_t B, int64_t H, int64_t H_kv,
+                                     int64_t T, int64_t N, int64_t D);
+
+cab_status_t cab_tree_attn_fwd(const void* q, const void* k, const void* v, cab_dtype_t dtype,
+                               int64_t B, int64_t H, int64_t H_kv, int64_t T, int64_t N, int64_t D,
+                               const int64_t q_strides[4], const int64_t k_strides[4],
+                               const int64_t v_strides[4], const int64_t o_strides[4],
+                               const int32_t* parents, int64_t parents_stride,
+                               const int32_t* lengths, int64_t length0, float scale, void* out,
+                               float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Verification of drafted tokens against the target's logits (no counterpart
  * in the reference, which decodes one token at a time). B sequences, each with
  * a tree of T <= 256 nodes: node 0 is the token the model has taken already
