@@ -52,6 +52,7 @@ def _hipcc() -> str:
 # (tests for them look at the bits).
 EXTRA_FLAGS = {
     "sparse_attn.hip": ["-Xarch_device", "-fno-honor-nans"],
+    "tree_attn.hip": ["-Xarch_device", "-fno-honor-nans"],
 }
 
 

@@ -100,7 +100,9 @@ SIGNATURES = {
                                          _f32, _ptr, _ptr, _ptr, ctypes.c_size_t, _ptr]),
     "cab_verify_drafts": (ctypes.c_int, [_ptr, _ptr, ctypes.c_int, _i64, _i64, _i64, _i64x4, _i64x4,
                                          _ptr, _ptr, _i64, _ptr, _ptr, _f32, _ptr, _ptr, _ptr,
-                                         _ptr]),
+                                         _ptr, ctypes.c_size_t, _ptr]),
+    "cab_verify_drafts_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, _i64, _i64, _i64,
+                                                            ctypes.c_int, ctypes.c_int]),
     "cab_token_frc": (ctypes.c_int, [_ptr, ctypes.c_int, _i64, _i64, _ptr, _ptr, _ptr, _ptr]),
     "cab_attention_symmetrize": (ctypes.c_int, [_ptr, ctypes.c_int, _i64, _i64, _i64, _i64, _i64x4,
                                                 _ptr, _i64, _ptr]),

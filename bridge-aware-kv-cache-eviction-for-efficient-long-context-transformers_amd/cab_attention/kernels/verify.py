@@ -80,13 +80,18 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Ten
         if draft_logits.stride(2) != 1:
             draft_logits = draft_logits.contiguous()
         ds = _I64x2(draft_logits.stride(0), draft_logits.stride(1))
+    lib = nat.load()
+    wbytes = lib.cab_verify_drafts_workspace_bytes(dt, B, T, V, temperature == 0.0,
+                                                   draft_logits is not None)
+    ws = torch.empty(wbytes, dtype=torch.uint8, device=dev) if wbytes else None
     path = torch.empty((B, T), dtype=torch.int32, device=dev)
     counts = torch.empty(B, dtype=torch.int32, device=dev)
     chosen = torch.empty(B, dtype=torch.int64, device=dev)
     with nat.on_device(dev):
-        st = nat.load().cab_verify_drafts(
+        st = lib.cab_verify_drafts(
             logits.data_ptr(), nat.ptr(draft_logits), dt, B, T, V, ls, ds, tokens.data_ptr(),
             parents.data_ptr(), 0 if shared else T, nat.ptr(uniforms), nat.ptr(noise), temperature,
-            path.data_ptr(), counts.data_ptr(), chosen.data_ptr(), nat.stream_ptr(dev))
+            path.data_ptr(), counts.data_ptr(), chosen.data_ptr(), nat.ptr(ws), wbytes,
+            nat.stream_ptr(dev))
     nat.check("cab_verify_drafts", st)
     return path, counts, chosen

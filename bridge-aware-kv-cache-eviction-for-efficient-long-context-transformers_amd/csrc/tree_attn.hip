@@ -3,8 +3,11 @@
 // the context and the drafts that are i or its ancestors. The query heads that share
 // a K / V head and their T nodes are the R = group * T rows of one unit (b, K / V head).
 //
-//  1. The context has no mask: every row of a unit sees all of it. It is split over
-//     workgroups, each leaving one partial (maximum m, row sum l, unnormalised O) per row:
+//  1. The context has no mask: every row of a unit sees all of it. The contexts of all
+//     units, cut into pieces of as many keys as a workgroup takes at a time, make one
+//     list, and each workgroup takes an equal stretch of it, whatever the lengths. Of
+//     each unit that its stretch touches it leaves one partial (maximum m, row sum l,
+//     unnormalised O) per row:
 //     - rows_kernel (up to 32 rows, and fp32): every wave walks its own 32-key steps, K
 //       and V straight from memory into matrix operands;
 //     - tile_kernel (more rows, 16 bits): 64-key tiles of K and V in LDS, read by all
@@ -23,9 +26,10 @@ namespace cab {
 namespace {
 
 constexpr int MAX_NODES = 256;
-constexpr int MAX_SPLITS = 256;
 constexpr int STEP = 32;  // keys of a wave's step in rows_kernel
-constexpr int TILE = 64;  // keys of a tile in tile_kernel
+constexpr int QUAD = 4 * STEP;  // its pieces: a step for each of four waves
+constexpr int TILE = 64;        // tile_kernel's pieces
+constexpr int FEW_PIECES = 32;  // of an even cut, up to which stretches begin anew with every unit
 
 struct TreeArgs {
   const char* q;
@@ -34,11 +38,14 @@ struct TreeArgs {
   int64_t qs[3], ks[3], vs[3];  // bytes: b, h, token
   const int32_t* lengths;       // may be null: length0
   int64_t length0, most;        // most: N - T, the longest context
-  int32_t Hkv, group, T, R, splits, row_tiles;
-  float c;    // scale * log2(e)
-  float* po;  // [unit][R][splits][D]
-  float* pm;  // [unit][R][splits] maxima of the scores * c
-  float* pl;  // [unit][R][splits] row sums
+  int32_t B, Hkv, group, T, R, row_tiles;
+  int32_t wgs, least;  // workgroups that share the list; the fewest pieces one takes
+  float c;             // scale * log2(e)
+  // Partials. Workgroup x's of unit u is number x + u: down the list either x or u goes
+  // up by one from one partial to the next.
+  float* po;  // [number][R][D]
+  float* pm;  // [number][R] maxima of the scores * c
+  float* pl;  // [number][R] row sums
 };
 
 __device__ __forceinline__ int context_length(const int32_t* lengths, int64_t length0, int64_t most,
@@ -47,15 +54,98 @@ __device__ __forceinline__ int context_length(const int32_t* lengths, int64_t le
   return static_cast<int>(n < 0 ? 0 : n < most ? n : most);
 }
 
-// Steps of `unit` keys a split takes of a context, and the splits that get any.
-__device__ __forceinline__ int split_steps(int length, int unit, int splits, int round) {
-  const int steps = (length + unit - 1) / unit;
-  const int per = (steps + splits - 1) / splits;
-  return (per + round - 1) / round * round;
+// Sums over lanes 0 .. lane of a wave (lane moves within rows of 16, then row by row).
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15, 31
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return x;
 }
-__device__ __forceinline__ int live_splits(int length, int unit, int splits, int round) {
-  const int per = split_steps(length, unit, splits, round);
-  return per ? ((length + unit - 1) / unit + per - 1) / per : 0;
+__device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
+
+// A lane's context lengths of sequences lane, lane + 64, ..; the first is kept.
+struct Lengths {
+  const TreeArgs& a;
+  int first;
+  __device__ __forceinline__ explicit Lengths(const TreeArgs& args) : a(args), first(0) {
+    if (lane_id() < a.B) first = context_length(a.lengths, a.length0, a.most, lane_id());
+  }
+  __device__ __forceinline__ int mine(int b0) const {  // of sequence b0 + lane, 0 past the last
+    if (b0 == 0) return first;
+    return b0 + lane_id() < a.B ? context_length(a.lengths, a.length0, a.most, b0 + lane_id()) : 0;
+  }
+  __device__ __forceinline__ int of(int b) const {  // b: the same in every lane
+    return __builtin_amdgcn_readfirstlane(
+        b < 64 ? __builtin_amdgcn_readlane(first, b) : context_length(a.lengths, a.length0, a.most, b));
+  }
+};
+
+__device__ __forceinline__ int round_to(int x, int grain) { return (x + grain - 1) / grain * grain; }
+
+// How the list is cut: pieces a workgroup takes, and what a unit's share of the list is
+// rounded up to. An even cut takes ceil(pieces / workgroups), and its stretches run on
+// from one unit into the next. Where that is only a few pieces, beginning a second part
+// costs as much as the pieces: then stretches begin anew with every unit, and are as
+// long as it takes for the workgroups to suffice.
+struct Cut {
+  int per, grain;
+};
+template <int KEYS>
+__device__ __forceinline__ int pieces_of(int length) { return (length + KEYS - 1) / KEYS; }
+
+template <int KEYS>
+__device__ __forceinline__ Cut list_cut(const TreeArgs& a, const Lengths& len) {
+  int all = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) all += wave_sum(pieces_of<KEYS>(len.mine(b0)));
+  int per = max(a.least, (all * a.Hkv + a.wgs - 1) / a.wgs);
+  if (per > FEW_PIECES || a.B * a.Hkv > a.wgs / 4) return Cut{per, 1};
+  for (;; ++per) {  // (ends: one a unit suffice)
+    int parts = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64)
+      parts += wave_sum((pieces_of<KEYS>(len.mine(b0)) + per - 1) / per);
+    if (parts * a.Hkv <= a.wgs) return Cut{per, per};
+  }
+}
+
+// f(sequence, head, first piece, pieces, length) for each part of workgroup x's stretch.
+template <int KEYS, typename F>
+__device__ __forceinline__ void over_stretch(const TreeArgs& a, int x, F f) {
+  const Lengths len(a);
+  const Cut cut = list_cut<KEYS>(a, len);
+  int at = x * cut.per;
+  int before = 0, b = -1, n = 0;  // n: the sequence's pieces, rounded up
+  for (int b0 = 0; b0 < a.B && b < 0; b0 += 64) {
+    const int mine = round_to(pieces_of<KEYS>(len.mine(b0)), cut.grain), upto = wave_scan(mine);
+    const uint64_t past = ballot64((before + upto) * a.Hkv > at);
+    if (past) {
+      const int i = __builtin_ctzll(past);
+      b = b0 + i;
+      n = __builtin_amdgcn_readlane(mine, i);
+      before += __builtin_amdgcn_readlane(upto, i) - n;
+    } else {
+      before += __builtin_amdgcn_readlane(upto, 63);
+    }
+  }
+  if (b < 0) return;  // past the list's end
+  at -= before * a.Hkv;
+  int head = at / n, piece = at - head * n;
+  for (int left = cut.per; left > 0;) {
+    const int length = len.of(b);
+    const int take = min(left, n - piece), there = pieces_of<KEYS>(length) - piece;
+    f(b, head, piece, min(take, there), length);  // (a rounded share ends in less than a stretch)
+    left -= take;
+    piece = 0;
+    if (++head == a.Hkv) {
+      head = 0;
+      do {
+        if (++b == a.B) return;
+        n = round_to(pieces_of<KEYS>(len.of(b)), cut.grain);
+      } while (n == 0);
+    }
+  }
 }
 
 // K and V are read once: non-temporal loads.
@@ -115,7 +205,7 @@ __device__ __forceinline__ f32x4 mfma4(float a, float b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-// Grid: (splits, units, row tiles of 16 QT rows).
+// Grid: (workgroups, row tiles of 16 QT rows).
 template <cab_dtype_t DT, int HD, int QT>
 __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void rows_kernel(TreeArgs a) {
   constexpr bool F32 = DT == CAB_F32, BF16 = DT == CAB_BF16;
@@ -125,19 +215,17 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void rows_kernel(TreeAr
   __shared__ f32x4 merge[4][NDT * 64];  // one query tile's O^T per wave
   __shared__ float sm[4][QT][16], sl[4][QT][16];
 
-  const int split = blockIdx.x, unit = blockIdx.y, row0 = blockIdx.z * (16 * QT);
-  const int b = unit / a.Hkv, hk = unit - b * a.Hkv;
-  const int len = context_length(a.lengths, a.length0, a.most, b);
-  const int steps = (len + STEP - 1) / STEP;
-  const int per = split_steps(len, STEP, a.splits, 4);
-  if (split * per >= steps) return;
+  const int row0 = blockIdx.y * (16 * QT);
   const int w = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
-  const int lane = lane_id(), l16 = lane & 15, g = lane >> 4;
   const float c = a.c;
-  const char* kb = a.k + b * a.ks[0] + hk * a.ks[1];
-  const char* vb = a.v + b * a.vs[0] + hk * a.vs[1];
   const uint32_t krow = static_cast<uint32_t>(a.ks[2]), vrow = static_cast<uint32_t>(a.vs[2]);
 
+  over_stretch<QUAD>(a, blockIdx.x, [&](int b, int hk, int piece, int pieces, int len) {
+  int lane = lane_id();
+  asm volatile("" : "+v"(lane));  // (what follows from it is not kept over the parts)
+  const int l16 = lane & 15, g = lane >> 4;
+  const char* kb = a.k + b * a.ks[0] + hk * a.ks[1];
+  const char* vb = a.v + b * a.vs[0] + hk * a.vs[1];
   u32x4 qr[QT][NJ];
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
@@ -252,8 +340,8 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void rows_kernel(TreeAr
     }
   };
 
-  const int end = min(steps, (split + 1) * per);
-  int step = split * per + w;
+  const int end = min((len + STEP - 1) / STEP, 4 * (piece + pieces));
+  int step = 4 * piece + w;
   if constexpr (F32 || QT * HD > 128) {  // (two register sets would spill)
     SR x;
     for (; step < end; step += 4) {
@@ -275,6 +363,8 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void rows_kernel(TreeAr
   }
 
   // Merge of the four waves: common maximum, then the scaled O^T and sums in wave order.
+  const int64_t part = static_cast<int64_t>(blockIdx.x) + b * a.Hkv + hk;
+  __syncthreads();  // (the last part's merge has been read)
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
     l[qt] += shfl_xor_f32(l[qt], 16);
@@ -294,22 +384,22 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void rows_kernel(TreeAr
       const int dt = e >> 6, ll = e & 63, row = row0 + 16 * qt + (ll & 15);
       const f32x4 y = (merge[0][e] + merge[1][e]) + (merge[2][e] + merge[3][e]);
       if (row < a.R) {
-        float* po = a.po + ((static_cast<int64_t>(unit) * a.R + row) * a.splits + split) * HD;
+        float* po = a.po + (part * a.R + row) * HD;
 #pragma unroll
         for (int r = 0; r < 4; ++r) po[NDT * (4 * (ll >> 4) + r) + dt] = y[r];
       }
     }
     const int row = row0 + 16 * qt + static_cast<int>(threadIdx.x);
     if (threadIdx.x < 16 && row < a.R) {
-      const int64_t x = (static_cast<int64_t>(unit) * a.R + row) * a.splits + split;
-      a.pm[x] = mm * c;
-      a.pl[x] = (sl[0][qt][l16] + sl[1][qt][l16]) + (sl[2][qt][l16] + sl[3][qt][l16]);
+      a.pm[part * a.R + row] = mm * c;
+      a.pl[part * a.R + row] = (sl[0][qt][l16] + sl[1][qt][l16]) + (sl[2][qt][l16] + sl[3][qt][l16]);
     }
     if (qt + 1 < QT) __syncthreads();
   }
+  });
 }
 
-// 64-key tiles of K and V in LDS, two of each; WAVES waves of 16 QT rows. Rows are
+// 64-key tiles of K and V in LDS; WAVES waves of 16 QT rows. Rows are
 // stored in 16-byte chunks, chunk x of row r at x ^ swizzle(r), so that neither the
 // K operand's reads (16 rows, one chunk each) nor V's transposing ones meet in a bank.
 template <int HD>
@@ -319,33 +409,77 @@ __device__ __forceinline__ uint32_t tile_offset(uint32_t row, uint32_t chunk) {
   return (row * CH + (chunk ^ z)) * 16u;
 }
 
-// Grid: 1-D over (row tile fastest, split, unit), neighbours on one XCD, so that a
-// split's row tiles find its K and V in one L2.
+// Grid: 1-D over (row tile fastest, workgroup), neighbours on one XCD, so that a
+// stretch's row tiles find its K and V in one L2.
+// bdma16_untracked for operands that may come out of a vector lane (a spilled scalar, a
+// readfirstlane): a load reads such a scalar rightly five wait states after it was
+// written, which the compiler does not count inside an asm block.
+__device__ __forceinline__ void dma16(const sgpr_rsrc_t& r, uint32_t voff, uint32_t soff, const void* l) {
+  const uint32_t lds = static_cast<uint32_t>(
+      __builtin_amdgcn_readfirstlane(static_cast<int>(reinterpret_cast<uintptr_t>(l))));
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
+               :
+               : "v"(voff), "s"(r), "s"(soff), "{m0}"(lds)
+               : "memory");
+}
+
+// Tiles go to LDS without passing through registers, the next one in flight while one is
+// computed (2 and 3 in flight measured 2 to 4 % slower). A wave waits for its own
+// loads of a tile, and the workgroup's barrier makes that everybody's; the same
+// barrier frees the tile before.
 template <cab_dtype_t DT, int HD, int QT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void tile_kernel(TreeArgs a) {
   constexpr bool BF16 = DT == CAB_BF16;
   constexpr int NDT = HD / 16, NDS = HD / 32, CH = HD / 8;
-  constexpr int THREADS = 64 * WAVES, LOADS = TILE * CH / THREADS;  // 16-byte pieces per thread
+  constexpr int ROWS = 64 / CH * WAVES;  // rows a round of the waves' loads covers (1 KB each)
+  constexpr int LOADS = TILE / ROWS;     // a wave's loads of a tile of K, and of V
+  static_assert(LOADS >= 1 && TILE % ROWS == 0, "a tile is whole rounds of loads");
   constexpr uint32_t TILE_BYTES = TILE * HD * 2;
-  __shared__ __align__(16) char lds[2][2][TILE_BYTES];  // [buffer][K, V]
+  __shared__ __align__(16) char lds[2][2][TILE_BYTES];  // [slot][K, V]
 
   const int64_t id = xcd_remap(blockIdx.x, gridDim.x);
-  const int rt = static_cast<int>(id % a.row_tiles);
-  const int64_t us = id / a.row_tiles;
-  const int split = static_cast<int>(us % a.splits), unit = static_cast<int>(us / a.splits);
-  const int b = unit / a.Hkv, hk = unit - b * a.Hkv;
-  const int len = context_length(a.lengths, a.length0, a.most, b);
-  const int tiles = (len + TILE - 1) / TILE;
-  const int per = split_steps(len, TILE, a.splits, 1);
-  const int begin = split * per, end = min(tiles, begin + per);
-  if (begin >= end) return;
-  const int tid = threadIdx.x;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int lane = lane_id(), l16 = lane & 15, g = lane >> 4;
+  const int rt = static_cast<int>(id % a.row_tiles), wg = static_cast<int>(id / a.row_tiles);
+  const int w = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int row0 = (rt * WAVES + w) * (16 * QT);
   const float c = a.c;
+
+  over_stretch<TILE>(a, wg, [&](int b, int hk, int begin, int pieces, int len) {
+  int lane = lane_id();
+  asm volatile("" : "+v"(lane));  // (what follows from it is not kept over the parts)
+  const int l16 = lane & 15, g = lane >> 4;
+  const int end = begin + pieces;
   const char* kb = a.k + b * a.ks[0] + hk * a.ks[1];
   const char* vb = a.v + b * a.vs[0] + hk * a.vs[1];
+  // A lane's row in a wave's first load and its place there. Lane i's 16 bytes land at
+  // 16 i, so each lane fetches the chunk that tile_offset() looks for at its place.
+  // (A round of loads further on the swizzle is the same.)
+  const uint32_t lrow = w * (64 / CH) + lane / CH;
+  const uint32_t lch = tile_offset<HD>(lrow, lane % CH) % (16 * CH);
+  const uint32_t koff = lrow * static_cast<uint32_t>(a.ks[2]) + lch;
+  const uint32_t voff = lrow * static_cast<uint32_t>(a.vs[2]) + lch;
+  auto load = [&](int tile, int slot) {
+    const int left = len - tile * TILE;
+    constexpr uint32_t END = 0xffffffe0u;  // rows past the context: an offset past it, read as zero
+    const sgpr_rsrc_t kr = make_sgpr_rsrc(kb + static_cast<int64_t>(tile) * TILE * a.ks[2], END);
+    const sgpr_rsrc_t vr = make_sgpr_rsrc(vb + static_cast<int64_t>(tile) * TILE * a.vs[2], END);
+#pragma unroll
+    for (int n = 0; n < LOADS; ++n) {
+      const uint32_t ks = n * ROWS * static_cast<uint32_t>(a.ks[2]);
+      const uint32_t vs = n * ROWS * static_cast<uint32_t>(a.vs[2]);
+      char* kt = &lds[slot][0][(n * WAVES + w) * 1024];
+      char* vt = &lds[slot][1][(n * WAVES + w) * 1024];
+      if (left >= TILE) {
+        dma16(kr, koff, ks, kt);
+        dma16(vr, voff, vs, vt);
+      } else {
+        const bool in = static_cast<int>(lrow) + n * ROWS < left;
+        dma16(kr, in ? koff + ks : END, 0, kt);
+        dma16(vr, in ? voff + vs : END, 0, vt);
+      }
+    }
+  };
+  lds_barrier();  // the last part's tiles have been read
+  load(begin, 0);
 
   u32x4 qr[QT][NDS];
 #pragma unroll
@@ -369,39 +503,18 @@ __global__ __launch_bounds__(64 * WAVES, 2) void tile_kernel(TreeArgs a) {
     for (int dt = 0; dt < NDT; ++dt) o[qt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // Piece n of a thread: row and chunk of the tile. Rows past the context are zero.
-  u32x4 kx[LOADS], vx[LOADS];
-  auto load = [&](int tile) {
-    const int left = len - tile * TILE;
-    const char* kp = kb + static_cast<int64_t>(tile) * TILE * a.ks[2];
-    const char* vp = vb + static_cast<int64_t>(tile) * TILE * a.vs[2];
+  // (held here, so that nothing in the loop waits for them and with them for the tiles)
 #pragma unroll
-    for (int n = 0; n < LOADS; ++n) {
-      const int p = n * THREADS + tid, row = p / CH, ch = p % CH;
-      kx[n] = vx[n] = u32x4{0u, 0u, 0u, 0u};
-      if (row < left) {
-        kx[n] = *reinterpret_cast<const u32x4*>(kp + row * a.ks[2] + 16 * ch);
-        vx[n] = *reinterpret_cast<const u32x4*>(vp + row * a.vs[2] + 16 * ch);
-      }
-    }
-  };
-  auto store = [&](int buf) {
+  for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
-    for (int n = 0; n < LOADS; ++n) {
-      const uint32_t p = n * THREADS + tid, at = tile_offset<HD>(p / CH, p % CH);
-      *reinterpret_cast<u32x4*>(&lds[buf][0][at]) = kx[n];
-      *reinterpret_cast<u32x4*>(&lds[buf][1][at]) = vx[n];
-    }
-  };
+    for (int ds = 0; ds < NDS; ++ds) asm volatile("" : "+v"(qr[qt][ds]));
 
-  load(begin);
-  store(0);
-  __syncthreads();
-  for (int tile = begin; tile < end; ++tile) {
-    const int buf = (tile - begin) & 1;
-    if (tile + 1 < end) load(tile + 1);
-    const char* kt = lds[buf][0];
-    const char* vt = lds[buf][1];
+  auto step = [&](int tile, const int slot) __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+    lds_barrier();
+    if (tile + 1 < end) load(tile + 1, slot ^ 1);
+    const char* kt = lds[slot][0];
+    const char* vt = lds[slot][1];
     f32x4 sc[QT][4];  // [qt][tt][r]: key 16 tt + 4 g + r, row 16 qt + l16
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt)
@@ -475,8 +588,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void tile_kernel(TreeArgs a) {
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) o[qt][dt] = mfma16<BF16>(vf, pb[qt][hh], o[qt][dt]);
       }
-    if (tile + 1 < end) store(buf ^ 1);
-    __syncthreads();
+  };
+  // (a slot's LDS addresses are constants of its own copy of the step)
+  for (int tile = begin; tile < end; tile += 2) {
+    step(tile, 0);
+    if (tile + 1 < end) step(tile + 1, 1);
   }
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
@@ -484,7 +600,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void tile_kernel(TreeArgs a) {
     l[qt] += shfl_xor_f32(l[qt], 32);
     const int row = row0 + 16 * qt + l16;
     if (row >= a.R) continue;
-    const int64_t x = (static_cast<int64_t>(unit) * a.R + row) * a.splits + split;
+    const int64_t x = (static_cast<int64_t>(wg) + b * a.Hkv + hk) * a.R + row;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
       *reinterpret_cast<f32x4*>(a.po + x * HD + 16 * dt + 4 * g) = o[qt][dt];
@@ -493,13 +609,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void tile_kernel(TreeArgs a) {
       a.pl[x] = l[qt];
     }
   }
+  });
 }
 
 struct JoinArgs {
   TreeArgs t;
   const int32_t* parents;
   int64_t parents_ld;  // 0: one tree for all
-  int32_t H, unit_keys, round;  // of the splits (see split_steps)
+  int32_t H;
   int64_t rows;                 // B * H * T
   char* out;
   int64_t os[3];  // bytes
@@ -528,12 +645,14 @@ __device__ __forceinline__ void load8(const char* p, float* x) {
 }
 
 // One wave per row; groups of D / 8 lanes, each lane eight of the row's values. A group
-// takes every G-th partial and every G-th ancestor.
-template <cab_dtype_t DT, int HD>
+// takes every G-th partial and every G-th ancestor. KEYS: of the context's pieces.
+template <cab_dtype_t DT, int HD, int KEYS>
 __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
   constexpr int LG = HD / 8, G = 64 / LG, ES = DT == CAB_F32 ? 4 : 2;
   __shared__ int16_t list[4][MAX_NODES];
-  const int w = threadIdx.x >> 6, lane = lane_id(), grp = lane / LG, at = lane % LG;
+  __shared__ int32_t above[4][MAX_NODES];
+  const int w = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const int lane = lane_id(), grp = lane / LG, at = lane % LG;
   const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + w;
   if (id >= a.rows) return;  // (waves work apart from each other)
   const TreeArgs& ta = a.t;
@@ -541,16 +660,19 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
   const int64_t bh = id / ta.T;
   const int b = static_cast<int>(bh / a.H), h = static_cast<int>(bh - static_cast<int64_t>(b) * a.H);
   const int hk = h / ta.group;
-  const int len = context_length(ta.lengths, ta.length0, ta.most, b);
-
   // The row's line: the node and its ancestors. A node that ends nowhere is absent.
+  const Lengths lens(ta);
+  float q[8];
+  load8<DT>(ta.q + b * ta.qs[0] + h * ta.qs[1] + node * ta.qs[2] + at * 8 * ES, q);
   const int32_t* parents = a.parents + b * a.parents_ld;
+  for (int x = lane; x <= node; x += 64) above[w][x] = parents[x];
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   int n = 0, i = node;
   bool present = true;
   for (;;) {
     if (lane == 0) list[w][n] = static_cast<int16_t>(i);
     ++n;
-    const int p = parents[i];
+    const int p = above[w][i];
     if (p < 0 || p >= i) {
       present = p == -1;
       break;
@@ -561,17 +683,28 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
   float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   float l = 0.f, m = M_EMPTY;
   if (present) {
-    const int splits = live_splits(len, a.unit_keys, ta.splits, a.round);
-    const int64_t row = ((static_cast<int64_t>(b) * ta.Hkv + hk) * ta.R +
-                         (h - hk * ta.group) * ta.T + node) * ta.splits;
-    for (int x = lane; x < splits; x += 64) m = fmaxf(m, ta.pm[row + x]);
+    const Cut cut = list_cut<KEYS>(ta, lens);
+    int before = 0, len = 0;  // the sequences' shares of the list before b; b's context
+    for (int b0 = 0; b0 <= b; b0 += 64) {
+      const int mine = lens.mine(b0);
+      before += wave_sum(b0 + lane < b ? round_to(pieces_of<KEYS>(mine), cut.grain) : 0);
+      len = __builtin_amdgcn_readlane(mine, b & 63);  // (the last round's)
+    }
+    // The unit's partials: of the workgroups whose stretches meet its pieces.
+    const int pieces = pieces_of<KEYS>(len);
+    const int start = before * ta.Hkv + hk * round_to(pieces, cut.grain), first = start / cut.per;
+    const int parts = pieces ? (start + pieces - 1) / cut.per - first + 1 : 0;
+    const int64_t row = (static_cast<int64_t>(first) + b * ta.Hkv + hk) * ta.R +
+                        (h - hk * ta.group) * ta.T + node;
+    for (int x = lane; x < parts; x += 64) m = fmaxf(m, ta.pm[row + static_cast<int64_t>(x) * ta.R]);
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, shfl_xor_f32(m, off));
 #pragma unroll 4
-    for (int x = grp; x < splits; x += G) {
-      const float f = __builtin_amdgcn_exp2f(ta.pm[row + x] - m);
-      l += ta.pl[row + x] * f;
-      const f32x4* po = reinterpret_cast<const f32x4*>(ta.po + (row + x) * HD) + 2 * at;
+    for (int x = grp; x < parts; x += G) {
+      const int64_t y = row + static_cast<int64_t>(x) * ta.R;
+      const float f = __builtin_amdgcn_exp2f(ta.pm[y] - m);
+      l += ta.pl[y] * f;
+      const f32x4* po = reinterpret_cast<const f32x4*>(ta.po + y * HD) + 2 * at;
       const f32x4 y0 = po[0], y1 = po[1];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -579,8 +712,6 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
         o[4 + e] += y1[e] * f;
       }
     }
-    float q[8];
-    load8<DT>(ta.q + b * ta.qs[0] + h * ta.qs[1] + node * ta.qs[2] + at * 8 * ES, q);
     const char* kp = ta.k + b * ta.ks[0] + hk * ta.ks[1] + len * ta.ks[2] + at * 8 * ES;
     const char* vp = ta.v + b * ta.vs[0] + hk * ta.vs[1] + len * ta.vs[2] + at * 8 * ES;
     constexpr int U = 4;
@@ -650,12 +781,21 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
 
 // How a problem is cut. tile: rows of a tile_kernel workgroup (0: rows_kernel).
 struct TreePlan {
-  int64_t units, R, splits, row_tiles;
+  int64_t units, R, row_tiles, wgs, least;
   int tile;
   size_t off_pm, off_pl, bytes;
 };
 
-constexpr int FEW_ROWS = 32;
+// Rows per unit up to which rows_kernel runs, and those beyond which it does for long
+// lists only (keys of all units' longest contexts). 32 heads on 8, D = 128, bf16, us, here ->
+// tile_kernel: 4 rows, 16 sequences of 32768 keys 198 -> 228; 32 rows, 8184 keys 22.9 ->
+// 19.7, but 16 sequences of 32768 keys 208 -> 238, and 20 rows, 8 of 16384 65 -> 72.
+constexpr int FEW_ROWS = 32, FEWER_ROWS = 16;
+constexpr int64_t LONG_LIST = int64_t{1} << 18;
+// Workgroups that share the list: one a CU (rows_kernel; 512: 4 rows, 16 x 32768 keys 202 us
+// against 198, fp32, 256 rows of 4032 keys 84 against 70), or as many as the registers
+// allow: one of 8 waves, two of 4 (256: 64 rows, 8 x 8192 keys 54 us against 49).
+constexpr int WGS = 256, SMALL_TILE_WGS = 512;
 
 TreePlan tree_plan(cab_dtype_t dtype, int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t N,
                    int64_t D) {
@@ -663,22 +803,28 @@ TreePlan tree_plan(cab_dtype_t dtype, int64_t B, int64_t H, int64_t Hkv, int64_t
   p.units = B * Hkv;
   p.R = H / Hkv * T;
   const int64_t most = N > T ? N - T : 0;
-  if (p.R <= FEW_ROWS || dtype == CAB_F32) {
+  int64_t slots = WGS;
+  int keys;
+  if (dtype == CAB_F32 || p.R <= FEWER_ROWS || (p.R <= FEW_ROWS && p.units * most > LONG_LIST)) {
     p.tile = 0;
     p.row_tiles = ceil_div(p.R, p.R <= 16 ? 16 : 32);
-    const int64_t want = ceil_div(1024, p.units * p.row_tiles);
-    p.splits = want < MAX_SPLITS ? want : MAX_SPLITS;
-    const int64_t steps = ceil_div(ceil_div(most, STEP), 4);  // four waves' steps
-    if (p.splits > steps) p.splits = steps < 1 ? 1 : steps;
+    p.least = 1;
+    keys = QUAD;
   } else {
     p.tile = p.R <= 64 ? 64 : p.R <= 128 ? 128 : 256;
     p.row_tiles = ceil_div(p.R, p.tile);
-    const int64_t want = ceil_div(p.tile == 256 ? 256 : 512, p.units * p.row_tiles);
-    p.splits = want < MAX_SPLITS ? want : MAX_SPLITS;
-    const int64_t tiles = ceil_div(most, TILE);
-    if (p.splits > tiles) p.splits = tiles < 1 ? 1 : tiles;
+    // (two tiles a workgroup at least; four of the small ones at D = 128: 64 rows of 8176
+    // keys 19.9 us against 22.1, 128 rows 25.1 against 29.0)
+    p.least = p.tile < 256 && D == 128 ? 4 : 2;
+    if (p.tile < 256) slots = SMALL_TILE_WGS;
+    keys = TILE;
   }
-  const int64_t parts = p.units * p.R * p.splits;
+  // No more workgroups than the longest contexts have stretches.
+  const int64_t list = p.units * ceil_div(most, keys);
+  p.wgs = ceil_div(slots, p.row_tiles);
+  if (p.wgs > ceil_div(list, p.least)) p.wgs = ceil_div(list, p.least);
+  if (p.wgs < 1) p.wgs = 1;
+  const int64_t parts = (p.wgs + p.units) * p.R;
   p.off_pm = static_cast<size_t>(parts * D) * 4;
   p.off_pl = p.off_pm + static_cast<size_t>(round_up(parts, 4)) * 4;
   p.bytes = p.off_pl + static_cast<size_t>(round_up(parts, 4)) * 4;
@@ -686,33 +832,36 @@ TreePlan tree_plan(cab_dtype_t dtype, int64_t B, int64_t H, int64_t Hkv, int64_t
 }
 
 bool tree_sizes(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t N, int64_t D) {
+  // (the list of pieces, and where a stretch begins, fit 32 bits)
   return B >= 1 && Hkv >= 1 && H >= Hkv && H % Hkv == 0 && T >= 1 && T <= MAX_NODES && N >= T &&
          N <= INT32_MAX - 1024 && (D == 64 || D == 128) && H <= 65535 && B <= 65535 &&
-         B * Hkv <= 65535 && H / Hkv * T <= 65535;
+         B * Hkv <= INT32_MAX / 2 / ceil_div(N, TILE) && H / Hkv * T <= 65535;
 }
 
 template <cab_dtype_t DT, int HD>
 void launch(const TreePlan& pl, const JoinArgs& j, hipStream_t s) {
   const TreeArgs& a = j.t;
-  const unsigned units = static_cast<unsigned>(pl.units), splits = static_cast<unsigned>(pl.splits);
-  if (a.most > 0) {
-    const dim3 grid(splits, units, static_cast<unsigned>(pl.row_tiles));
-    const unsigned wgs = static_cast<unsigned>(pl.units * pl.splits * pl.row_tiles);
-    if (pl.tile == 0) {
+  const unsigned wgs = static_cast<unsigned>(pl.wgs), tiles = static_cast<unsigned>(pl.row_tiles);
+  const unsigned join = static_cast<unsigned>(ceil_div(j.rows, 4));
+  if (pl.tile == 0) {
+    if (a.most > 0) {
       if (pl.R <= 16)
-        rows_kernel<DT, HD, 1><<<grid, 256, 0, s>>>(a);
+        rows_kernel<DT, HD, 1><<<dim3(wgs, tiles), 256, 0, s>>>(a);
       else
-        rows_kernel<DT, HD, 2><<<grid, 256, 0, s>>>(a);
-    } else if constexpr (DT != CAB_F32) {
-      if (pl.tile == 64)
-        tile_kernel<DT, HD, 1, 4><<<wgs, 256, 0, s>>>(a);
-      else if (pl.tile == 128)
-        tile_kernel<DT, HD, 2, 4><<<wgs, 256, 0, s>>>(a);
-      else
-        tile_kernel<DT, HD, 2, 8><<<wgs, 512, 0, s>>>(a);
+        rows_kernel<DT, HD, 2><<<dim3(wgs, tiles), 256, 0, s>>>(a);
     }
+    join_kernel<DT, HD, QUAD><<<join, 256, 0, s>>>(j);
+  } else if constexpr (DT != CAB_F32) {
+    if (a.most > 0) {
+      if (pl.tile == 64)
+        tile_kernel<DT, HD, 1, 4><<<wgs * tiles, 256, 0, s>>>(a);
+      else if (pl.tile == 128)
+        tile_kernel<DT, HD, 2, 4><<<wgs * tiles, 256, 0, s>>>(a);
+      else
+        tile_kernel<DT, HD, 2, 8><<<wgs * tiles, 512, 0, s>>>(a);
+    }
+    join_kernel<DT, HD, TILE><<<join, 256, 0, s>>>(j);
   }
-  join_kernel<DT, HD><<<static_cast<unsigned>(ceil_div(j.rows, 4)), 256, 0, s>>>(j);
 }
 
 }  // namespace
@@ -766,7 +915,6 @@ extern "C" cab_status_t cab_tree_attn_fwd(
   const TreePlan pl = tree_plan(dtype, B, H, H_kv, T, N, D);
   CAB_REQUIRE(workspace && workspace_bytes >= pl.bytes && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
               CAB_EWORKSPACE, "%s: workspace needs %zu bytes, 16-byte aligned", fn, pl.bytes);
-  CAB_REQUIRE(pl.units * pl.splits * pl.row_tiles <= INT32_MAX, CAB_ESHAPE, "%s: problem too large", fn);
   JoinArgs j;
   TreeArgs& a = j.t;
   a.q = static_cast<const char*>(q);
@@ -785,7 +933,9 @@ extern "C" cab_status_t cab_tree_attn_fwd(
   a.group = static_cast<int32_t>(H / H_kv);
   a.T = static_cast<int32_t>(T);
   a.R = static_cast<int32_t>(pl.R);
-  a.splits = static_cast<int32_t>(pl.splits);
+  a.B = static_cast<int32_t>(B);
+  a.wgs = static_cast<int32_t>(pl.wgs);
+  a.least = static_cast<int32_t>(pl.least);
   a.row_tiles = static_cast<int32_t>(pl.row_tiles);
   a.c = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
   char* ws = static_cast<char*>(workspace);
@@ -795,8 +945,6 @@ extern "C" cab_status_t cab_tree_attn_fwd(
   j.parents = parents;
   j.parents_ld = parents_stride;
   j.H = static_cast<int32_t>(H);
-  j.unit_keys = pl.tile ? TILE : STEP;
-  j.round = pl.tile ? 1 : 4;
   j.rows = B * H * T;
   j.out = static_cast<char*>(out);
   j.lse = lse;

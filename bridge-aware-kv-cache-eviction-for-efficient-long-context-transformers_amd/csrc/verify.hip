@@ -15,15 +15,22 @@
 // the residual w; with noise ~ Exp(1) that is a sample of w / sum w. It needs no
 // cumulative sum (whose order would decide between tokens) and no normaliser.
 //
-// Only the rows of accepted nodes are read. One workgroup of 16 waves walks a
-// sequence's tree.
+// One walk needs the rows of the accepted nodes, one after another. Two ways:
+//  - walk_kernel<.., false>: one workgroup of 16 waves a sequence reads just those
+//    rows. A row takes a CU about 8 us per 100000 values (the exponentials), whatever
+//    the batch up to the chip's 256 CUs.
+//  - where the logits are few enough, stats_kernel first takes the maximum and sum (or the
+//    argmax) of every row that has children, spread over the chip; walk_kernel<.., true>
+//    then decides from these alone, and pick_kernel draws the next token, several
+//    workgroups a sequence.
 #include "cab_internal.h"
 
 namespace cab {
 namespace {
 
 constexpr int MAX_NODES = 256;
-constexpr int THREADS = 1024, WAVES = THREADS / 64;
+constexpr int WALK_THREADS = 1024;  // of a walk that reads rows
+constexpr int SLICE_THREADS = 256;  // of stats_kernel, pick_kernel and a walk that reads none
 enum { GREEDY = 0, POINT = 1, DRAFT = 2 };
 
 // 16 bytes at any element's alignment (global loads need none on gfx950).
@@ -43,6 +50,41 @@ struct VerifyArgs {
   int32_t* path;
   int32_t* counts;
   int64_t* next;
+  // With rows' statistics (see VerifyPlan):
+  struct RowStats* stats;    // [logits, drafts][row][slices]
+  struct WalkEnd* ends;      // [B]
+  struct Candidate* picks;   // [B][picks of a row]
+  int32_t slices, slice;     // slices of a row in stats_kernel, their values
+  int32_t pick_slices, pick_slice;
+  int64_t rows;              // B * T
+};
+
+// A slice of a row: its maximum (at least the lowest float) and sum of weights, or
+// (greedy) the order_key of its argmax.
+struct RowStats {
+  union {
+    double s;
+    unsigned long long key;
+  };
+  float m, unused;
+};
+
+// Where a sequence's walk ended, for pick_kernel.
+struct WalkEnd {
+  double ip, iq, used;  // 1 / sums of weights; a
+  float m, mq;
+  int32_t node, n_gone;
+  uint32_t done;  // pick_kernel's workgroups that are through
+  uint32_t unused;
+  int32_t gone[MAX_NODES];
+};
+
+// The best of a slice: scores of weights relative to m; from the residual, and from
+// the whole row for when nothing is left of it.
+struct Candidate {
+  float m, score[2];
+  int32_t index[2];
+  int32_t unused[3];
 };
 
 template <cab_dtype_t DT>
@@ -91,13 +133,16 @@ __device__ __forceinline__ double residual(float ep, double ip, float eq, double
   return fmax(p - q, 0.0);
 }
 
+template <int THREADS>
 struct Scratch {
+  static constexpr int WAVES = THREADS / 64;
   float m[WAVES];
   double s[WAVES];
   unsigned long long key[WAVES];
 };
 
-__device__ __forceinline__ double block_sum(double v, Scratch& sh) {
+template <int THREADS>
+__device__ __forceinline__ double block_sum(double v, Scratch<THREADS>& sh) {
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) v += shfl_xor_f64(v, off);
   __syncthreads();
@@ -105,11 +150,12 @@ __device__ __forceinline__ double block_sum(double v, Scratch& sh) {
   __syncthreads();
   v = 0.0;
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) v += sh.s[w];
+  for (int w = 0; w < THREADS / 64; ++w) v += sh.s[w];
   return v;
 }
 
-__device__ __forceinline__ unsigned long long block_max(unsigned long long k, Scratch& sh) {
+template <int THREADS>
+__device__ __forceinline__ unsigned long long block_max(unsigned long long k, Scratch<THREADS>& sh) {
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) {
     const unsigned long long o = __shfl_xor(k, off, 64);
@@ -120,8 +166,19 @@ __device__ __forceinline__ unsigned long long block_max(unsigned long long k, Sc
   __syncthreads();
   k = 0;
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) k = sh.key[w] > k ? sh.key[w] : k;
+  for (int w = 0; w < THREADS / 64; ++w) k = sh.key[w] > k ? sh.key[w] : k;
   return k;
+}
+
+// Which of N values from `at` on are among n indexes.
+template <int N>
+__device__ __forceinline__ uint32_t gone_mask(const int32_t* gone, int n, int at) {
+  uint32_t mask = 0;
+  for (int k = 0; k < n; ++k) {
+    const uint32_t d = static_cast<uint32_t>(gone[k] - at);
+    if (d < static_cast<uint32_t>(N)) mask |= 1u << d;
+  }
+  return mask;
 }
 
 // Order of floats as unsigned numbers, and the lower of equal ones' indexes first.
@@ -134,9 +191,9 @@ __device__ __forceinline__ int key_index(unsigned long long k) {
   return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k));
 }
 
-// f(first index, number, values...) over a row's 16-byte chunks, U of them loaded at
-// a time, then its last values one by one.
-template <cab_dtype_t DT, int U, typename F>
+// f(first index, values, how many) over the 16-byte chunks of V values, U of them loaded
+// at a time, then the last values one by one.
+template <cab_dtype_t DT, int U, int THREADS, typename F>
 __device__ __forceinline__ void over_row(const char* row, int V, F f) {
   constexpr int N = Chunk<DT>::N;
   const int n = V / N;
@@ -161,12 +218,15 @@ __device__ __forceinline__ void over_row(const char* row, int V, F f) {
   }
 }
 
-// Maximum (at least the lowest float) and sum of weights of a row.
-template <cab_dtype_t DT>
-__device__ void row_softmax(const char* row, const VerifyArgs& a, Scratch& sh, float& m, double& s) {
+// Maximum (at least the lowest float) and sum of weights of a row. The sum's terms
+// take the exponent in one product: those that count in it are near the maximum,
+// where that is as exact as weight().
+template <cab_dtype_t DT, int THREADS>
+__device__ void row_softmax(const char* row, int V, const VerifyArgs& a, Scratch<THREADS>& sh, float& m,
+                            double& s) {
   float mt = -__FLT_MAX__;
   double st = 0.0;
-  over_row<DT, 4>(row, a.V, [&](int, const float* v, auto n) {
+  over_row<DT, 4, THREADS>(row, V, [&](int, const float* v, auto n) {
     constexpr int N = decltype(n)::value;
     float hi = v[0];
 #pragma unroll
@@ -176,8 +236,14 @@ __device__ void row_softmax(const char* row, const VerifyArgs& a, Scratch& sh, f
       mt = hi;
     }
     float sum = 0.f;
+    if (mt < INFINITY) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) sum += weight(v[i], mt, a);
+      for (int i = 0; i < N; ++i)
+        sum += __builtin_amdgcn_exp2f(fmaxf(v[i] - mt, a.d_min) * a.c_hi);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) sum += v[i] == mt ? 1.f : 0.f;
+    }
     st += sum;
   });
   float mw = mt;
@@ -188,40 +254,107 @@ __device__ void row_softmax(const char* row, const VerifyArgs& a, Scratch& sh, f
   __syncthreads();
   m = sh.m[0];
 #pragma unroll
-  for (int w = 1; w < WAVES; ++w) m = fmaxf(m, sh.m[w]);
-  s = block_sum(st * weight(mt, m, a), sh);
+  for (int w = 1; w < THREADS / 64; ++w) m = fmaxf(m, sh.m[w]);
+  s = block_sum<THREADS>(st * weight(mt, m, a), sh);
 }
 
-// The row's largest value (NaN below all) and its lowest index; -1 if there is none.
-template <cab_dtype_t DT>
-__device__ int row_argmax(const char* row, const VerifyArgs& a, Scratch& sh) {
-  unsigned long long key = 0;
-  over_row<DT, 4>(row, a.V, [&](int at, const float* v, auto n) {
+// order_key of the largest value (NaN below all) and its lowest index; 0 if there is none.
+template <cab_dtype_t DT, int THREADS>
+__device__ unsigned long long row_argmax(const char* row, int V, Scratch<THREADS>& sh) {
+  float best = -INFINITY;
+  int index = -1;
+  over_row<DT, 4, THREADS>(row, V, [&](int at, const float* v, auto n) {
 #pragma unroll
-    for (int i = 0; i < decltype(n)::value; ++i) {
-      const unsigned long long k = order_key(v[i], at + i);
-      if (v[i] > -INFINITY && k > key) key = k;
-    }
+    for (int i = 0; i < decltype(n)::value; ++i)
+      if (v[i] > best) {  // (indexes ascend within a thread)
+        best = v[i];
+        index = at + i;
+      }
   });
-  key = block_max(key, sh);
-  return key ? key_index(key) : -1;
+  return block_max<THREADS>(index >= 0 ? order_key(best, index) : 0, sh);
 }
 
+// Grid: slices of rows, row-major; blockIdx.y: logits, or the drafts'.
 template <cab_dtype_t DT, int MODE>
-__global__ __launch_bounds__(THREADS) void verify_kernel(VerifyArgs a) {
+__global__ __launch_bounds__(SLICE_THREADS) void stats_kernel(VerifyArgs a) {
+  __shared__ Scratch<SLICE_THREADS> sh;
+  const int64_t row = blockIdx.x / a.slices;
+  const int slice = static_cast<int>(blockIdx.x - row * a.slices);
+  const int b = static_cast<int>(row / a.T), node = static_cast<int>(row - static_cast<int64_t>(b) * a.T);
+  // Rows without children decide nothing (greedy: any row may give the next token).
+  if constexpr (MODE != GREEDY) {
+    const int i = threadIdx.x;  // (as many threads as a tree has nodes at most)
+    const int mine = i > node && i < a.T && a.parents[b * a.parents_ld + i] == node;
+    if (!__syncthreads_or(mine)) return;
+  }
+  constexpr int ES = DT == CAB_F32 ? 4 : 2;
+  const char* p = blockIdx.y ? a.drafts + b * a.ds[0] + node * a.ds[1] : a.logits + b * a.ls[0] + node * a.ls[1];
+  const int from = slice * a.slice, n = min(a.slice, a.V - from);
+  p += static_cast<int64_t>(from) * ES;
+  RowStats r;
+  if constexpr (MODE == GREEDY) {
+    r.key = row_argmax<DT, SLICE_THREADS>(p, n, sh);
+    if (r.key) r.key -= static_cast<uint32_t>(from);  // (indexes are stored downwards)
+    r.m = 0.f;
+  } else {
+    row_softmax<DT, SLICE_THREADS>(p, n, a, sh, r.m, r.s);
+  }
+  r.unused = 0.f;
+  if (threadIdx.x == 0) a.stats[(blockIdx.y * a.rows + row) * a.slices + slice] = r;
+}
+
+// A row's statistics from its slices' (at most 64), in every lane.
+__device__ __forceinline__ void merge_softmax(const RowStats* st, const VerifyArgs& a, float& m, double& s) {
+  const int lane = lane_id();
+  float ml = -__FLT_MAX__;
+  double sl = 0.0;
+  if (lane < a.slices) {
+    ml = st[lane].m;
+    sl = st[lane].s;
+  }
+  m = ml;
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, shfl_xor_f32(m, off));
+  s = sl * weight(ml, m, a);
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) s += shfl_xor_f64(s, off);
+}
+__device__ __forceinline__ unsigned long long merge_argmax(const RowStats* st, const VerifyArgs& a) {
+  unsigned long long key = lane_id() < a.slices ? st[lane_id()].key : 0;
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    const unsigned long long o = __shfl_xor(key, off, 64);
+    key = o > key ? o : key;
+  }
+  return key;
+}
+
+// STATS: rows' statistics are there, and where the walk ended is left for pick_kernel.
+template <cab_dtype_t DT, int MODE, bool STATS, int THREADS>
+__global__ __launch_bounds__(THREADS) void walk_kernel(VerifyArgs a) {
   __shared__ int32_t parent[MAX_NODES], token[MAX_NODES], out[MAX_NODES], gone[MAX_NODES];
-  __shared__ float uniform[MODE == GREEDY ? 1 : MAX_NODES];
-  __shared__ Scratch sh;
+  // Each draft's uniform number, and its logit in its parent's row (and the draft's).
+  __shared__ float uniform[MAX_NODES], value[MAX_NODES], drawn[MODE == DRAFT ? MAX_NODES : 1];
+  __shared__ Scratch<THREADS> sh;
   const int b = blockIdx.x, tid = threadIdx.x, lane = lane_id();
+  const char* logits = a.logits + b * a.ls[0];
+  const char* drafts = MODE == DRAFT ? a.drafts + b * a.ds[0] : nullptr;
   for (int i = tid; i < MAX_NODES; i += THREADS) {
     out[i] = -1;
     parent[i] = -1;  // (nodes 0 and past T are nobody's children)
     if (i > 0 && i < a.T) {
       const int32_t p = a.parents[b * a.parents_ld + i];
       const int64_t x = a.tokens[static_cast<int64_t>(b) * a.T + i];
+      const bool in = x >= 0 && x < a.V;
       parent[i] = p < i ? p : -1;
-      token[i] = x >= 0 && x < a.V ? static_cast<int32_t>(x) : -1;  // -1: never accepted
-      if constexpr (MODE != GREEDY) uniform[i] = a.uniforms[static_cast<int64_t>(b) * a.T + i];
+      token[i] = in ? static_cast<int32_t>(x) : -1;  // -1: passed over
+      if constexpr (MODE != GREEDY) {
+        uniform[i] = a.uniforms[static_cast<int64_t>(b) * a.T + i];
+        if (in && p >= 0 && p < i) {
+          value[i] = value_at<DT>(logits + p * a.ls[1], static_cast<int>(x));
+          if constexpr (MODE == DRAFT) drawn[i] = value_at<DT>(drafts + p * a.ds[1], static_cast<int>(x));
+        }
+      }
     }
   }
   __syncthreads();
@@ -234,6 +367,14 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(VerifyArgs a) {
     }
     return -1;
   };
+  const RowStats* stats = nullptr;
+  if constexpr (STATS) stats = a.stats + static_cast<int64_t>(b) * a.T * a.slices;
+  auto softmax_of = [&](bool drafted, int node, const char* row, float& m, double& s) {
+    if constexpr (STATS)
+      merge_softmax(stats + ((drafted ? a.rows : 0) + node) * a.slices, a, m, s);
+    else
+      row_softmax<DT, THREADS>(row, a.V, a, sh, m, s);
+  };
   const char* lrow;
   const char* qrow = nullptr;
   float m = 0.f, mq = 0.f;
@@ -242,16 +383,19 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(VerifyArgs a) {
   for (;;) {
     if (tid == 0) out[count] = node;
     ++count;
-    lrow = a.logits + b * a.ls[0] + node * a.ls[1];
+    lrow = logits + node * a.ls[1];
     int taken = -1;
+    const int first = next_child(node, node);
     if constexpr (MODE == GREEDY) {
-      best = row_argmax<DT>(lrow, a, sh);
-      for (int i = next_child(node, node); i >= 0 && taken < 0; i = next_child(node, i))
+      const unsigned long long key =
+          STATS ? merge_argmax(stats + static_cast<int64_t>(node) * a.slices, a) : row_argmax<DT, THREADS>(lrow, a.V, sh);
+      best = key ? key_index(key) : -1;
+      for (int i = first; i >= 0 && taken < 0; i = next_child(node, i))
         if (token[i] >= 0 && token[i] == best) taken = i;
     } else if constexpr (MODE == POINT) {
-      row_softmax<DT>(lrow, a, sh, m, s);
+      if (first >= 0 || !STATS) softmax_of(false, node, lrow, m, s);
       left = s;
-      for (int i = next_child(node, node); i >= 0 && taken < 0; i = next_child(node, i)) {
+      for (int i = first; i >= 0 && taken < 0; i = next_child(node, i)) {
         const int x = token[i];
         if (x < 0) continue;
         bool before = false;  // an earlier sibling's token: its weight is gone
@@ -260,27 +404,30 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(VerifyArgs a) {
           before = before || ballot64(j < i && parent[j] == node && token[j] == x) != 0;
         }
         if (before) continue;
-        const float e = weight(value_at<DT>(lrow, x), m, a);
+        const float e = weight(value[i], m, a);
         if (static_cast<double>(uniform[i]) * left < static_cast<double>(e))
           taken = i;
         else
           left = fmax(left - static_cast<double>(e), 0.0);
       }
     } else {
-      double sq;
-      qrow = a.drafts + b * a.ds[0] + node * a.ds[1];
-      row_softmax<DT>(lrow, a, sh, m, s);
-      row_softmax<DT>(qrow, a, sh, mq, sq);
-      ip = s > 0.0 ? 1.0 / s : 0.0;
-      iq = sq > 0.0 ? 1.0 / sq : 0.0;
+      qrow = drafts + node * a.ds[1];
       left = 1.0;
       used = 0.0;
+      if (first >= 0 || !STATS) {
+        double sq;
+        softmax_of(false, node, lrow, m, s);
+        softmax_of(true, node, qrow, mq, sq);
+        ip = s > 0.0 ? 1.0 / s : 0.0;
+        iq = sq > 0.0 ? 1.0 / sq : 0.0;
+      }
       bool known = true;  // left is the residual's sum
-      for (int i = next_child(node, node); i >= 0 && taken < 0; i = next_child(node, i)) {
+      for (int i = first; i >= 0 && taken < 0; i = next_child(node, i)) {
+        if (token[i] < 0) continue;
         if (!known) {
           double c = 0.0;
           const double uq = used * iq;
-          over_row<DT, 2>(lrow, a.V, [&](int at, const float* v, auto n) {
+          over_row<DT, 2, THREADS>(lrow, a.V, [&](int at, const float* v, auto n) {
 #pragma unroll
             for (int k = 0; k < decltype(n)::value; ++k) {
               const float ep = weight(v[k], m, a);
@@ -288,13 +435,11 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(VerifyArgs a) {
               c += residual(ep, ip, eq, uq);
             }
           });
-          left = block_sum(c, sh);
+          left = block_sum<THREADS>(c, sh);
           known = true;
         }
-        const int x = token[i];
-        if (x < 0) continue;
-        const float ep = weight(value_at<DT>(lrow, x), m, a);
-        const float eq = weight(value_at<DT>(qrow, x), mq, a);
+        const float ep = weight(value[i], m, a);
+        const float eq = weight(drawn[i], mq, a);
         if (static_cast<double>(uniform[i]) * left * (eq * iq) < residual(ep, ip, eq, used * iq)) {
           taken = i;
         } else {
@@ -307,27 +452,40 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(VerifyArgs a) {
     node = taken;
   }
 
-  int64_t chosen = best;
-  if constexpr (MODE != GREEDY) {
-    // The rejected tokens: all the children's.
-    int n_gone = 0;
-    for (int i = next_child(node, node); MODE == POINT && i >= 0; i = next_child(node, i)) {
+  // The rejected tokens: all the children's.
+  int n_gone = 0;
+  if constexpr (MODE == POINT)
+    for (int i = next_child(node, node); i >= 0; i = next_child(node, i)) {
       if (tid == 0) gone[n_gone] = token[i];
       ++n_gone;
     }
-    __syncthreads();
+  __syncthreads();
+  for (int i = tid; i < a.T; i += THREADS) a.path[static_cast<int64_t>(b) * a.T + i] = out[i];
+  if (tid == 0) a.counts[b] = count;
+  if constexpr (MODE == GREEDY) {
+    if (tid == 0) a.next[b] = best;
+  } else if constexpr (STATS) {
+    WalkEnd& e = a.ends[b];
+    for (int i = tid; i < n_gone; i += THREADS) e.gone[i] = gone[i];
+    if (tid == 0) {
+      e.ip = ip;
+      e.iq = iq;
+      e.used = used;
+      e.m = m;
+      e.mq = mq;
+      e.node = node;
+      e.n_gone = n_gone;
+      e.done = 0;
+    }
+  } else {
     const float* noise = a.noise + static_cast<int64_t>(b) * a.V;
     double uq = used * iq;
     unsigned long long key = 0;
     // The second time over the whole row's weights, if nothing is left of them.
     for (int pass = 0; pass < 2 && key == 0; ++pass) {
-      over_row<DT, 2>(lrow, a.V, [&](int at, const float* v, auto n) {
+      over_row<DT, 2, THREADS>(lrow, a.V, [&](int at, const float* v, auto n) {
         constexpr int N = decltype(n)::value;
-        uint32_t out_of = 0;
-        for (int k = 0; k < n_gone; ++k) {
-          const uint32_t d = static_cast<uint32_t>(gone[k] - at);
-          if (d < static_cast<uint32_t>(N)) out_of |= 1u << d;
-        }
+        const uint32_t out_of = gone_mask<N>(gone, n_gone, at);
 #pragma unroll
         for (int k = 0; k < N; ++k) {
           float w = weight(v[k], m, a);
@@ -338,26 +496,166 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(VerifyArgs a) {
           if (w > 0.f && score >= 0.f && !(out_of >> k & 1) && o > key) key = o;
         }
       });
-      key = block_max(key, sh);
+      key = block_max<THREADS>(key, sh);
       uq = 0.0;
       n_gone = 0;
     }
-    chosen = key ? key_index(key) : -1;
-  }
-  __syncthreads();
-  for (int i = tid; i < a.T; i += THREADS) a.path[static_cast<int64_t>(b) * a.T + i] = out[i];
-  if (tid == 0) {
-    a.counts[b] = count;
-    a.next[b] = chosen;
+    if (tid == 0) a.next[b] = key ? key_index(key) : -1;
   }
 }
 
+// Grid: slices of a row, by sequence. Scores are relative to the slice's own maximum
+// where nothing was taken off the row (a leaf has no statistics), else to the row's.
+// The sequence's last workgroup compares the slices' candidates.
+template <cab_dtype_t DT, int MODE>
+__global__ __launch_bounds__(SLICE_THREADS) void pick_kernel(VerifyArgs a) {
+  constexpr int ES = DT == CAB_F32 ? 4 : 2;
+  __shared__ Scratch<SLICE_THREADS> sh;
+  __shared__ int32_t gone[MAX_NODES];
+  __shared__ bool last;
+  const int b = blockIdx.x / a.pick_slices, at_slice = blockIdx.x - b * a.pick_slices, tid = threadIdx.x;
+  WalkEnd& e = a.ends[b];
+  const int n_gone = e.n_gone;
+  if (tid < n_gone) gone[tid] = e.gone[tid];
+  const int from = at_slice * a.pick_slice, n = min(a.pick_slice, a.V - from);
+  const char* lrow = a.logits + b * a.ls[0] + e.node * a.ls[1] + static_cast<int64_t>(from) * ES;
+  const char* qrow = nullptr;
+  const bool whole = MODE == POINT || e.used == 0.0;
+  if constexpr (MODE == DRAFT) qrow = a.drafts + b * a.ds[0] + e.node * a.ds[1] + static_cast<int64_t>(from) * ES;
+  const float* noise = a.noise + static_cast<int64_t>(b) * a.V + from;
+  float m = e.m;
+  if (whole) {
+    float mt = -__FLT_MAX__;
+    over_row<DT, 4, SLICE_THREADS>(lrow, n, [&](int, const float* v, auto k) {
+#pragma unroll
+      for (int i = 0; i < decltype(k)::value; ++i) mt = fmaxf(mt, v[i]);
+    });
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) mt = fmaxf(mt, shfl_xor_f32(mt, off));
+    if (lane_id() == 0) sh.m[tid >> 6] = mt;
+    __syncthreads();
+    m = fmaxf(fmaxf(sh.m[0], sh.m[1]), fmaxf(sh.m[2], sh.m[3]));
+  }
+  __syncthreads();
+  const double ip = e.ip, uq = e.used * e.iq;
+  const float mq = e.mq;
+  unsigned long long key[2] = {0, 0};  // of the residual, of the row
+  over_row<DT, 2, SLICE_THREADS>(lrow, n, [&](int at, const float* v, auto nn) {
+    constexpr int N = decltype(nn)::value;
+    const uint32_t out_of = gone_mask<N>(gone, n_gone, from + at);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const float w = weight(v[k], m, a), rn = __builtin_amdgcn_rcpf(noise[at + k]);
+      const float score = w * rn;
+      const unsigned long long o = order_key(score, from + at + k);
+      const bool ok = w > 0.f && score >= 0.f;
+      if (ok && o > key[1]) key[1] = o;
+      if constexpr (MODE == DRAFT) {
+        if (!whole) {
+          const float r = static_cast<float>(residual(w, ip, weight(value_at<DT>(qrow, at + k), mq, a), uq));
+          const unsigned long long or_ = order_key(r * rn, from + at + k);
+          if (r > 0.f && r * rn >= 0.f && or_ > key[0]) key[0] = or_;
+        } else if (ok && o > key[0]) {
+          key[0] = o;
+        }
+      } else if (ok && !(out_of >> k & 1) && o > key[0]) {
+        key[0] = o;
+      }
+    }
+  });
+  Candidate c;
+  c.m = m;
+  for (int i = 0; i < 2; ++i) {
+    key[i] = block_max<SLICE_THREADS>(key[i], sh);
+    c.score[i] = __uint_as_float(static_cast<uint32_t>(key[i] >> 32) & 0x7fffffffu);
+    c.index[i] = key[i] ? key_index(key[i]) : -1;
+  }
+  if (tid == 0) {
+    a.picks[blockIdx.x] = c;
+    last = __hip_atomic_fetch_add(&e.done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) + 1 ==
+           static_cast<uint32_t>(a.pick_slices);
+  }
+  __syncthreads();
+  if (!last || tid >= 64) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  const Candidate* cs = a.picks + static_cast<int64_t>(b) * a.pick_slices;
+  float hi = -__FLT_MAX__;
+  for (int x = tid; x < a.pick_slices; x += 64) hi = fmaxf(hi, cs[x].m);
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) hi = fmaxf(hi, shfl_xor_f32(hi, off));
+  key[0] = key[1] = 0;
+  for (int x = tid; x < a.pick_slices; x += 64) {
+    const Candidate y = cs[x];
+    const float f = weight(y.m, hi, a);
+    for (int i = 0; i < 2; ++i) {
+      const unsigned long long o = order_key(y.score[i] * f, y.index[i]);
+      if (y.index[i] >= 0 && f > 0.f && o > key[i]) key[i] = o;
+    }
+  }
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) {
+      const unsigned long long o = __shfl_xor(key[i], off, 64);
+      key[i] = o > key[i] ? o : key[i];
+    }
+  if (tid == 0) a.next[b] = key[0] ? key_index(key[0]) : key[1] ? key_index(key[1]) : -1;
+}
+
+// How a call is run: the statistics' and candidates' slices and workspace.
+struct VerifyPlan {
+  bool stats;
+  int64_t slices, slice, pick_slices, pick_slice;
+  size_t off_ends, off_picks, bytes;
+};
+
+// Bytes of logits up to which all rows' statistics are taken.
+constexpr int64_t STATS_BYTES = int64_t{384} << 20;
+
+VerifyPlan verify_plan(cab_dtype_t dtype, int mode, int64_t B, int64_t T, int64_t V) {
+  VerifyPlan p = {};
+  const int64_t es = static_cast<int64_t>(dtype_size(dtype)), rows = B * T, sides = mode == DRAFT ? 2 : 1;
+  p.stats = rows * sides <= STATS_BYTES / (V * es);
+  if (!p.stats) return p;
+  // 16 KB slices: four 16-byte loads a thread.
+  const int64_t unit = SLICE_THREADS * 64 / es;
+  auto cut = [&](int64_t most, int64_t& n, int64_t& size) {
+    n = ceil_div(V, unit) < most ? ceil_div(V, unit) : most;
+    size = round_up(ceil_div(V, n), 16 / es);
+    n = ceil_div(V, size);
+  };
+  cut(64, p.slices, p.slice);
+  cut(64, p.pick_slices, p.pick_slice);
+  p.off_ends = static_cast<size_t>(sides * rows * p.slices) * sizeof(RowStats);
+  p.off_picks = p.off_ends + (mode == GREEDY ? 0 : static_cast<size_t>(B) * sizeof(WalkEnd));
+  p.bytes = p.off_picks + (mode == GREEDY ? 0 : static_cast<size_t>(B * p.pick_slices) * sizeof(Candidate));
+  return p;
+}
+
+bool verify_sizes(int64_t B, int64_t T, int64_t V) {
+  return T >= 1 && T <= MAX_NODES && B >= 1 && B <= INT32_MAX / T && V >= 1 && V <= INT32_MAX / 2;
+}
+
+template <cab_dtype_t DT, int MODE>
+void run(const VerifyPlan& p, const VerifyArgs& a, unsigned B, hipStream_t s) {
+  if (!p.stats) {
+    walk_kernel<DT, MODE, false, WALK_THREADS><<<B, WALK_THREADS, 0, s>>>(a);
+    return;
+  }
+  const dim3 grid(static_cast<unsigned>(a.rows * p.slices), MODE == DRAFT ? 2 : 1);
+  stats_kernel<DT, MODE><<<grid, SLICE_THREADS, 0, s>>>(a);
+  // (residuals' sums are rows read in the walk)
+  constexpr int THREADS = MODE == DRAFT ? WALK_THREADS : SLICE_THREADS;
+  walk_kernel<DT, MODE, true, THREADS><<<B, THREADS, 0, s>>>(a);
+  if constexpr (MODE != GREEDY)
+    pick_kernel<DT, MODE><<<static_cast<unsigned>(p.pick_slices) * B, SLICE_THREADS, 0, s>>>(a);
+}
+
 template <cab_dtype_t DT>
-void launch(const VerifyArgs& a, int mode, unsigned B, hipStream_t s) {
+void launch(const VerifyPlan& p, const VerifyArgs& a, int mode, unsigned B, hipStream_t s) {
   switch (mode) {
-    case GREEDY: verify_kernel<DT, GREEDY><<<B, THREADS, 0, s>>>(a); break;
-    case POINT: verify_kernel<DT, POINT><<<B, THREADS, 0, s>>>(a); break;
-    default: verify_kernel<DT, DRAFT><<<B, THREADS, 0, s>>>(a); break;
+    case GREEDY: run<DT, GREEDY>(p, a, B, s); break;
+    case POINT: run<DT, POINT>(p, a, B, s); break;
+    default: run<DT, DRAFT>(p, a, B, s); break;
   }
 }
 
@@ -366,6 +664,12 @@ void launch(const VerifyArgs& a, int mode, unsigned B, hipStream_t s) {
 
 using namespace cab;
 
+extern "C" size_t cab_verify_drafts_workspace_bytes(cab_dtype_t dtype, int64_t B, int64_t T,
+                                                     int64_t V, int greedy, int drafted) {
+  if (!valid_dtype(dtype) || !verify_sizes(B, T, V)) return 0;
+  return verify_plan(dtype, greedy ? GREEDY : drafted ? DRAFT : POINT, B, T, V).bytes;
+}
+
 extern "C" cab_status_t cab_verify_drafts(const void* logits, const void* draft_logits,
                                           cab_dtype_t dtype, int64_t B, int64_t T, int64_t V,
                                           const int64_t logit_strides[2],
@@ -373,17 +677,18 @@ extern "C" cab_status_t cab_verify_drafts(const void* logits, const void* draft_
                                           const int32_t* parents, int64_t parents_stride,
                                           const float* uniforms, const float* noise,
                                           float temperature, int32_t* path, int32_t* counts,
-                                          int64_t* next_tokens, void* stream) {
+                                          int64_t* next_tokens, void* workspace,
+                                          size_t workspace_bytes, void* stream) {
   const char* fn = "cab_verify_drafts";
   clear_error();
   CAB_REQUIRE(valid_dtype(dtype), CAB_EDTYPE, "%s: unknown dtype %d", fn, static_cast<int>(dtype));
   CAB_REQUIRE(B >= 0 && T >= 1 && V >= 1, CAB_ESHAPE, "%s: bad shape", fn);
   CAB_REQUIRE(T <= MAX_NODES, CAB_ESHAPE, "%s: a tree holds at most %d nodes", fn, MAX_NODES);
-  CAB_REQUIRE(V <= INT32_MAX / 2 && B <= INT32_MAX, CAB_ESHAPE, "%s: problem too large", fn);
   // (1 / temperature and the exponents it scales stay ordinary floats)
   CAB_REQUIRE(temperature == 0.f || (temperature >= 1e-6f && temperature <= 1e6f), CAB_EINVAL,
               "%s: temperature must be 0 (greedy) or in [1e-6, 1e6]", fn);
   if (B == 0) return CAB_OK;
+  CAB_REQUIRE(verify_sizes(B, T, V), CAB_ESHAPE, "%s: problem too large", fn);
   const bool greedy = temperature == 0.f;
   CAB_REQUIRE(logits && logit_strides && tokens && parents && path && counts && next_tokens,
               CAB_EINVAL, "%s: null argument", fn);
@@ -416,11 +721,24 @@ extern "C" cab_status_t cab_verify_drafts(const void* logits, const void* draft_
   a.counts = counts;
   a.next = next_tokens;
   const int mode = greedy ? GREEDY : draft_logits ? DRAFT : POINT;
+  const VerifyPlan p = verify_plan(dtype, mode, B, T, V);
+  CAB_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes &&
+                               reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+              CAB_EWORKSPACE, "%s: workspace needs %zu bytes, 16-byte aligned", fn, p.bytes);
+  char* ws = static_cast<char*>(workspace);
+  a.stats = reinterpret_cast<RowStats*>(ws);
+  a.ends = reinterpret_cast<WalkEnd*>(ws + p.off_ends);
+  a.picks = reinterpret_cast<Candidate*>(ws + p.off_picks);
+  a.slices = static_cast<int32_t>(p.slices);
+  a.slice = static_cast<int32_t>(p.slice);
+  a.pick_slices = static_cast<int32_t>(p.pick_slices);
+  a.pick_slice = static_cast<int32_t>(p.pick_slice);
+  a.rows = B * T;
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
-    case CAB_F32: launch<CAB_F32>(a, mode, static_cast<unsigned>(B), s); break;
-    case CAB_BF16: launch<CAB_BF16>(a, mode, static_cast<unsigned>(B), s); break;
-    default: launch<CAB_F16>(a, mode, static_cast<unsigned>(B), s); break;
+    case CAB_F32: launch<CAB_F32>(p, a, mode, static_cast<unsigned>(B), s); break;
+    case CAB_BF16: launch<CAB_BF16>(p, a, mode, static_cast<unsigned>(B), s); break;
+    default: launch<CAB_F16>(p, a, mode, static_cast<unsigned>(B), s); break;
   }
   return launch_status(fn);
 }

@@ -520,14 +520,20 @@ cab_status_t cab_tree_attn_fwd(const void* q, const void* k, const void* v, cab_
  * one tree for all sequences, else entries from one to the next. Out: path int32
  * [B,T], the accepted nodes ascending (node 0 first), then -1; counts int32 [B],
  * how many; next_tokens int64 [B]. Arrays are contiguous unless a stride is
- * given.
+ * given. workspace: cab_verify_drafts_workspace_bytes() bytes (greedy, drafted:
+ * whether temperature is 0, whether there are draft_logits; may be 0), 16-byte
+ * aligned, overwritten.
  */
+size_t cab_verify_drafts_workspace_bytes(cab_dtype_t dtype, int64_t B, int64_t T, int64_t V,
+                                         int greedy, int drafted);
+
 cab_status_t cab_verify_drafts(const void* logits, const void* draft_logits, cab_dtype_t dtype,
                                int64_t B, int64_t T, int64_t V, const int64_t logit_strides[2],
                                const int64_t draft_strides[2], const int64_t* tokens,
                                const int32_t* parents, int64_t parents_stride,
                                const float* uniforms, const float* noise, float temperature,
-                               int32_t* path, int32_t* counts, int64_t* next_tokens, void* stream);
+                               int32_t* path, int32_t* counts, int64_t* next_tokens,
+                               void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Token-level Forman-Ricci curvature of a weighted directed graph A [n, n]
