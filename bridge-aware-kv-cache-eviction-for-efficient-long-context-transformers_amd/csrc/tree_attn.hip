@@ -813,9 +813,9 @@ TreePlan tree_plan(cab_dtype_t dtype, int64_t B, int64_t H, int64_t Hkv, int64_t
   } else {
     p.tile = p.R <= 64 ? 64 : p.R <= 128 ? 128 : 256;
     p.row_tiles = ceil_div(p.R, p.tile);
-    // (two tiles a workgroup at least; four of the small ones at D = 128: 64 rows of 8176
-    // keys 19.9 us against 22.1, 128 rows 25.1 against 29.0)
-    p.least = p.tile < 256 && D == 128 ? 4 : 2;
+    // (two tiles a workgroup at least; four of the small ones at D = 128 in all but short
+    // lists: 64 rows of 8 x 8176 keys 19.9 us against 22.1, 20 of 8 x 595 15.1 against 12.9)
+    p.least = p.tile < 256 && D == 128 && p.units * most > 512 * TILE ? 4 : 2;
     if (p.tile < 256) slots = SMALL_TILE_WGS;
     keys = TILE;
   }

@@ -29,8 +29,8 @@ namespace cab {
 namespace {
 
 constexpr int MAX_NODES = 256;
-constexpr int WALK_THREADS = 1024;  // of a walk that reads rows
-constexpr int SLICE_THREADS = 256;  // of stats_kernel, pick_kernel and a walk that reads none
+constexpr int WALK_THREADS = 1024;
+constexpr int SLICE_THREADS = 256;  // of stats_kernel and pick_kernel
 enum { GREEDY = 0, POINT = 1, DRAFT = 2 };
 
 // 16 bytes at any element's alignment (global loads need none on gfx950).
@@ -55,7 +55,7 @@ struct VerifyArgs {
   struct WalkEnd* ends;      // [B]
   struct Candidate* picks;   // [B][picks of a row]
   int32_t slices, slice;     // slices of a row in stats_kernel, their values
-  int32_t pick_slices, pick_slice;
+  int32_t picks_a_row, pick;  // in pick_kernel
   int64_t rows;              // B * T
 };
 
@@ -79,13 +79,24 @@ struct WalkEnd {
   int32_t gone[MAX_NODES];
 };
 
-// The best of a slice: scores of weights relative to m; from the residual, and from
-// the whole row for when nothing is left of it.
+// The best of a slice, from the residual, and from the whole row for when nothing is left
+// of it: score (relative to m), and the logit and 1 / noise it comes from.
 struct Candidate {
-  float m, score[2];
+  float m, score[2], x[2], y[2];
   int32_t index[2];
   int32_t unused[3];
 };
+// What one workgroup leaves for another of the same launch goes past the L2 caches, which
+// the XCDs do not share; a release fence would write a whole L2 back (512 workgroups of
+// pick_kernel: 28 us with fences, 12 so).
+template <typename T>
+__device__ __forceinline__ void put(T* p, T v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename T>
+__device__ __forceinline__ T get(const T* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
 
 template <cab_dtype_t DT>
 __device__ __forceinline__ float value_at(const char* row, int i) {
@@ -133,12 +144,19 @@ __device__ __forceinline__ double residual(float ep, double ip, float eq, double
   return fmax(p - q, 0.0);
 }
 
+// The same in 32 bits, for sums of many.
+__device__ __forceinline__ float residual32(float ep, float ip, float eq, float uq) {
+#pragma clang fp contract(off)
+  const float p = ep * ip, q = eq * uq;
+  return fmaxf(p - q, 0.f);
+}
+
 template <int THREADS>
 struct Scratch {
   static constexpr int WAVES = THREADS / 64;
   float m[WAVES];
   double s[WAVES];
-  unsigned long long key[WAVES];
+  unsigned long long key[WAVES], key2[WAVES];
 };
 
 template <int THREADS>
@@ -152,6 +170,32 @@ __device__ __forceinline__ double block_sum(double v, Scratch<THREADS>& sh) {
 #pragma unroll
   for (int w = 0; w < THREADS / 64; ++w) v += sh.s[w];
   return v;
+}
+
+// The largest of each of two keys, over a wave and over the workgroup.
+__device__ __forceinline__ void wave_max2(unsigned long long (&k)[2]) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const unsigned long long o = __shfl_xor(k[i], off, 64);
+      k[i] = o > k[i] ? o : k[i];
+    }
+}
+template <int THREADS>
+__device__ __forceinline__ void block_max2(unsigned long long (&k)[2], Scratch<THREADS>& sh) {
+  wave_max2(k);
+  __syncthreads();
+  if (lane_id() == 0) {
+    sh.key[threadIdx.x >> 6] = k[0];
+    sh.key2[threadIdx.x >> 6] = k[1];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    k[0] = sh.key[w] > k[0] ? sh.key[w] : k[0];
+    k[1] = sh.key2[w] > k[1] ? sh.key2[w] : k[1];
+  }
 }
 
 template <int THREADS>
@@ -191,36 +235,51 @@ __device__ __forceinline__ int key_index(unsigned long long k) {
   return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k));
 }
 
-// f(first index, values, how many) over the 16-byte chunks of V values, U of them loaded
-// at a time, then the last values one by one.
-template <cab_dtype_t DT, int U, int THREADS, typename F>
-__device__ __forceinline__ void over_row(const char* row, int V, F f) {
+// f(first index, values, other row's values, how many) over the 16-byte chunks of V values,
+// U of them loaded at a time, then the last values one by one. TWO: of two rows alike.
+template <cab_dtype_t DT, int U, int THREADS, bool TWO, typename F>
+__device__ __forceinline__ void over_rows(const char* row, const char* other, int V, F f) {
   constexpr int N = Chunk<DT>::N;
   const int n = V / N;
   for (int c0 = threadIdx.x; c0 < n; c0 += U * THREADS) {
-    Chunk<DT> x[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (c0 + u * THREADS < n) x[u].load(row, c0 + u * THREADS);
+    Chunk<DT> x[U], y[TWO ? U : 1];
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (c0 + u * THREADS < n) {
-        float v[N];
+        x[u].load(row, c0 + u * THREADS);
+        if constexpr (TWO) y[u].load(other, c0 + u * THREADS);
+      }
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = x[u].get(i);
-        f((c0 + u * THREADS) * N, v, std::integral_constant<int, N>{});
+    for (int u = 0; u < U; ++u)
+      if (c0 + u * THREADS < n) {
+        float v[N], v2[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          v[i] = x[u].get(i);
+          v2[i] = TWO ? y[TWO ? u : 0].get(i) : 0.f;
+        }
+        f((c0 + u * THREADS) * N, v, v2, std::integral_constant<int, N>{});
       }
   }
   const int i = n * N + static_cast<int>(threadIdx.x);
   if (i < V) {
-    float v[1] = {value_at<DT>(row, i)};
-    f(i, v, std::integral_constant<int, 1>{});
+    const float v[1] = {value_at<DT>(row, i)}, v2[1] = {TWO ? value_at<DT>(other, i) : 0.f};
+    f(i, v, v2, std::integral_constant<int, 1>{});
   }
 }
+template <cab_dtype_t DT, int U, int THREADS, typename F>
+__device__ __forceinline__ void over_row(const char* row, int V, F f) {
+  over_rows<DT, U, THREADS, false>(row, nullptr, V,
+                                   [&](int at, const float* v, const float*, auto n) { f(at, v, n); });
+}
 
-// Maximum (at least the lowest float) and sum of weights of a row. The sum's terms
-// take the exponent in one product: those that count in it are near the maximum,
-// where that is as exact as weight().
+// weight() with the exponent in one product: off by 2^-24 of the exponent, which is as
+// exact for the values near the maximum that sums are made of.
+__device__ __forceinline__ float near_weight(float x, float m, const VerifyArgs& a) {
+  return x == m ? 1.f : __builtin_amdgcn_exp2f(fmaxf(x - m, a.d_min) * a.c_hi);
+}
+
+// Maximum (at least the lowest float) and sum of weights of a row.
 template <cab_dtype_t DT, int THREADS>
 __device__ void row_softmax(const char* row, int V, const VerifyArgs& a, Scratch<THREADS>& sh, float& m,
                             double& s) {
@@ -236,14 +295,8 @@ __device__ void row_softmax(const char* row, int V, const VerifyArgs& a, Scratch
       mt = hi;
     }
     float sum = 0.f;
-    if (mt < INFINITY) {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        sum += __builtin_amdgcn_exp2f(fmaxf(v[i] - mt, a.d_min) * a.c_hi);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) sum += v[i] == mt ? 1.f : 0.f;
-    }
+    for (int i = 0; i < N; ++i) sum += near_weight(v[i], mt, a);
     st += sum;
   });
   float mw = mt;
@@ -303,38 +356,38 @@ __global__ __launch_bounds__(SLICE_THREADS) void stats_kernel(VerifyArgs a) {
   if (threadIdx.x == 0) a.stats[(blockIdx.y * a.rows + row) * a.slices + slice] = r;
 }
 
-// A row's statistics from its slices' (at most 64), in every lane.
-__device__ __forceinline__ void merge_softmax(const RowStats* st, const VerifyArgs& a, float& m, double& s) {
-  const int lane = lane_id();
-  float ml = -__FLT_MAX__;
-  double sl = 0.0;
-  if (lane < a.slices) {
-    ml = st[lane].m;
-    sl = st[lane].s;
-  }
+// A row's statistics from its slices', in the `width` lanes that hold one each (a power of
+// two; st null: none).
+__device__ __forceinline__ void merge_softmax(const RowStats* st, int width, const VerifyArgs& a, float& m,
+                                              double& s) {
+  const float ml = st ? st->m : -__FLT_MAX__;
+  const double sl = st ? st->s : 0.0;
   m = ml;
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, shfl_xor_f32(m, off));
+  for (int off = width >> 1; off >= 1; off >>= 1) m = fmaxf(m, shfl_xor_f32(m, off));
   s = sl * weight(ml, m, a);
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) s += shfl_xor_f64(s, off);
+  for (int off = width >> 1; off >= 1; off >>= 1) s += shfl_xor_f64(s, off);
 }
-__device__ __forceinline__ unsigned long long merge_argmax(const RowStats* st, const VerifyArgs& a) {
-  unsigned long long key = lane_id() < a.slices ? st[lane_id()].key : 0;
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) {
+__device__ __forceinline__ unsigned long long merge_argmax(const RowStats* st, int width) {
+  unsigned long long key = st ? st->key : 0;
+  for (int off = width >> 1; off >= 1; off >>= 1) {
     const unsigned long long o = __shfl_xor(key, off, 64);
     key = o > key ? o : key;
   }
   return key;
 }
 
-// STATS: rows' statistics are there, and where the walk ended is left for pick_kernel.
-template <cab_dtype_t DT, int MODE, bool STATS, int THREADS>
-__global__ __launch_bounds__(THREADS) void walk_kernel(VerifyArgs a) {
+// STATS: rows' statistics are there. Where the walk ended is left for pick_kernel.
+template <cab_dtype_t DT, int MODE, bool STATS>
+__global__ __launch_bounds__(WALK_THREADS) void walk_kernel(VerifyArgs a) {
+  constexpr int THREADS = WALK_THREADS;
+  // gone: rejected tokens at the end; greedy with STATS: the rows' argmax.
   __shared__ int32_t parent[MAX_NODES], token[MAX_NODES], out[MAX_NODES], gone[MAX_NODES];
   // Each draft's uniform number, and its logit in its parent's row (and the draft's).
   __shared__ float uniform[MAX_NODES], value[MAX_NODES], drawn[MODE == DRAFT ? MAX_NODES : 1];
+  // STATS: rows' maxima and sums (of nodes without children, whatever the workspace held).
+  constexpr int SIDES = MODE == DRAFT ? 2 : 1;
+  __shared__ float high[STATS ? SIDES : 1][MAX_NODES];
+  __shared__ double total[STATS ? SIDES : 1][MAX_NODES];
   __shared__ Scratch<THREADS> sh;
   const int b = blockIdx.x, tid = threadIdx.x, lane = lane_id();
   const char* logits = a.logits + b * a.ls[0];
@@ -357,6 +410,30 @@ __global__ __launch_bounds__(THREADS) void walk_kernel(VerifyArgs a) {
       }
     }
   }
+  if constexpr (STATS) {
+    // All at once: the walk itself then waits for no memory.
+    const RowStats* stats = a.stats + static_cast<int64_t>(b) * a.T * a.slices;
+    int width = 1;  // lanes a row
+    while (width < a.slices) width <<= 1;
+    const int at = tid & (width - 1);
+    for (int x = tid / width; x - tid / width < SIDES * a.T; x += THREADS / width) {
+      const int side = x >= a.T, i = x - side * a.T;
+      const bool in = x < SIDES * a.T;
+      const RowStats* st = in && at < a.slices ? stats + (side * a.rows + i) * a.slices + at : nullptr;
+      if constexpr (MODE == GREEDY) {
+        const unsigned long long key = merge_argmax(st, width);
+        if (in && at == 0) gone[i] = key ? key_index(key) : -1;
+      } else {
+        float m;
+        double s;
+        merge_softmax(st, width, a, m, s);
+        if (in && at == 0) {
+          high[side][i] = m;
+          total[side][i] = s;
+        }
+      }
+    }
+  }
   __syncthreads();
   // (every wave scans and decides alike; only row passes meet at barriers)
   auto next_child = [&](int node, int after) {
@@ -367,13 +444,13 @@ __global__ __launch_bounds__(THREADS) void walk_kernel(VerifyArgs a) {
     }
     return -1;
   };
-  const RowStats* stats = nullptr;
-  if constexpr (STATS) stats = a.stats + static_cast<int64_t>(b) * a.T * a.slices;
-  auto softmax_of = [&](bool drafted, int node, const char* row, float& m, double& s) {
-    if constexpr (STATS)
-      merge_softmax(stats + ((drafted ? a.rows : 0) + node) * a.slices, a, m, s);
-    else
+  auto softmax_of = [&](int side, int node, const char* row, float& m, double& s) {
+    if constexpr (STATS) {
+      m = high[side][node];
+      s = total[side][node];
+    } else {
       row_softmax<DT, THREADS>(row, a.V, a, sh, m, s);
+    }
   };
   const char* lrow;
   const char* qrow = nullptr;
@@ -387,13 +464,16 @@ __global__ __launch_bounds__(THREADS) void walk_kernel(VerifyArgs a) {
     int taken = -1;
     const int first = next_child(node, node);
     if constexpr (MODE == GREEDY) {
-      const unsigned long long key =
-          STATS ? merge_argmax(stats + static_cast<int64_t>(node) * a.slices, a) : row_argmax<DT, THREADS>(lrow, a.V, sh);
-      best = key ? key_index(key) : -1;
+      if constexpr (STATS) {
+        best = gone[node];
+      } else {
+        const unsigned long long key = row_argmax<DT, THREADS>(lrow, a.V, sh);
+        best = key ? key_index(key) : -1;
+      }
       for (int i = first; i >= 0 && taken < 0; i = next_child(node, i))
         if (token[i] >= 0 && token[i] == best) taken = i;
     } else if constexpr (MODE == POINT) {
-      if (first >= 0 || !STATS) softmax_of(false, node, lrow, m, s);
+      if (first >= 0) softmax_of(0, node, lrow, m, s);
       left = s;
       for (int i = first; i >= 0 && taken < 0; i = next_child(node, i)) {
         const int x = token[i];
@@ -414,10 +494,10 @@ __global__ __launch_bounds__(THREADS) void walk_kernel(VerifyArgs a) {
       qrow = drafts + node * a.ds[1];
       left = 1.0;
       used = 0.0;
-      if (first >= 0 || !STATS) {
+      if (first >= 0) {
         double sq;
-        softmax_of(false, node, lrow, m, s);
-        softmax_of(true, node, qrow, mq, sq);
+        softmax_of(0, node, lrow, m, s);
+        softmax_of(1, node, qrow, mq, sq);
         ip = s > 0.0 ? 1.0 / s : 0.0;
         iq = sq > 0.0 ? 1.0 / sq : 0.0;
       }
@@ -427,13 +507,13 @@ __global__ __launch_bounds__(THREADS) void walk_kernel(VerifyArgs a) {
         if (!known) {
           double c = 0.0;
           const double uq = used * iq;
-          over_row<DT, 2, THREADS>(lrow, a.V, [&](int at, const float* v, auto n) {
+          const float fp = static_cast<float>(ip), fq = static_cast<float>(uq);
+          over_rows<DT, 4, THREADS, true>(lrow, qrow, a.V, [&](int, const float* v, const float* v2, auto n) {
+            float sum = 0.f;
 #pragma unroll
-            for (int k = 0; k < decltype(n)::value; ++k) {
-              const float ep = weight(v[k], m, a);
-              const float eq = weight(value_at<DT>(qrow, at + k), mq, a);
-              c += residual(ep, ip, eq, uq);
-            }
+            for (int k = 0; k < decltype(n)::value; ++k)
+              sum += residual32(near_weight(v[k], m, a), fp, near_weight(v2[k], mq, a), fq);
+            c += sum;
           });
           left = block_sum<THREADS>(c, sh);
           known = true;
@@ -464,7 +544,7 @@ __global__ __launch_bounds__(THREADS) void walk_kernel(VerifyArgs a) {
   if (tid == 0) a.counts[b] = count;
   if constexpr (MODE == GREEDY) {
     if (tid == 0) a.next[b] = best;
-  } else if constexpr (STATS) {
+  } else {
     WalkEnd& e = a.ends[b];
     for (int i = tid; i < n_gone; i += THREADS) e.gone[i] = gone[i];
     if (tid == 0) {
@@ -477,177 +557,184 @@ __global__ __launch_bounds__(THREADS) void walk_kernel(VerifyArgs a) {
       e.n_gone = n_gone;
       e.done = 0;
     }
-  } else {
-    const float* noise = a.noise + static_cast<int64_t>(b) * a.V;
-    double uq = used * iq;
-    unsigned long long key = 0;
-    // The second time over the whole row's weights, if nothing is left of them.
-    for (int pass = 0; pass < 2 && key == 0; ++pass) {
-      over_row<DT, 2, THREADS>(lrow, a.V, [&](int at, const float* v, auto n) {
-        constexpr int N = decltype(n)::value;
-        const uint32_t out_of = gone_mask<N>(gone, n_gone, at);
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-          float w = weight(v[k], m, a);
-          if constexpr (MODE == DRAFT)
-            w = static_cast<float>(residual(w, ip, weight(value_at<DT>(qrow, at + k), mq, a), uq));
-          const float score = w * __builtin_amdgcn_rcpf(noise[at + k]);
-          const unsigned long long o = order_key(score, at + k);
-          if (w > 0.f && score >= 0.f && !(out_of >> k & 1) && o > key) key = o;
-        }
-      });
-      key = block_max<THREADS>(key, sh);
-      uq = 0.0;
-      n_gone = 0;
-    }
-    if (tid == 0) a.next[b] = key ? key_index(key) : -1;
   }
 }
 
-// Grid: slices of a row, by sequence. Scores are relative to the slice's own maximum
-// where nothing was taken off the row (a leaf has no statistics), else to the row's.
-// The sequence's last workgroup compares the slices' candidates.
+// Grid: slices of a row, by sequence. A thread compares its values relative to the
+// largest it has seen (a leaf's row has no statistics, and none are needed: the
+// argmax is the same whatever all weights are relative to), or, where the residual takes
+// the draft's weights off, to the row's. The sequence's last workgroup compares the slices'.
 template <cab_dtype_t DT, int MODE>
 __global__ __launch_bounds__(SLICE_THREADS) void pick_kernel(VerifyArgs a) {
   constexpr int ES = DT == CAB_F32 ? 4 : 2;
   __shared__ Scratch<SLICE_THREADS> sh;
   __shared__ int32_t gone[MAX_NODES];
   __shared__ bool last;
-  const int b = blockIdx.x / a.pick_slices, at_slice = blockIdx.x - b * a.pick_slices, tid = threadIdx.x;
+  const int b = blockIdx.x / a.picks_a_row, at_slice = blockIdx.x - b * a.picks_a_row, tid = threadIdx.x;
   WalkEnd& e = a.ends[b];
-  const int n_gone = e.n_gone;
-  if (tid < n_gone) gone[tid] = e.gone[tid];
-  const int from = at_slice * a.pick_slice, n = min(a.pick_slice, a.V - from);
+  const int n_gone = MODE == POINT ? e.n_gone : 0;
+  const int from = at_slice * a.pick, n = min(a.pick, a.V - from);
   const char* lrow = a.logits + b * a.ls[0] + e.node * a.ls[1] + static_cast<int64_t>(from) * ES;
-  const char* qrow = nullptr;
-  const bool whole = MODE == POINT || e.used == 0.0;
-  if constexpr (MODE == DRAFT) qrow = a.drafts + b * a.ds[0] + e.node * a.ds[1] + static_cast<int64_t>(from) * ES;
   const float* noise = a.noise + static_cast<int64_t>(b) * a.V + from;
-  float m = e.m;
+  if constexpr (MODE == POINT) {
+    gone[tid] = e.gone[tid] - from;  // (behind n_gone: whatever the workspace held)
+    __syncthreads();
+  }
+  // top[0]: of the residual; top[1]: of the row, for when nothing is left of that.
+  const bool whole = MODE == POINT || e.used == 0.0;
+  struct Top {
+    float score, x, y;  // x, y: the logit and 1 / noise it comes from
+    int32_t at;
+  };
+  Top top[2] = {{-1.f, 0.f, 0.f, -1}, {-1.f, 0.f, 0.f, -1}};
+  float m = -__FLT_MAX__;
+  auto score_of = [&](float x, float iy, float to) {
+    const float w = weight(x, to, a);
+    return w > 0.f ? w * iy : -1.f;
+  };
+  auto beat = [](Top& t, float score, float x, float y, int at) {
+    if (score > t.score) t = Top{score, x, y, at};  // (indexes ascend within a thread; NaN beats nothing)
+  };
+  // Scores of another reference are formed anew from logit and noise: equal ones stay equal.
+  auto refer = [&](Top& t, float to) {
+    t.score = t.at >= 0 ? score_of(t.x, t.y, to) : -1.f;
+    if (!(t.score >= 0.f)) t = Top{-1.f, 0.f, 0.f, -1};
+  };
   if (whole) {
-    float mt = -__FLT_MAX__;
-    over_row<DT, 4, SLICE_THREADS>(lrow, n, [&](int, const float* v, auto k) {
+    over_row<DT, 1, SLICE_THREADS>(lrow, n, [&](int at, const float* v, auto nn) {
+      constexpr int N = decltype(nn)::value;
+      float y[N], hi = m;
 #pragma unroll
-      for (int i = 0; i < decltype(k)::value; ++i) mt = fmaxf(mt, v[i]);
+      for (int k = 0; k < N; ++k) {
+        y[k] = noise[at + k];
+        hi = fmaxf(hi, v[k]);
+      }
+      if (hi > m) {
+        m = hi;
+        refer(top[0], m);
+        refer(top[1], m);
+      }
+      const uint32_t out_of = gone_mask<N>(gone, n_gone, at);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const float iy = __builtin_amdgcn_rcpf(y[k]), score = score_of(v[k], iy, m);
+        const bool out = out_of >> k & 1;
+        beat(top[0], out ? -1.f : score, v[k], iy, from + at + k);
+        if (out_of) beat(top[1], out ? score : -1.f, v[k], iy, from + at + k);
+      }
     });
+  } else {
+    const char* qrow = a.drafts + b * a.ds[0] + e.node * a.ds[1] + static_cast<int64_t>(from) * ES;
+    const double ip = e.ip, uq = e.used * e.iq;
+    const float mq = e.mq;
+    m = e.m;
+    over_rows<DT, 1, SLICE_THREADS, true>(lrow, qrow, n, [&](int at, const float* v, const float* v2, auto nn) {
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) mt = fmaxf(mt, shfl_xor_f32(mt, off));
-    if (lane_id() == 0) sh.m[tid >> 6] = mt;
+      for (int k = 0; k < decltype(nn)::value; ++k) {
+        const float w = weight(v[k], m, a), iy = __builtin_amdgcn_rcpf(noise[at + k]);
+        const float r = static_cast<float>(residual(w, ip, weight(v2[k], mq, a), uq));
+        beat(top[0], r > 0.f ? r * iy : -1.f, v[k], iy, from + at + k);
+        beat(top[1], w > 0.f ? w * iy : -1.f, v[k], iy, from + at + k);
+      }
+    });
+  }
+  // The workgroup's candidates.
+  if (whole) {
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, shfl_xor_f32(m, off));
+    if (lane_id() == 0) sh.m[tid >> 6] = m;
     __syncthreads();
     m = fmaxf(fmaxf(sh.m[0], sh.m[1]), fmaxf(sh.m[2], sh.m[3]));
+    refer(top[0], m);
+    refer(top[1], m);
   }
-  __syncthreads();
-  const double ip = e.ip, uq = e.used * e.iq;
-  const float mq = e.mq;
-  unsigned long long key[2] = {0, 0};  // of the residual, of the row
-  over_row<DT, 2, SLICE_THREADS>(lrow, n, [&](int at, const float* v, auto nn) {
-    constexpr int N = decltype(nn)::value;
-    const uint32_t out_of = gone_mask<N>(gone, n_gone, from + at);
+  unsigned long long mine[2], most[2];
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const float w = weight(v[k], m, a), rn = __builtin_amdgcn_rcpf(noise[at + k]);
-      const float score = w * rn;
-      const unsigned long long o = order_key(score, from + at + k);
-      const bool ok = w > 0.f && score >= 0.f;
-      if (ok && o > key[1]) key[1] = o;
-      if constexpr (MODE == DRAFT) {
-        if (!whole) {
-          const float r = static_cast<float>(residual(w, ip, weight(value_at<DT>(qrow, at + k), mq, a), uq));
-          const unsigned long long or_ = order_key(r * rn, from + at + k);
-          if (r > 0.f && r * rn >= 0.f && or_ > key[0]) key[0] = or_;
-        } else if (ok && o > key[0]) {
-          key[0] = o;
-        }
-      } else if (ok && !(out_of >> k & 1) && o > key[0]) {
-        key[0] = o;
-      }
+  for (int i = 0; i < 2; ++i) most[i] = mine[i] = top[i].at >= 0 ? order_key(top[i].score, top[i].at) : 0;
+  block_max2<SLICE_THREADS>(most, sh);
+  Candidate* const c = a.picks + blockIdx.x;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (most[i] ? mine[i] == most[i] : tid == 0) {  // (keys of two threads differ: their indexes do)
+      put(&c->index[i], top[i].at);
+      put(&c->score[i], top[i].score);
+      put(&c->x[i], top[i].x);
+      put(&c->y[i], top[i].y);
     }
-  });
-  Candidate c;
-  c.m = m;
-  for (int i = 0; i < 2; ++i) {
-    key[i] = block_max<SLICE_THREADS>(key[i], sh);
-    c.score[i] = __uint_as_float(static_cast<uint32_t>(key[i] >> 32) & 0x7fffffffu);
-    c.index[i] = key[i] ? key_index(key[i]) : -1;
-  }
-  if (tid == 0) {
-    a.picks[blockIdx.x] = c;
-    last = __hip_atomic_fetch_add(&e.done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) + 1 ==
-           static_cast<uint32_t>(a.pick_slices);
-  }
+  if (tid == 0) put(&c->m, m);
+  asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // (what was put has arrived)
+  __syncthreads();
+  if (tid == 0)
+    last = __hip_atomic_fetch_add(&e.done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 ==
+           static_cast<uint32_t>(a.picks_a_row);
   __syncthreads();
   if (!last || tid >= 64) return;
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-  const Candidate* cs = a.picks + static_cast<int64_t>(b) * a.pick_slices;
-  float hi = -__FLT_MAX__;
-  for (int x = tid; x < a.pick_slices; x += 64) hi = fmaxf(hi, cs[x].m);
+  const bool in = tid < a.picks_a_row;  // (at most 64)
+  const Candidate* all = a.picks + static_cast<int64_t>(b) * a.picks_a_row + (in ? tid : 0);
+  float hi = get(&all->m);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    top[i] = Top{get(&all->score[i]), get(&all->x[i]), get(&all->y[i]), get(&all->index[i])};
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) hi = fmaxf(hi, shfl_xor_f32(hi, off));
-  key[0] = key[1] = 0;
-  for (int x = tid; x < a.pick_slices; x += 64) {
-    const Candidate y = cs[x];
-    const float f = weight(y.m, hi, a);
-    for (int i = 0; i < 2; ++i) {
-      const unsigned long long o = order_key(y.score[i] * f, y.index[i]);
-      if (y.index[i] >= 0 && f > 0.f && o > key[i]) key[i] = o;
-    }
-  }
-  for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
-      const unsigned long long o = __shfl_xor(key[i], off, 64);
-      key[i] = o > key[i] ? o : key[i];
-    }
-  if (tid == 0) a.next[b] = key[0] ? key_index(key[0]) : key[1] ? key_index(key[1]) : -1;
+  for (int i = 0; i < 2; ++i) {
+    if (whole) refer(top[i], hi);
+    most[i] = in && top[i].at >= 0 ? order_key(top[i].score, top[i].at) : 0;
+  }
+  wave_max2(most);
+  if (tid == 0) a.next[b] = most[0] ? key_index(most[0]) : most[1] ? key_index(most[1]) : -1;
 }
 
-// How a call is run: the statistics' and candidates' slices and workspace.
+// How a call is run: a row's slices, and the workspace.
 struct VerifyPlan {
   bool stats;
-  int64_t slices, slice, pick_slices, pick_slice;
+  int64_t slices, slice, picks, pick;
   size_t off_ends, off_picks, bytes;
 };
 
-// Bytes of logits up to which all rows' statistics are taken.
-constexpr int64_t STATS_BYTES = int64_t{384} << 20;
+// Bytes of logits up to which all rows' statistics are taken (us, bf16, so -> rows one after
+// another: 1 tree of 64, 128000 tokens 24 -> 43, 32 of 5 30 -> 55, 4 drafted ones of 26,
+// fp32, 50001 32 -> 87; 32 of 32, 128000, 262 MB 58 -> 56; 64 of 64, 64000, 524 MB 96 -> 47).
+constexpr int64_t STATS_BYTES = int64_t{1} << 28;
 
 VerifyPlan verify_plan(cab_dtype_t dtype, int mode, int64_t B, int64_t T, int64_t V) {
   VerifyPlan p = {};
   const int64_t es = static_cast<int64_t>(dtype_size(dtype)), rows = B * T, sides = mode == DRAFT ? 2 : 1;
   p.stats = rows * sides <= STATS_BYTES / (V * es);
-  if (!p.stats) return p;
-  // 16 KB slices: four 16-byte loads a thread.
-  const int64_t unit = SLICE_THREADS * 64 / es;
-  auto cut = [&](int64_t most, int64_t& n, int64_t& size) {
-    n = ceil_div(V, unit) < most ? ceil_div(V, unit) : most;
+  // At most 64 slices a row (one wave merges them), and no more than fill the chip: a
+  // slice is at least `loads` 16-byte loads a thread. (32 trees of 32 rows: 2048 workgroups
+  // of statistics 68 us the call, 4096 60, 16384 62; 512 that pick 60, 1024 58, 2048 59.)
+  auto cut = [&](int64_t loads, int64_t units, int64_t fill, int64_t& n, int64_t& size) {
+    n = ceil_div(V, SLICE_THREADS * loads * 16 / es);
+    if (n > ceil_div(fill, units)) n = ceil_div(fill, units);
+    if (n > 64) n = 64;
     size = round_up(ceil_div(V, n), 16 / es);
     n = ceil_div(V, size);
   };
-  cut(64, p.slices, p.slice);
-  cut(64, p.pick_slices, p.pick_slice);
-  p.off_ends = static_cast<size_t>(sides * rows * p.slices) * sizeof(RowStats);
+  cut(4, rows * sides, 4096, p.slices, p.slice);
+  cut(1, B, 1024, p.picks, p.pick);
+  p.off_ends = p.stats ? static_cast<size_t>(sides * rows * p.slices) * sizeof(RowStats) : 0;
   p.off_picks = p.off_ends + (mode == GREEDY ? 0 : static_cast<size_t>(B) * sizeof(WalkEnd));
-  p.bytes = p.off_picks + (mode == GREEDY ? 0 : static_cast<size_t>(B * p.pick_slices) * sizeof(Candidate));
+  p.bytes = p.off_picks + (mode == GREEDY ? 0 : static_cast<size_t>(B * p.picks) * sizeof(Candidate));
   return p;
 }
 
 bool verify_sizes(int64_t B, int64_t T, int64_t V) {
-  return T >= 1 && T <= MAX_NODES && B >= 1 && B <= INT32_MAX / T && V >= 1 && V <= INT32_MAX / 2;
+  return T >= 1 && T <= MAX_NODES && B >= 1 && B <= INT32_MAX / 64 / T && V >= 1 && V <= INT32_MAX / 2;
 }
 
 template <cab_dtype_t DT, int MODE>
 void run(const VerifyPlan& p, const VerifyArgs& a, unsigned B, hipStream_t s) {
   if (!p.stats) {
-    walk_kernel<DT, MODE, false, WALK_THREADS><<<B, WALK_THREADS, 0, s>>>(a);
-    return;
+    walk_kernel<DT, MODE, false><<<B, WALK_THREADS, 0, s>>>(a);
+  } else {
+    const dim3 grid(static_cast<unsigned>(a.rows * p.slices), MODE == DRAFT ? 2 : 1);
+    stats_kernel<DT, MODE><<<grid, SLICE_THREADS, 0, s>>>(a);
+    walk_kernel<DT, MODE, true><<<B, WALK_THREADS, 0, s>>>(a);
   }
-  const dim3 grid(static_cast<unsigned>(a.rows * p.slices), MODE == DRAFT ? 2 : 1);
-  stats_kernel<DT, MODE><<<grid, SLICE_THREADS, 0, s>>>(a);
-  // (residuals' sums are rows read in the walk)
-  constexpr int THREADS = MODE == DRAFT ? WALK_THREADS : SLICE_THREADS;
-  walk_kernel<DT, MODE, true, THREADS><<<B, THREADS, 0, s>>>(a);
   if constexpr (MODE != GREEDY)
-    pick_kernel<DT, MODE><<<static_cast<unsigned>(p.pick_slices) * B, SLICE_THREADS, 0, s>>>(a);
+    pick_kernel<DT, MODE><<<static_cast<unsigned>(p.picks) * B, SLICE_THREADS, 0, s>>>(a);
 }
 
 template <cab_dtype_t DT>
@@ -731,8 +818,8 @@ extern "C" cab_status_t cab_verify_drafts(const void* logits, const void* draft_
   a.picks = reinterpret_cast<Candidate*>(ws + p.off_picks);
   a.slices = static_cast<int32_t>(p.slices);
   a.slice = static_cast<int32_t>(p.slice);
-  a.pick_slices = static_cast<int32_t>(p.pick_slices);
-  a.pick_slice = static_cast<int32_t>(p.pick_slice);
+  a.picks_a_row = static_cast<int32_t>(p.picks);
+  a.pick = static_cast<int32_t>(p.pick);
   a.rows = B * T;
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
