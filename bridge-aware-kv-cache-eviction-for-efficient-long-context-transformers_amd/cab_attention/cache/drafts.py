@@ -110,14 +110,29 @@ def commit_drafts(caches: Sequence[torch.Tensor], lengths: torch.Tensor, path: t
     return new
 
 
-def _commit(caches, lengths, length, path, counts, count, new, dev, es):
+def _commit(caches, lengths, length, path, counts, count, new, dev, es, columns=None):
     B, H, N, D = caches[0].shape
     n = len(caches)
+    st = caches[0].stride()
+    if columns is not None:  # rows as values of another size
+        D, st = columns, tuple(x * columns // D for x in st[:3]) + (1,)
     ptrs = (ctypes.c_void_p * n)(*[c.data_ptr() for c in caches])
     with nat.on_device(dev):
-        st = nat.load().cab_kv_commit(
-            ptrs, n, es, B, H, N, D, nat.strides4(caches[0]), nat.ptr(lengths), length,
-            path.data_ptr(), path.shape[1], path.shape[1] if path.shape[0] == B else 0,
-            nat.ptr(counts), count, nat.ptr(new), nat.stream_ptr(dev))
-    nat.check("cab_kv_commit", st)
+        status = nat.load().cab_kv_commit(
+            ptrs, n, es, B, H, N, D, nat.I64x4(*st), nat.ptr(lengths), length, path.data_ptr(),
+            path.shape[-1], path.shape[-1] if path.dim() == 2 else 0, nat.ptr(counts), count,
+            nat.ptr(new), nat.stream_ptr(dev))
+    nat.check("cab_kv_commit", status)
     nat.wrote(*caches)
+
+
+def commit_rows(caches: Sequence[torch.Tensor], path: torch.Tensor, length: int, count: int) -> None:
+    """:func:`commit_drafts` for contiguous buffers of one length, ``length`` rows before
+    the drafts, of which every sequence keeps ``count`` (int32 path ``[B, T]``, or ``[T]`` for
+    all). Rows of any dtype whose bytes are a multiple of 4."""
+    ref = caches[0]
+    nat.require_device(path, *caches)
+    nat.require_plain("commit", *caches)
+    _writable("commit", *caches)
+    _commit(caches, None, length, path, None, count, None, ref.device, 4,
+            ref.shape[3] * ref.element_size() // 4)

@@ -18,6 +18,10 @@ the next append or prune of that layer: a prune writes into the former
 active buffer, so a view kept across it changes. Callers that keep K or V
 across updates copy them.
 
+Drafted rows (speculative decoding) lie behind a layer's rows, uncounted, until
+``commit`` keeps the accepted ones; the next append, draft or prune of the layer
+drops them.
+
 ``EvictingCache`` is the decision layer: it counts update calls, asks its
 ``selector`` for the positions to keep when an eviction is due, prunes the
 store and the importance tracker with them and keeps the statistics. The
@@ -31,20 +35,24 @@ from typing import Any, Callable, Dict, List, Optional, Tuple
 
 import torch
 
+from .. import _native as nat
+from ..kernels.flash_attention_accumulate import key_scores
 from ..scoring import ImportanceTracker
+from .drafts import commit_rows
 from .prune import append_rows, gather_into
 
 _GRAIN = 16  # bytes: rows are padded to whole 16-byte chunks for the gather kernel
 
 
 class _Layer:
-    __slots__ = ("k", "v", "k_spare", "v_spare", "length", "width")
+    __slots__ = ("k", "v", "k_spare", "v_spare", "length", "width", "drafted")
 
     def __init__(self, k, v, width):
         self.k, self.v = k, v
         self.k_spare = self.v_spare = None
         self.length = 0
         self.width = width  # the caller's D (buffers may be wider)
+        self.drafted = 0    # rows behind `length` that wait for a commit
 
 
 class LayeredKV:
@@ -75,12 +83,54 @@ class LayeredKV:
         if layer >= len(self.layers) or self.layers[layer] is None:
             return None, None
         L = self.layers[layer]
-        k, v = L.k.narrow(2, 0, L.length), L.v.narrow(2, 0, L.length)
+        return self._rows(L, L.length)
+
+    @staticmethod
+    def _rows(L: _Layer, n: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        k, v = L.k.narrow(2, 0, n), L.v.narrow(2, 0, n)
         if L.width != L.k.shape[3]:
             k, v = k.narrow(3, 0, L.width), v.narrow(3, 0, L.width)
         return k, v
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor):
+        L = self._write(layer, k, v)
+        L.length += k.shape[2]
+        L.drafted = 0
+
+    def draft(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Writes drafted rows ``[B, H, T, D]`` behind the layer's rows without counting
+        them (a second call replaces the first's) and returns views of both: the
+        layer's rows and, last, the drafts."""
+        L = self._write(layer, k, v)
+        L.drafted = k.shape[2]
+        return self._rows(L, L.length + L.drafted)
+
+    def commit(self, path: torch.Tensor, count: int):
+        """Keeps ``count`` of every present layer's drafted rows: those at ``path[b, :count]``
+        (int32 ``[B, T]`` or ``[T]``, ascending), moved to the front of the drafts; the
+        other drafts are dropped. One launch per 64 tensors of one geometry."""
+        present = [L for L in self.layers if L is not None]
+        drafts = {L.drafted for L in present}
+        if len(drafts) != 1 or drafts == {0}:
+            raise ValueError("every layer must hold the same number of drafted rows")
+        T = drafts.pop()
+        count = int(count)
+        if not 0 <= count <= T or path.shape[-1] != T or path.dim() not in (1, 2):
+            raise ValueError(f"path must hold {T} nodes, the first {count} accepted")
+        groups: Dict[tuple, List[_Layer]] = {}
+        for L in present:
+            groups.setdefault((tuple(L.k.shape), L.k.dtype, L.k.device, L.length), []).append(L)
+        for (shape, _, dev, length), members in groups.items() if count else ():
+            if path.dim() == 2 and path.shape[0] != shape[0]:
+                raise ValueError(f"path must be [{shape[0]}, {T}]; got {list(path.shape)}")
+            rows = nat.index32(path.to(dev), "path", tuple(path.shape))
+            commit_rows([L.k for L in members] + [L.v for L in members], rows, length, count)
+        for L in present:
+            L.length += count
+            L.drafted = 0
+
+    def _write(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> _Layer:
+        """Copies rows behind the layer's counted rows (buffers made or grown as needed)."""
         if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype:
             raise ValueError("key/value states must be two [B, H, n, D] tensors of one dtype")
         while len(self.layers) <= layer:
@@ -107,7 +157,7 @@ class LayeredKV:
         if not append_rows(k, v, L.k, L.v, L.length):
             L.k[:, :, L.length:need, :L.width].copy_(k)
             L.v[:, :, L.length:need, :L.width].copy_(v)
-        L.length = need
+        return L
 
     def capacity(self, layer: int) -> int:
         """Rows the layer's active buffer holds (0 for an absent layer)."""
@@ -152,6 +202,7 @@ class LayeredKV:
             if id(L) in shrunk:
                 L.k_spare = L.v_spare = None  # the large buffers are released
             L.length = n_keep
+            L.drafted = 0
 
     def clear(self):
         self.layers = []
@@ -217,12 +268,58 @@ class EvictingCache:
             self.importance_tracker.update(attention_weights)
         self.stats["total_tokens_processed"] += 1
         self.tokens_since_last_eviction += 1
-        n = self._store.length(layer_idx)
+        self._evict_if_due(self._store.length(layer_idx))
+        return self._store.view(layer_idx)
+
+    def draft(self, key_states: torch.Tensor, value_states: torch.Tensor,
+              layer_idx: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Puts one layer's drafted K/V ``[B, H, T, D]`` behind its cached rows for one
+        pass over a tree of drafts, and returns the layer's K and V with the drafts as their
+        last T rows (``kernels.tree_attention`` without lengths). Nothing is evicted or
+        counted; the next draft or update of the layer replaces the drafts, and
+        :meth:`commit` keeps the accepted ones."""
+        return self._store.draft(layer_idx, key_states, value_states)
+
+    def commit(self, path: torch.Tensor, count: int, query: Optional[torch.Tensor] = None,
+               lse: Optional[torch.Tensor] = None, scale: Optional[float] = None):
+        """Keeps the ``count`` accepted drafts of every layer, the rows at ``path[b, :count]``
+        (``kernels.verify_drafts``' path; one count for the batch, the smallest where
+        sequences differ), and drops the others. Counts as ``count`` tokens' updates of
+        every layer, after which an eviction that is due takes place.
+
+        query, lse: layer 0's queries ``[B, H, T, D]`` of the drafts and
+        ``tree_attention``'s log-sum-exp ``[B, H, T]`` (``scale`` as there): the accepted
+        tokens' attention is added to the importance totals, as ``update``'s weights are."""
+        if (query is None) != (lse is None):
+            raise ValueError("query and lse come together")
+        if query is not None:
+            if (query.dim() != 4 or query.shape[2] != path.shape[-1] or lse.shape != query.shape[:3]
+                    or query.shape[3] not in (64, 128) or self._store.view(0)[0] is None):
+                raise ValueError("query must be [B, H, T, D] of layer 0 with D = 64 or 128, lse "
+                                 f"[B, H, T] with T = {path.shape[-1]}")
+        count = int(count)
+        self._store.commit(path, count)
+        if count == 0:
+            return
+        if query is not None:
+            # The accepted path is a plain causal chain behind the context now.
+            rows = path.to(device=query.device, dtype=torch.int64).reshape(-1, path.shape[-1])
+            rows = rows[:, :count].clamp(0, path.shape[-1] - 1)  # (a padded path reads some row)
+            rows = rows.expand(query.shape[0], count)[:, None, :, None]
+            keys, _ = self._store.view(0)
+            totals = key_scores(torch.take_along_dim(query, rows, 2), keys,
+                                torch.take_along_dim(lse, rows[..., 0], 2), scale, causal=True)
+            self.importance_tracker.add_scores(totals.sum((0, 1)), count)
+        layers = [L for L in self._store.layers if L is not None]
+        self.stats["total_tokens_processed"] += count * len(layers)
+        self.tokens_since_last_eviction += count * len(layers)
+        self._evict_if_due(max(L.length for L in layers))
+
+    def _evict_if_due(self, n: int):
         due = (n > int(self.max_cache_size * 1.1)
                or self.tokens_since_last_eviction >= self.eviction_interval)
         if due and n > self._floor:
             self._evict()
-        return self._store.view(layer_idx)
 
     def _evict(self):
         lengths = [L.length for L in self._store.layers if L is not None]
