@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import os
 import pathlib
 import threading
@@ -189,6 +190,13 @@ def strides4(t: torch.Tensor):
     return I64x4(*t.stride())
 
 
+@functools.lru_cache(maxsize=1024)
+def stride_array(stride: tuple):
+    """The strides as an array of C integers, one for each set of them (read only: a
+    decoding loop passes the same ones per layer and step)."""
+    return (ctypes.c_int64 * len(stride))(*stride)
+
+
 def rows_aligned(t: torch.Tensor) -> bool:
     """Last dim contiguous and rows starting on 16-byte boundaries (what the
     kernels' vector loads need)."""
@@ -257,6 +265,26 @@ def require_plain(fn: str, *tensors: torch.Tensor) -> None:
                                    "detached tensors")
 
 
+def plain_index(fn: str, *tensors: torch.Tensor) -> int:
+    """The device index of plain GPU tensors of one device, without gradients to record:
+    :func:`require_device` and :func:`require_plain` in one pass (which say what is
+    wrong; a step of a decoding loop asks this per layer)."""
+    grad = torch.is_grad_enabled()
+    index = tensors[0].get_device() if isinstance(tensors[0], torch.Tensor) else -1
+    if index >= 0 and not _is_compiling():
+        for t in tensors:
+            if (type(t) not in _PLAIN or t.get_device() != index or t.is_neg()
+                    or (grad and t.requires_grad)):
+                break
+        else:
+            if (_interpreter() is None and _forward_ad._current_level < 0 and not _is_tracing()
+                    and not _dispatch_modes() and (not _function_modes() or _only_device_modes())):
+                return index
+    require_device(*tensors)
+    require_plain(fn, *tensors)
+    return tensors[0].get_device()
+
+
 def index32(t: torch.Tensor, name: str, shape: tuple) -> torch.Tensor:
     """``t`` as a contiguous int32 tensor of ``shape`` (itself where it is one)."""
     if t.shape != shape:
@@ -284,6 +312,11 @@ def on_device(device: torch.device):
     if device.index is None or device.index == torch.cuda.current_device():
         return _SAME_DEVICE
     return torch.cuda.device(device)
+
+
+def at_index(index: int):
+    """:func:`on_device` of a device index."""
+    return _SAME_DEVICE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
 raw_stream = torch._C._cuda_getCurrentRawStream  # of a device index

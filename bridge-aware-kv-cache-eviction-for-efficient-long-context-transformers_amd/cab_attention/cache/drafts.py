@@ -53,22 +53,21 @@ def append_drafts(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cac
     es = _SIZES.get(dt)
     if es is None or v.dtype is not dt or k_cache.dtype is not dt or v_cache.dtype is not dt:
         raise TypeError("k, v and the caches must be of one dtype: bfloat16, float16 or float32")
-    dev = nat.require_device(k, v, k_cache, v_cache, lengths)
-    nat.require_plain("append_drafts", k, v, k_cache, v_cache)
-    _writable("append_drafts", k_cache, v_cache)
+    dev = nat.plain_index("append_drafts", k, v, k_cache, v_cache, lengths)
+    if k_cache.is_inference() or v_cache.is_inference():
+        _writable("append_drafts", k_cache, v_cache)
     lengths = nat.index32(lengths, "lengths", (B,))
     if counts is not None:
-        nat.require_device(k, counts)
+        nat.plain_index("append_drafts", k, counts)
         counts = nat.index32(counts, "counts", (B,))
-    k_st, v_st, kc_st, vc_st = k.stride(), v.stride(), k_cache.stride(), v_cache.stride()
-    ks, kc = nat.I64x4(*k_st), nat.I64x4(*kc_st)
-    with nat.on_device(dev):
+    arr = nat.stride_array
+    with nat.at_index(dev):
         st = nat.load().cab_kv_append_at(
             k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), es, B, H, n, D,
-            shape[2], ks, ks if v_st == k_st else nat.I64x4(*v_st), kc,
-            kc if vc_st == kc_st else nat.I64x4(*vc_st), lengths.data_ptr(), nat.ptr(counts),
-            nat.stream_ptr(dev))
-    nat.check("cab_kv_append_at", st)
+            shape[2], arr(k.stride()), arr(v.stride()), arr(k_cache.stride()), arr(v_cache.stride()),
+            lengths.data_ptr(), nat.ptr(counts), nat.raw_stream(dev))
+    if st:
+        nat.check("cab_kv_append_at", st)
     nat.wrote(k_cache, v_cache)
 
 
@@ -95,17 +94,20 @@ def commit_drafts(caches: Sequence[torch.Tensor], lengths: torch.Tensor, path: t
         raise ValueError("caches must be [B, H, N, D] and path [B, T]")
     if es is None:
         raise TypeError(f"unsupported dtype {dt}; expected float32, float16 or bfloat16")
-    for c in caches:
+    B = shape[0]
+    alike, grad = ref.get_device(), torch.is_grad_enabled()
+    for c in caches:  # (every layer's K and V: as few questions as there can be)
         if c.shape != shape or c.dtype is not dt or c.stride() != stride:
             raise ValueError("the caches must share one shape, dtype and stride set")
-    B, H, N, D = shape
-    dev = nat.require_device(lengths, path, counts, *caches)
-    nat.require_plain("commit_drafts", *caches)
-    _writable("commit_drafts", *caches)
+        if (type(c) is not torch.Tensor or c.get_device() != alike or c.is_inference()
+                or (grad and c.requires_grad)):
+            nat.plain_index("commit_drafts", ref, c)
+            _writable("commit_drafts", c)
+    dev = nat.plain_index("commit_drafts", ref, lengths, path, counts)
     lengths = nat.index32(lengths, "lengths", (B,))
     counts = nat.index32(counts, "counts", (B,))
     path = nat.index32(path, "path", (B, path.shape[1]))
-    new = torch.empty(B, dtype=torch.int32, device=dev)
+    new = torch.empty_like(counts)
     _commit(caches, lengths, 0, path, counts, 0, new, dev, es)
     return new
 
@@ -117,12 +119,13 @@ def _commit(caches, lengths, length, path, counts, count, new, dev, es, columns=
     if columns is not None:  # rows as values of another size
         D, st = columns, tuple(x * columns // D for x in st[:3]) + (1,)
     ptrs = (ctypes.c_void_p * n)(*[c.data_ptr() for c in caches])
-    with nat.on_device(dev):
+    with nat.at_index(dev):
         status = nat.load().cab_kv_commit(
-            ptrs, n, es, B, H, N, D, nat.I64x4(*st), nat.ptr(lengths), length, path.data_ptr(),
+            ptrs, n, es, B, H, N, D, nat.stride_array(st), nat.ptr(lengths), length, path.data_ptr(),
             path.shape[-1], path.shape[-1] if path.dim() == 2 else 0, nat.ptr(counts), count,
-            nat.ptr(new), nat.stream_ptr(dev))
-    nat.check("cab_kv_commit", status)
+            nat.ptr(new), nat.raw_stream(dev))
+    if status:
+        nat.check("cab_kv_commit", status)
     nat.wrote(*caches)
 
 
@@ -131,8 +134,7 @@ def commit_rows(caches: Sequence[torch.Tensor], path: torch.Tensor, length: int,
     the drafts, of which every sequence keeps ``count`` (int32 path ``[B, T]``, or ``[T]`` for
     all). Rows of any dtype whose bytes are a multiple of 4."""
     ref = caches[0]
-    nat.require_device(path, *caches)
-    nat.require_plain("commit", *caches)
+    dev = nat.plain_index("commit", path, *caches)
     _writable("commit", *caches)
-    _commit(caches, None, length, path, None, count, None, ref.device, 4,
+    _commit(caches, None, length, path, None, count, None, dev, 4,
             ref.shape[3] * ref.element_size() // 4)

@@ -43,38 +43,37 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, parents: t
     if not (q.dtype is k.dtype is v.dtype):
         raise TypeError("q, k, v dtypes differ")
     H_kv, N = k.shape[1], k.shape[2]
-    dev = nat.require_device(q, k, v, parents)
-    nat.require_plain("tree_attention", q, k, v)
+    if lengths is None:
+        dev = nat.plain_index("tree_attention", q, k, v, parents)
+    else:
+        dev = nat.plain_index("tree_attention", q, k, v, parents, lengths)
+        lengths = nat.index32(lengths, "lengths", (B,))
     dt = nat.dtype_code(q)
     shared = parents.dim() == 1
     parents = nat.index32(parents, "parents", (T,) if shared else (B, T))
-    if lengths is not None:
-        nat.require_device(q, lengths)
-        lengths = nat.index32(lengths, "lengths", (B,))
     if out is None:
-        out = torch.empty((B, H, T, D), dtype=q.dtype, device=dev)
+        out = q.new_empty((B, H, T, D))
     else:
         if out.shape != q.shape or out.dtype is not q.dtype:
             raise ValueError("out must match q's shape and dtype")
-        nat.require_device(q, out)
-        nat.require_plain("tree_attention", out)
+        nat.plain_index("tree_attention", q, out)
         if nat.closed(out):
             raise RuntimeError("tree_attention: out is an inference tensor; write to it in "
                                "inference mode")
     q, k, v = nat.aligned_rows(q), nat.aligned_rows(k), nat.aligned_rows(v)
-    lse = torch.empty((B, H, T), dtype=torch.float32, device=dev) if return_lse else None
+    lse = q.new_empty((B, H, T), dtype=torch.float32) if return_lse else None
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     lib = nat.load()
-    ks = nat.strides4(k)
-    ws = torch.empty(max(16, lib.cab_tree_attn_workspace_bytes(dt, B, H, H_kv, T, N, D)),
-                     dtype=torch.uint8, device=dev)
-    with nat.on_device(dev):
+    arr = nat.stride_array
+    wbytes = lib.cab_tree_attn_workspace_bytes(dt, B, H, H_kv, T, N, D)
+    ws = q.new_empty(wbytes or 16, dtype=torch.uint8)
+    with nat.at_index(dev):
         st = lib.cab_tree_attn_fwd(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, B, H, H_kv, T, N, D, nat.strides4(q), ks,
-            ks if v.stride() == k.stride() else nat.strides4(v), nat.strides4(out),
-            parents.data_ptr(), 0 if shared else T, nat.ptr(lengths),
-            0 if lengths is not None else N - T, scale, out.data_ptr(), nat.ptr(lse), ws.data_ptr(),
-            ws.numel(), nat.stream_ptr(dev))
-    nat.check("cab_tree_attn_fwd", st)
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, B, H, H_kv, T, N, D, arr(q.stride()),
+            arr(k.stride()), arr(v.stride()), arr(out.stride()), parents.data_ptr(),
+            0 if shared else T, nat.ptr(lengths), 0 if lengths is not None else N - T, scale, out.data_ptr(), nat.ptr(lse), ws.data_ptr(),
+            wbytes, nat.raw_stream(dev))
+    if st:
+        nat.check("cab_tree_attn_fwd", st)
     return (out, lse) if return_lse else out

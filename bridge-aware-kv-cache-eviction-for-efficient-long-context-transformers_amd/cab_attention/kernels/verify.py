@@ -4,14 +4,11 @@ The reference decodes one token at a time and has no counterpart."""
 
 from __future__ import annotations
 
-import ctypes
 from typing import Optional, Tuple
 
 import torch
 
 from .. import _native as nat
-
-_I64x2 = ctypes.c_int64 * 2
 
 
 def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor,
@@ -46,8 +43,7 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Ten
     if logits.dim() != 3:
         raise ValueError(f"logits must be [B, T, V]; got {list(logits.shape)}")
     B, T, V = logits.shape
-    dev = nat.require_device(logits, tokens, parents)
-    nat.require_plain("verify_drafts", logits)
+    dev = nat.plain_index("verify_drafts", logits, tokens, parents)
     dt = nat.dtype_code(logits)
     if tokens.shape != (B, T):
         raise ValueError(f"tokens must be {[B, T]}; got {list(tokens.shape)}")
@@ -64,34 +60,34 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Ten
     else:
         if uniforms is None or noise is None:
             raise ValueError("sampling (temperature > 0) needs uniforms and noise")
-        nat.require_device(logits, uniforms, noise)
+        nat.plain_index("verify_drafts", logits, uniforms, noise)
         for t, name, shape in ((uniforms, "uniforms", (B, T)), (noise, "noise", (B, V))):
             if t.shape != shape or t.dtype is not torch.float32:
                 raise ValueError(f"{name} must be fp32 {list(shape)}; got {t.dtype} {list(t.shape)}")
         uniforms, noise = uniforms.contiguous(), noise.contiguous()
     if logits.stride(2) != 1:
         logits = logits.contiguous()
-    ls = ds = _I64x2(logits.stride(0), logits.stride(1))
+    ls = ds = nat.stride_array(logits.stride()[:2])
     if draft_logits is not None:
         if draft_logits.shape != logits.shape or draft_logits.dtype is not logits.dtype:
             raise ValueError("draft_logits must match logits' shape and dtype")
-        nat.require_device(logits, draft_logits)
-        nat.require_plain("verify_drafts", draft_logits)
+        nat.plain_index("verify_drafts", logits, draft_logits)
         if draft_logits.stride(2) != 1:
             draft_logits = draft_logits.contiguous()
-        ds = _I64x2(draft_logits.stride(0), draft_logits.stride(1))
+        ds = nat.stride_array(draft_logits.stride()[:2])
     lib = nat.load()
     wbytes = lib.cab_verify_drafts_workspace_bytes(dt, B, T, V, temperature == 0.0,
                                                    draft_logits is not None)
-    ws = torch.empty(wbytes, dtype=torch.uint8, device=dev) if wbytes else None
-    path = torch.empty((B, T), dtype=torch.int32, device=dev)
-    counts = torch.empty(B, dtype=torch.int32, device=dev)
-    chosen = torch.empty(B, dtype=torch.int64, device=dev)
-    with nat.on_device(dev):
+    ws = logits.new_empty(wbytes, dtype=torch.uint8) if wbytes else None
+    path = parents.new_empty((B, T))
+    counts = parents.new_empty(B)
+    chosen = tokens.new_empty(B)
+    with nat.at_index(dev):
         st = lib.cab_verify_drafts(
             logits.data_ptr(), nat.ptr(draft_logits), dt, B, T, V, ls, ds, tokens.data_ptr(),
             parents.data_ptr(), 0 if shared else T, nat.ptr(uniforms), nat.ptr(noise), temperature,
             path.data_ptr(), counts.data_ptr(), chosen.data_ptr(), nat.ptr(ws), wbytes,
-            nat.stream_ptr(dev))
-    nat.check("cab_verify_drafts", st)
+            nat.raw_stream(dev))
+    if st:
+        nat.check("cab_verify_drafts", st)
     return path, counts, chosen

@@ -701,7 +701,8 @@ constexpr int64_t STATS_BYTES = int64_t{1} << 28;
 VerifyPlan verify_plan(cab_dtype_t dtype, int mode, int64_t B, int64_t T, int64_t V) {
   VerifyPlan p = {};
   const int64_t es = static_cast<int64_t>(dtype_size(dtype)), rows = B * T, sides = mode == DRAFT ? 2 : 1;
-  p.stats = rows * sides <= STATS_BYTES / (V * es);
+  // (stats_kernel's threads: 256 a slice, within 32 bits)
+  p.stats = rows * sides <= STATS_BYTES / (V * es) && rows <= (int64_t{1} << 23);
   // At most 64 slices a row (one wave merges them), and no more than fill the chip: a
   // slice is at least `loads` 16-byte loads a thread. (32 trees of 32 rows: 2048 workgroups
   // of statistics 68 us the call, 4096 60, 16384 62; 512 that pick 60, 1024 58, 2048 59.)
@@ -721,7 +722,8 @@ VerifyPlan verify_plan(cab_dtype_t dtype, int mode, int64_t B, int64_t T, int64_
 }
 
 bool verify_sizes(int64_t B, int64_t T, int64_t V) {
-  return T >= 1 && T <= MAX_NODES && B >= 1 && B <= INT32_MAX / 64 / T && V >= 1 && V <= INT32_MAX / 2;
+  // (walk_kernel's threads: 1024 a sequence, within 32 bits)
+  return T >= 1 && T <= MAX_NODES && B >= 1 && B <= (int64_t{1} << 21) && V >= 1 && V <= INT32_MAX / 2;
 }
 
 template <cab_dtype_t DT, int MODE>

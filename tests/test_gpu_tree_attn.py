@@ -167,6 +167,26 @@ def test_large_scores(cuda, dt):
     np.testing.assert_allclose(np64(out), w_out, atol=ATOL[dt] + 7e-3, rtol=0)
 
 
+@pytest.mark.parametrize("dt,H,T", [("bf16", 1, 1), ("bf16", 3, 7), ("fp32", 2, 2), ("fp16", 4, 40)])
+@pytest.mark.parametrize("B,Hkv", [(70, 1), (131, 1), (17, 1), (33, 2)])
+def test_many_sequences(cuda, B, Hkv, dt, H, T):
+    """More sequences than a wave has lanes, more units than a quarter of the workgroups (whose
+    stretches then run from one unit into the next), empty contexts among them."""
+    from cab_attention.kernels import tree_attention
+    N, D = 700 + T, 64
+    rng = np.random.default_rng(B)
+    n = np.where(rng.random(B) < 0.3, 0, rng.integers(0, 701, B))
+    n[0], n[-1] = 0, 700
+    q, k, v = rand((B, H * Hkv, T, D), dt, 1, 1.3), rand((B, Hkv, N, D), dt, 2), rand((B, Hkv, N, D), dt, 3)
+    parents = trees(B, T, "tree", 2)
+    want = S.tree_attention(np64(q), np64(k), np64(v), parents, n)
+    for b in range(B):
+        v[b, :, n[b] + T:] = float("nan")
+    got = tree_attention(q.to(cuda), k.to(cuda), v.to(cuda), torch.tensor(parents).to(cuda),
+                         torch.tensor(n).to(cuda), return_lse=True)
+    close(*got, want, dt)
+
+
 def test_far_rows(cuda):
     """A cache whose last sequence lies past 2^32 bytes, its context read at the end of it."""
     from cab_attention.kernels import tree_attention

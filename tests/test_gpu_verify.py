@@ -84,6 +84,51 @@ def test_against_oracle(cuda, T, V, shape, mode, dt):
 
 
 @pytest.mark.parametrize("mode", ["greedy", "point", "draft"])
+def test_rows_one_after_another(cuda, mode):
+    """Logits past the size up to which all rows' statistics are taken."""
+    from cab_attention.kernels import verify_drafts
+    g = torch.Generator(device=cuda).manual_seed(8)
+    B, T, V = 4, 32, 600_001
+    t = 0.0 if mode == "greedy" else 0.8
+    logits = torch.randn((B, T, V), generator=g, device=cuda)  # 307 MB
+    top = torch.randint(0, V, (B, T, 3), generator=g, device=cuda)
+    logits.scatter_(2, top, 14 + 3 * torch.rand((B, T, 3), generator=g, device=cuda))
+    logits[:, :, -7:] = -torch.inf
+    drafts = None
+    if mode == "draft":
+        drafts = logits + 0.3 * torch.randn((B, T, V), generator=g, device=cuda)
+    parents = torch.tensor([-1] + [i // 2 for i in range(T - 1)], dtype=torch.int32)
+    tokens = top[:, [max(p, 0) for p in parents.tolist()], 0].clone()
+    tokens[:, 1::2] = torch.randint(0, V, (B, T // 2), generator=g, device=cuda)
+    if mode == "greedy":
+        tokens[:, 2::2] = logits.argmax(2)[:, parents[2::2].tolist()]
+    u = torch.rand((B, T), generator=g, device=cuda)
+    noise = torch.empty((B, V), device=cuda).exponential_(generator=g)
+    got = verify_drafts(logits, tokens, parents.to(cuda), u, noise, t, drafts)
+    for b in range(B):
+        path, token, m = S.verify(logits[b].cpu().numpy(), tokens[b].tolist(), parents.tolist(),
+                                  u[b].cpu().numpy(), noise[b].cpu().numpy(), t,
+                                  None if drafts is None else drafts[b].cpu().numpy())
+        assert m > MARGIN
+        assert got[0][b, :len(path)].tolist() == path and int(got[1][b]) == len(path)
+        assert int(got[2][b]) == token
+
+
+@pytest.mark.parametrize("mode", ["greedy", "point"])
+def test_equal_scores_go_to_the_lowest_index(cuda, mode):
+    """Equal logits (and equal noise) far apart in a long row, in every slice of it."""
+    from cab_attention.kernels import verify_drafts
+    V = 130_000
+    logits = torch.zeros((1, 1, V), device=cuda)
+    logits[0, 0, [V - 1, 77_777, 31_000, 65_536]] = 3.0
+    ones = torch.ones((1, V), device=cuda)
+    token = verify_drafts(logits, torch.zeros((1, 1), dtype=torch.int64, device=cuda),
+                          torch.tensor([-1], device=cuda), torch.zeros((1, 1), device=cuda), ones,
+                          0.0 if mode == "greedy" else 0.7)[2]
+    assert token.tolist() == [31_000]
+
+
+@pytest.mark.parametrize("mode", ["greedy", "point", "draft"])
 def test_long_walks(cuda, mode):
     """Certain drafts: the whole chain is taken."""
     x = make(3, 40, 500, "fp32", mode, "chain", 5, 0.0 if mode == "greedy" else 1.0)
