@@ -4,9 +4,10 @@
 // every layer (cab_kv_commit). lengths, counts and paths are read on the device, so
 // a decode loop needs no read-back and can be captured.
 //
-// A step moves little: B = 4, 8 heads, D = 128, bf16, 64 drafts, 6 accepted: 1 MB a
+// A step moves little: 4 sequences, 8 heads, D = 128, bf16, 64 drafts, up to 6 accepted: 1 MB a
 // layer in, at most 0.1 MB a layer moved. What counts is launches: one per layer for
-// K and V together, one per 64 tensors for the compaction.
+// K and V together (3.4 us there, 2.3 for 5 drafts of one sequence), one per 64 tensors for the
+// compaction (4.9 us for 32 layers, 3.6 for 28).
 #include "cab_internal.h"
 
 namespace cab {

@@ -8,8 +8,8 @@
 //     list, and each workgroup takes an equal stretch of it, whatever the lengths. Of
 //     each unit that its stretch touches it leaves one partial (maximum m, row sum l,
 //     unnormalised O) per row:
-//     - rows_kernel (up to 32 rows, and fp32): every wave walks its own 32-key steps, K
-//       and V straight from memory into matrix operands;
+//     - rows_kernel (few rows, and fp32, on the fp32 matrix instructions): every wave walks
+//       its own 32-key steps, K and V straight from memory into matrix operands;
 //     - tile_kernel (more rows, 16 bits): 64-key tiles of K and V in LDS, read by all
 //       waves, each of which holds 16 or 32 rows.
 //     Both compute S^T = K Q^T, an online softmax in the log2 domain (maxima, sums and O
@@ -18,18 +18,24 @@
 //     sees, found by walking its ancestors: a node has few of them, and no other
 //     draft's K or V is touched, so nothing a row does not see can reach it.
 //
-// Bound: HBM (the context's K and V, read once) up to about 256 rows in 16 bits, the
-// matrix cores beyond.
+// Bound: HBM (the context's K and V, read once) for few rows; for many the chain of one
+// tile (operand reads, products, maxima, exponentials, products), of which two waves a
+// SIMD overlap little. Measured, 32 query heads on 8, D = 128, bf16: one token of 16
+// sequences of up to 32768 keys 191 + 5.6 us (contexts + join; some 6.8 TB/s of K and V); a
+// tree of 64 over 65472 keys 84 + 12 us (816 TFLOP/s), over 8128 23 + 12 us, of which the
+// partials of 256 workgroups (33 MB out and in) are about a third.
 #include "attn_common.h"
 
 namespace cab {
 namespace {
 
 constexpr int MAX_NODES = 256;
-constexpr int STEP = 32;  // keys of a wave's step in rows_kernel
+constexpr int STEP = 32;        // keys of a wave's step in rows_kernel
 constexpr int QUAD = 4 * STEP;  // its pieces: a step for each of four waves
 constexpr int TILE = 64;        // tile_kernel's pieces
-constexpr int FEW_PIECES = 32;  // of an even cut, up to which stretches begin anew with every unit
+// Pieces a workgroup of an even cut, up to which stretches begin anew with every unit (us, so
+// -> running on: 256 rows, 8 units of 8128 keys 33.5 -> 40.7, of 65472 99 -> 104).
+constexpr int FEW_PIECES = 32;
 
 struct TreeArgs {
   const char* q;
@@ -221,181 +227,181 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void rows_kernel(TreeAr
   const uint32_t krow = static_cast<uint32_t>(a.ks[2]), vrow = static_cast<uint32_t>(a.vs[2]);
 
   over_stretch<QUAD>(a, blockIdx.x, [&](int b, int hk, int piece, int pieces, int len) {
-  int lane = lane_id();
-  asm volatile("" : "+v"(lane));  // (what follows from it is not kept over the parts)
-  const int l16 = lane & 15, g = lane >> 4;
-  const char* kb = a.k + b * a.ks[0] + hk * a.ks[1];
-  const char* vb = a.v + b * a.vs[0] + hk * a.vs[1];
-  u32x4 qr[QT][NJ];
+    int lane = lane_id();
+    asm volatile("" : "+v"(lane));  // (what follows from it is not kept over the parts)
+    const int l16 = lane & 15, g = lane >> 4;
+    const char* kb = a.k + b * a.ks[0] + hk * a.ks[1];
+    const char* vb = a.v + b * a.vs[0] + hk * a.vs[1];
+    u32x4 qr[QT][NJ];
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    const int r = row0 + 16 * qt + l16;
-    const int hg = r / a.T, t = r - hg * a.T;
-    const char* qp = a.q + b * a.qs[0] + (static_cast<int64_t>(hk) * a.group + hg) * a.qs[1] + t * a.qs[2];
+    for (int qt = 0; qt < QT; ++qt) {
+      const int r = row0 + 16 * qt + l16;
+      const int hg = r / a.T, t = r - hg * a.T;
+      const char* qp = a.q + b * a.qs[0] + (static_cast<int64_t>(hk) * a.group + hg) * a.qs[1] + t * a.qs[2];
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      qr[qt][j] = u32x4{0u, 0u, 0u, 0u};
-      if (r < a.R) qr[qt][j] = *reinterpret_cast<const u32x4*>(qp + 64 * j + 16 * g);
+      for (int j = 0; j < NJ; ++j) {
+        qr[qt][j] = u32x4{0u, 0u, 0u, 0u};
+        if (r < a.R) qr[qt][j] = *reinterpret_cast<const u32x4*>(qp + 64 * j + 16 * g);
+      }
     }
-  }
-  f32x4 o[QT][NDT];
-  float l[QT], m[QT];  // l: of this lane's keys alone
+    f32x4 o[QT][NDT];
+    float l[QT], m[QT];  // l: of this lane's keys alone
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    l[qt] = 0.f;
-    m[qt] = M_EMPTY;
+    for (int qt = 0; qt < QT; ++qt) {
+      l[qt] = 0.f;
+      m[qt] = M_EMPTY;
 #pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) o[qt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+      for (int dt = 0; dt < NDT; ++dt) o[qt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
 
-  auto load = [&](int step, SR& x) {
-    const int left = len - STEP * step;
-    const char* kp = kb + static_cast<int64_t>(STEP * step) * krow;
-    const char* vp = vb + static_cast<int64_t>(STEP * step) * vrow;
-    if (left >= STEP)
-      load_step<DT, HD, false>(x, kp, vp, krow, vrow, left, l16, g);
-    else
-      load_step<DT, HD, true>(x, kp, vp, krow, vrow, left, l16, g);
-  };
-  auto compute = [&](int step, const SR& x) {
-    const int left = len - STEP * step;
-    f32x4 sc[QT][2];  // [qt][tt][r]: key 16 tt + 4 g + r, row 16 qt + l16
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt) sc[qt][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-          if constexpr (F32) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t kx = x.k[tt][j][e], qx = qr[qt][j][e];
-              sc[qt][tt] = mfma4(__uint_as_float(kx), __uint_as_float(qx), sc[qt][tt]);
-            }
-          } else {
-            sc[qt][tt] = mfma16<BF16>(x.k[tt][j], qr[qt][j], sc[qt][tt]);
-          }
-        }
-    if (left < STEP) {
+    auto load = [&](int step, SR& x) {
+      const int left = len - STEP * step;
+      const char* kp = kb + static_cast<int64_t>(STEP * step) * krow;
+      const char* vp = vb + static_cast<int64_t>(STEP * step) * vrow;
+      if (left >= STEP)
+        load_step<DT, HD, false>(x, kp, vp, krow, vrow, left, l16, g);
+      else
+        load_step<DT, HD, true>(x, kp, vp, krow, vrow, left, l16, g);
+    };
+    auto compute = [&](int step, const SR& x) {
+      const int left = len - STEP * step;
+      f32x4 sc[QT][2];  // [qt][tt][r]: key 16 tt + 4 g + r, row 16 qt + l16
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) sc[qt][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) {
+            if constexpr (F32) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t kx = x.k[tt][j][e], qx = qr[qt][j][e];
+                sc[qt][tt] = mfma4(__uint_as_float(kx), __uint_as_float(qx), sc[qt][tt]);
+              }
+            } else {
+              sc[qt][tt] = mfma16<BF16>(x.k[tt][j], qr[qt][j], sc[qt][tt]);
+            }
+          }
+      if (left < STEP) {
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (16 * tt + 4 * g + r >= left) sc[qt][tt][r] = -INFINITY;
+      }
+      u32x4 pb[QT];
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        const float m0 = fmaxf(fmaxf(sc[qt][0][0], sc[qt][0][1]), fmaxf(sc[qt][0][2], sc[qt][0][3]));
+        const float m1 = fmaxf(fmaxf(sc[qt][1][0], sc[qt][1][1]), fmaxf(sc[qt][1][2], sc[qt][1][3]));
+        float mx = fmaxf(m0, m1), mdup = mx;
+        colmax2(mx, mdup);
+        if (__builtin_amdgcn_ballot_w64(mx > m[qt]) != 0) {
+          const float mn = fmaxf(mx, m[qt]);
+          const float alpha = __builtin_amdgcn_exp2f((m[qt] - mn) * c);
+          l[qt] *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < NDT; ++dt) o[qt][dt] *= alpha;
+          m[qt] = mn;
+        }
+        const float nmc = -m[qt] * c;
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (16 * tt + 4 * g + r >= left) sc[qt][tt][r] = -INFINITY;
+            sc[qt][tt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qt][tt][r], c, nmc));
+        const f32x4 s2 = sc[qt][0] + sc[qt][1];
+        l[qt] += (s2[0] + s2[1]) + (s2[2] + s2[3]);
+        if constexpr (!F32)
+          pb[qt] = u32x4{pack2<BF16>(sc[qt][0][0], sc[qt][0][1]), pack2<BF16>(sc[qt][0][2], sc[qt][0][3]),
+                         pack2<BF16>(sc[qt][1][0], sc[qt][1][1]), pack2<BF16>(sc[qt][1][2], sc[qt][1][3])};
+      }
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) {
+        if constexpr (F32) {
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            const uint32_t vx = x.v[r][dt >> 1][dt & 1];
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+              o[qt][dt] = mfma4(__uint_as_float(vx), sc[qt][r >> 2][r & 3], o[qt][dt]);
+          }
+        } else {
+          u32x4 vo;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t lo = x.v[2 * e][dt >> 2][(dt >> 1) & 1];
+            const uint32_t hi = x.v[2 * e + 1][dt >> 2][(dt >> 1) & 1];
+            vo[e] = __builtin_amdgcn_perm(hi, lo, dt & 1 ? 0x07060302u : 0x05040100u);
+          }
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) o[qt][dt] = mfma16<BF16>(vo, pb[qt], o[qt][dt]);
+        }
+      }
+    };
+
+    const int end = min((len + STEP - 1) / STEP, 4 * (piece + pieces));
+    int step = 4 * piece + w;
+    if constexpr (F32 || QT * HD > 128) {  // (two register sets would spill)
+      SR x;
+      for (; step < end; step += 4) {
+        load(step, x);
+        compute(step, x);
+      }
+    } else {
+      // Two register sets: a step's loads are in flight while the one before it is computed.
+      SR x, y;
+      if (step < end) load(step, x);
+      for (; step < end; step += 8) {
+        if (step + 4 < end) load(step + 4, y);
+        compute(step, x);
+        if (step + 4 < end) {
+          if (step + 8 < end) load(step + 8, x);
+          compute(step + 4, y);
+        }
+      }
     }
-    u32x4 pb[QT];
+
+    // Merge of the four waves: common maximum, then the scaled O^T and sums in wave order.
+    const int64_t part = static_cast<int64_t>(blockIdx.x) + b * a.Hkv + hk;
+    __syncthreads();  // (the last part's merge has been read)
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-      const float m0 = fmaxf(fmaxf(sc[qt][0][0], sc[qt][0][1]), fmaxf(sc[qt][0][2], sc[qt][0][3]));
-      const float m1 = fmaxf(fmaxf(sc[qt][1][0], sc[qt][1][1]), fmaxf(sc[qt][1][2], sc[qt][1][3]));
-      float mx = fmaxf(m0, m1), mdup = mx;
-      colmax2(mx, mdup);
-      if (__builtin_amdgcn_ballot_w64(mx > m[qt]) != 0) {
-        const float mn = fmaxf(mx, m[qt]);
-        const float alpha = __builtin_amdgcn_exp2f((m[qt] - mn) * c);
-        l[qt] *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) o[qt][dt] *= alpha;
-        m[qt] = mn;
-      }
-      const float nmc = -m[qt] * c;
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          sc[qt][tt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qt][tt][r], c, nmc));
-      const f32x4 s2 = sc[qt][0] + sc[qt][1];
-      l[qt] += (s2[0] + s2[1]) + (s2[2] + s2[3]);
-      if constexpr (!F32)
-        pb[qt] = u32x4{pack2<BF16>(sc[qt][0][0], sc[qt][0][1]), pack2<BF16>(sc[qt][0][2], sc[qt][0][3]),
-                       pack2<BF16>(sc[qt][1][0], sc[qt][1][1]), pack2<BF16>(sc[qt][1][2], sc[qt][1][3])};
+      l[qt] += shfl_xor_f32(l[qt], 16);
+      l[qt] += shfl_xor_f32(l[qt], 32);
+      if (g == 0) sm[w][qt][l16] = m[qt];
     }
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) {
-      if constexpr (F32) {
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          const uint32_t vx = x.v[r][dt >> 1][dt & 1];
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt)
-            o[qt][dt] = mfma4(__uint_as_float(vx), sc[qt][r >> 2][r & 3], o[qt][dt]);
-        }
-      } else {
-        u32x4 vo;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t lo = x.v[2 * e][dt >> 2][(dt >> 1) & 1];
-          const uint32_t hi = x.v[2 * e + 1][dt >> 2][(dt >> 1) & 1];
-          vo[e] = __builtin_amdgcn_perm(hi, lo, dt & 1 ? 0x07060302u : 0x05040100u);
-        }
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) o[qt][dt] = mfma16<BF16>(vo, pb[qt], o[qt][dt]);
-      }
-    }
-  };
-
-  const int end = min((len + STEP - 1) / STEP, 4 * (piece + pieces));
-  int step = 4 * piece + w;
-  if constexpr (F32 || QT * HD > 128) {  // (two register sets would spill)
-    SR x;
-    for (; step < end; step += 4) {
-      load(step, x);
-      compute(step, x);
-    }
-  } else {
-    // Two register sets: a step's loads are in flight while the one before it is computed.
-    SR x, y;
-    if (step < end) load(step, x);
-    for (; step < end; step += 8) {
-      if (step + 4 < end) load(step + 4, y);
-      compute(step, x);
-      if (step + 4 < end) {
-        if (step + 8 < end) load(step + 8, x);
-        compute(step + 4, y);
-      }
-    }
-  }
-
-  // Merge of the four waves: common maximum, then the scaled O^T and sums in wave order.
-  const int64_t part = static_cast<int64_t>(blockIdx.x) + b * a.Hkv + hk;
-  __syncthreads();  // (the last part's merge has been read)
-#pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    l[qt] += shfl_xor_f32(l[qt], 16);
-    l[qt] += shfl_xor_f32(l[qt], 32);
-    if (g == 0) sm[w][qt][l16] = m[qt];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    const float mm = fmaxf(fmaxf(sm[0][qt][l16], sm[1][qt][l16]), fmaxf(sm[2][qt][l16], sm[3][qt][l16]));
-    const float f = __builtin_amdgcn_exp2f((m[qt] - mm) * c);
-    if (g == 0) sl[w][qt][l16] = l[qt] * f;
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) merge[w][dt * 64 + lane] = o[qt][dt] * f;
     __syncthreads();
-    for (int e = threadIdx.x; e < NDT * 64; e += 256) {
-      const int dt = e >> 6, ll = e & 63, row = row0 + 16 * qt + (ll & 15);
-      const f32x4 y = (merge[0][e] + merge[1][e]) + (merge[2][e] + merge[3][e]);
-      if (row < a.R) {
-        float* po = a.po + (part * a.R + row) * HD;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) po[NDT * (4 * (ll >> 4) + r) + dt] = y[r];
+    for (int qt = 0; qt < QT; ++qt) {
+      const float mm = fmaxf(fmaxf(sm[0][qt][l16], sm[1][qt][l16]), fmaxf(sm[2][qt][l16], sm[3][qt][l16]));
+      const float f = __builtin_amdgcn_exp2f((m[qt] - mm) * c);
+      if (g == 0) sl[w][qt][l16] = l[qt] * f;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) merge[w][dt * 64 + lane] = o[qt][dt] * f;
+      __syncthreads();
+      for (int e = threadIdx.x; e < NDT * 64; e += 256) {
+        const int dt = e >> 6, ll = e & 63, row = row0 + 16 * qt + (ll & 15);
+        const f32x4 y = (merge[0][e] + merge[1][e]) + (merge[2][e] + merge[3][e]);
+        if (row < a.R) {
+          float* po = a.po + (part * a.R + row) * HD;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) po[NDT * (4 * (ll >> 4) + r) + dt] = y[r];
+        }
       }
+      const int row = row0 + 16 * qt + static_cast<int>(threadIdx.x);
+      if (threadIdx.x < 16 && row < a.R) {
+        a.pm[part * a.R + row] = mm * c;
+        a.pl[part * a.R + row] = (sl[0][qt][l16] + sl[1][qt][l16]) + (sl[2][qt][l16] + sl[3][qt][l16]);
+      }
+      if (qt + 1 < QT) __syncthreads();
     }
-    const int row = row0 + 16 * qt + static_cast<int>(threadIdx.x);
-    if (threadIdx.x < 16 && row < a.R) {
-      a.pm[part * a.R + row] = mm * c;
-      a.pl[part * a.R + row] = (sl[0][qt][l16] + sl[1][qt][l16]) + (sl[2][qt][l16] + sl[3][qt][l16]);
-    }
-    if (qt + 1 < QT) __syncthreads();
-  }
   });
 }
 
@@ -444,171 +450,171 @@ __global__ __launch_bounds__(64 * WAVES, 2) void tile_kernel(TreeArgs a) {
   const float c = a.c;
 
   over_stretch<TILE>(a, wg, [&](int b, int hk, int begin, int pieces, int len) {
-  int lane = lane_id();
-  asm volatile("" : "+v"(lane));  // (what follows from it is not kept over the parts)
-  const int l16 = lane & 15, g = lane >> 4;
-  const int end = begin + pieces;
-  const char* kb = a.k + b * a.ks[0] + hk * a.ks[1];
-  const char* vb = a.v + b * a.vs[0] + hk * a.vs[1];
-  // A lane's row in a wave's first load and its place there. Lane i's 16 bytes land at
-  // 16 i, so each lane fetches the chunk that tile_offset() looks for at its place.
-  // (A round of loads further on the swizzle is the same.)
-  const uint32_t lrow = w * (64 / CH) + lane / CH;
-  const uint32_t lch = tile_offset<HD>(lrow, lane % CH) % (16 * CH);
-  const uint32_t koff = lrow * static_cast<uint32_t>(a.ks[2]) + lch;
-  const uint32_t voff = lrow * static_cast<uint32_t>(a.vs[2]) + lch;
-  auto load = [&](int tile, int slot) {
-    const int left = len - tile * TILE;
-    constexpr uint32_t END = 0xffffffe0u;  // rows past the context: an offset past it, read as zero
-    const sgpr_rsrc_t kr = make_sgpr_rsrc(kb + static_cast<int64_t>(tile) * TILE * a.ks[2], END);
-    const sgpr_rsrc_t vr = make_sgpr_rsrc(vb + static_cast<int64_t>(tile) * TILE * a.vs[2], END);
+    int lane = lane_id();
+    asm volatile("" : "+v"(lane));  // (what follows from it is not kept over the parts)
+    const int l16 = lane & 15, g = lane >> 4;
+    const int end = begin + pieces;
+    const char* kb = a.k + b * a.ks[0] + hk * a.ks[1];
+    const char* vb = a.v + b * a.vs[0] + hk * a.vs[1];
+    // A lane's row in a wave's first load and its place there. Lane i's 16 bytes land at
+    // 16 i, so each lane fetches the chunk that tile_offset() looks for at its place.
+    // (A round of loads further on the swizzle is the same.)
+    const uint32_t lrow = w * (64 / CH) + lane / CH;
+    const uint32_t lch = tile_offset<HD>(lrow, lane % CH) % (16 * CH);
+    const uint32_t koff = lrow * static_cast<uint32_t>(a.ks[2]) + lch;
+    const uint32_t voff = lrow * static_cast<uint32_t>(a.vs[2]) + lch;
+    auto load = [&](int tile, int slot) {
+      const int left = len - tile * TILE;
+      constexpr uint32_t END = 0xffffffe0u;  // rows past the context: an offset past it, read as zero
+      const sgpr_rsrc_t kr = make_sgpr_rsrc(kb + static_cast<int64_t>(tile) * TILE * a.ks[2], END);
+      const sgpr_rsrc_t vr = make_sgpr_rsrc(vb + static_cast<int64_t>(tile) * TILE * a.vs[2], END);
 #pragma unroll
-    for (int n = 0; n < LOADS; ++n) {
-      const uint32_t ks = n * ROWS * static_cast<uint32_t>(a.ks[2]);
-      const uint32_t vs = n * ROWS * static_cast<uint32_t>(a.vs[2]);
-      char* kt = &lds[slot][0][(n * WAVES + w) * 1024];
-      char* vt = &lds[slot][1][(n * WAVES + w) * 1024];
-      if (left >= TILE) {
-        dma16(kr, koff, ks, kt);
-        dma16(vr, voff, vs, vt);
-      } else {
-        const bool in = static_cast<int>(lrow) + n * ROWS < left;
-        dma16(kr, in ? koff + ks : END, 0, kt);
-        dma16(vr, in ? voff + vs : END, 0, vt);
+      for (int n = 0; n < LOADS; ++n) {
+        const uint32_t ks = n * ROWS * static_cast<uint32_t>(a.ks[2]);
+        const uint32_t vs = n * ROWS * static_cast<uint32_t>(a.vs[2]);
+        char* kt = &lds[slot][0][(n * WAVES + w) * 1024];
+        char* vt = &lds[slot][1][(n * WAVES + w) * 1024];
+        if (left >= TILE) {
+          dma16(kr, koff, ks, kt);
+          dma16(vr, voff, vs, vt);
+        } else {
+          const bool in = static_cast<int>(lrow) + n * ROWS < left;
+          dma16(kr, in ? koff + ks : END, 0, kt);
+          dma16(vr, in ? voff + vs : END, 0, vt);
+        }
+      }
+    };
+    lds_barrier();  // the last part's tiles have been read
+    load(begin, 0);
+
+    u32x4 qr[QT][NDS];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const int r = row0 + 16 * qt + l16;
+      const int hg = r / a.T, t = r - hg * a.T;
+      const char* qp = a.q + b * a.qs[0] + (static_cast<int64_t>(hk) * a.group + hg) * a.qs[1] + t * a.qs[2];
+#pragma unroll
+      for (int ds = 0; ds < NDS; ++ds) {
+        qr[qt][ds] = u32x4{0u, 0u, 0u, 0u};
+        if (r < a.R) qr[qt][ds] = *reinterpret_cast<const u32x4*>(qp + 64 * ds + 16 * g);
       }
     }
-  };
-  lds_barrier();  // the last part's tiles have been read
-  load(begin, 0);
-
-  u32x4 qr[QT][NDS];
+    f32x4 o[QT][NDT];  // [dt][r]: d = 16 dt + 4 g + r
+    float l[QT], m[QT];
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    const int r = row0 + 16 * qt + l16;
-    const int hg = r / a.T, t = r - hg * a.T;
-    const char* qp = a.q + b * a.qs[0] + (static_cast<int64_t>(hk) * a.group + hg) * a.qs[1] + t * a.qs[2];
+    for (int qt = 0; qt < QT; ++qt) {
+      l[qt] = 0.f;
+      m[qt] = M_EMPTY;
 #pragma unroll
-    for (int ds = 0; ds < NDS; ++ds) {
-      qr[qt][ds] = u32x4{0u, 0u, 0u, 0u};
-      if (r < a.R) qr[qt][ds] = *reinterpret_cast<const u32x4*>(qp + 64 * ds + 16 * g);
+      for (int dt = 0; dt < NDT; ++dt) o[qt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-  }
-  f32x4 o[QT][NDT];  // [dt][r]: d = 16 dt + 4 g + r
-  float l[QT], m[QT];
-#pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    l[qt] = 0.f;
-    m[qt] = M_EMPTY;
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) o[qt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
 
-  // (held here, so that nothing in the loop waits for them and with them for the tiles)
-#pragma unroll
-  for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-    for (int ds = 0; ds < NDS; ++ds) asm volatile("" : "+v"(qr[qt][ds]));
-
-  auto step = [&](int tile, const int slot) __attribute__((always_inline)) {
-    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-    lds_barrier();
-    if (tile + 1 < end) load(tile + 1, slot ^ 1);
-    const char* kt = lds[slot][0];
-    const char* vt = lds[slot][1];
-    f32x4 sc[QT][4];  // [qt][tt][r]: key 16 tt + 4 g + r, row 16 qt + l16
+    // (held here, so that nothing in the loop waits for them and with them for the tiles)
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt) sc[qt][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int ds = 0; ds < NDS; ++ds)
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt) {
-        const u32x4 kf = *reinterpret_cast<const u32x4*>(kt + tile_offset<HD>(16 * tt + l16, 4 * ds + g));
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) sc[qt][tt] = mfma16<BF16>(kf, qr[qt][ds], sc[qt][tt]);
-      }
-    const int left = len - tile * TILE;
-    if (left < TILE) {
+      for (int ds = 0; ds < NDS; ++ds) asm volatile("" : "+v"(qr[qt][ds]));
+
+    auto step = [&](int tile, const int slot) __attribute__((always_inline)) {
+      asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+      lds_barrier();
+      if (tile + 1 < end) load(tile + 1, slot ^ 1);
+      const char* kt = lds[slot][0];
+      const char* vt = lds[slot][1];
+      f32x4 sc[QT][4];  // [qt][tt][r]: key 16 tt + 4 g + r, row 16 qt + l16
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) sc[qt][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ds = 0; ds < NDS; ++ds)
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+          const u32x4 kf = *reinterpret_cast<const u32x4*>(kt + tile_offset<HD>(16 * tt + l16, 4 * ds + g));
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) sc[qt][tt] = mfma16<BF16>(kf, qr[qt][ds], sc[qt][tt]);
+        }
+      const int left = len - tile * TILE;
+      if (left < TILE) {
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+          for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (16 * tt + 4 * g + r >= left) sc[qt][tt][r] = -INFINITY;
+      }
+      float mx[2];
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        f32x4 y;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          y[r] = fmaxf(fmaxf(sc[qt][0][r], sc[qt][1][r]), fmaxf(sc[qt][2][r], sc[qt][3][r]));
+        mx[qt] = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
+      }
+      if constexpr (QT == 1) mx[1] = mx[0];
+      colmax2(mx[0], mx[1]);
+      u32x4 pb[QT][2];
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        if (__builtin_amdgcn_ballot_w64(mx[qt] > m[qt]) != 0) {
+          const float mn = fmaxf(mx[qt], m[qt]);
+          const float alpha = __builtin_amdgcn_exp2f((m[qt] - mn) * c);
+          l[qt] *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < NDT; ++dt) o[qt][dt] *= alpha;
+          m[qt] = mn;
+        }
+        const float nmc = -m[qt] * c;
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (16 * tt + 4 * g + r >= left) sc[qt][tt][r] = -INFINITY;
-    }
-    float mx[2];
+            sc[qt][tt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qt][tt][r], c, nmc));
+        const f32x4 s4 = (sc[qt][0] + sc[qt][1]) + (sc[qt][2] + sc[qt][3]);
+        l[qt] += (s4[0] + s4[1]) + (s4[2] + s4[3]);
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-      f32x4 y;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        y[r] = fmaxf(fmaxf(sc[qt][0][r], sc[qt][1][r]), fmaxf(sc[qt][2][r], sc[qt][3][r]));
-      mx[qt] = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
-    }
-    if constexpr (QT == 1) mx[1] = mx[0];
-    colmax2(mx[0], mx[1]);
-    u32x4 pb[QT][2];
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-      if (__builtin_amdgcn_ballot_w64(mx[qt] > m[qt]) != 0) {
-        const float mn = fmaxf(mx[qt], m[qt]);
-        const float alpha = __builtin_amdgcn_exp2f((m[qt] - mn) * c);
-        l[qt] *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) o[qt][dt] *= alpha;
-        m[qt] = mn;
+        for (int hh = 0; hh < 2; ++hh)
+          pb[qt][hh] = u32x4{pack2<BF16>(sc[qt][2 * hh][0], sc[qt][2 * hh][1]),
+                             pack2<BF16>(sc[qt][2 * hh][2], sc[qt][2 * hh][3]),
+                             pack2<BF16>(sc[qt][2 * hh + 1][0], sc[qt][2 * hh + 1][1]),
+                             pack2<BF16>(sc[qt][2 * hh + 1][2], sc[qt][2 * hh + 1][3])};
       }
-      const float nmc = -m[qt] * c;
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          sc[qt][tt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qt][tt][r], c, nmc));
-      const f32x4 s4 = (sc[qt][0] + sc[qt][1]) + (sc[qt][2] + sc[qt][3]);
-      l[qt] += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+      // V^T operand of keys 32 hh ..: k-slot 8 g + e is key 16 (e / 4) + 4 g + e % 4.
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh)
-        pb[qt][hh] = u32x4{pack2<BF16>(sc[qt][2 * hh][0], sc[qt][2 * hh][1]),
-                           pack2<BF16>(sc[qt][2 * hh][2], sc[qt][2 * hh][3]),
-                           pack2<BF16>(sc[qt][2 * hh + 1][0], sc[qt][2 * hh + 1][1]),
-                           pack2<BF16>(sc[qt][2 * hh + 1][2], sc[qt][2 * hh + 1][3])};
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) {
+          const uint32_t row = 32 * hh + 4 * g + (l16 >> 2);
+          const uint32_t ch = 2 * dt + ((l16 & 3) >> 1), in = 8 * (l16 & 1);
+          const u32x2 v0 = lds_read_tr16(vt + tile_offset<HD>(row, ch) + in);
+          const u32x2 v1 = lds_read_tr16(vt + tile_offset<HD>(row + 16, ch) + in);
+          const u32x4 vf = {v0[0], v0[1], v1[0], v1[1]};
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) o[qt][dt] = mfma16<BF16>(vf, pb[qt][hh], o[qt][dt]);
+        }
+    };
+    // (a slot's LDS addresses are constants of its own copy of the step)
+    for (int tile = begin; tile < end; tile += 2) {
+      step(tile, 0);
+      if (tile + 1 < end) step(tile + 1, 1);
     }
-    // V^T operand of keys 32 hh ..: k-slot 8 g + e is key 16 (e / 4) + 4 g + e % 4.
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh)
+    for (int qt = 0; qt < QT; ++qt) {
+      l[qt] += shfl_xor_f32(l[qt], 16);
+      l[qt] += shfl_xor_f32(l[qt], 32);
+      const int row = row0 + 16 * qt + l16;
+      if (row >= a.R) continue;
+      const int64_t x = (static_cast<int64_t>(wg) + b * a.Hkv + hk) * a.R + row;
 #pragma unroll
-      for (int dt = 0; dt < NDT; ++dt) {
-        const uint32_t row = 32 * hh + 4 * g + (l16 >> 2);
-        const uint32_t ch = 2 * dt + ((l16 & 3) >> 1), in = 8 * (l16 & 1);
-        const u32x2 v0 = lds_read_tr16(vt + tile_offset<HD>(row, ch) + in);
-        const u32x2 v1 = lds_read_tr16(vt + tile_offset<HD>(row + 16, ch) + in);
-        const u32x4 vf = {v0[0], v0[1], v1[0], v1[1]};
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) o[qt][dt] = mfma16<BF16>(vf, pb[qt][hh], o[qt][dt]);
+      for (int dt = 0; dt < NDT; ++dt)
+        *reinterpret_cast<f32x4*>(a.po + x * HD + 16 * dt + 4 * g) = o[qt][dt];
+      if (g == 0) {
+        a.pm[x] = m[qt] * c;
+        a.pl[x] = l[qt];
       }
-  };
-  // (a slot's LDS addresses are constants of its own copy of the step)
-  for (int tile = begin; tile < end; tile += 2) {
-    step(tile, 0);
-    if (tile + 1 < end) step(tile + 1, 1);
-  }
-#pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    l[qt] += shfl_xor_f32(l[qt], 16);
-    l[qt] += shfl_xor_f32(l[qt], 32);
-    const int row = row0 + 16 * qt + l16;
-    if (row >= a.R) continue;
-    const int64_t x = (static_cast<int64_t>(wg) + b * a.Hkv + hk) * a.R + row;
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt)
-      *reinterpret_cast<f32x4*>(a.po + x * HD + 16 * dt + 4 * g) = o[qt][dt];
-    if (g == 0) {
-      a.pm[x] = m[qt] * c;
-      a.pl[x] = l[qt];
     }
-  }
   });
 }
 
