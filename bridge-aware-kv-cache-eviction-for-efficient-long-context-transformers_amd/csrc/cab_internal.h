@@ -185,9 +185,12 @@ __device__ __forceinline__ void bdma16_untracked(const sgpr_rsrc_t& r, uint32_t 
                                                  const void* l) {
   const uint32_t lds = static_cast<uint32_t>(
       __builtin_amdgcn_readfirstlane(static_cast<int>(reinterpret_cast<uintptr_t>(l))));
-  // M0 (the LDS base of the load) is an input the compiler sets; the s_nop
-  // is the wait state an LDS load needs after an M0 write.
-  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
+  // M0 (the LDS base of the load) and the scalars are inputs the compiler sets, whose wait
+  // states it does not count for an asm block: one after an M0 write, five after a vector
+  // instruction (make_sgpr_rsrc's readfirstlane) wrote a scalar the load reads. Four here and
+  // the M0 write before them are five. (Three more than the M0 write alone needs: the
+  // block-sparse executor 3.40 -> 3.42 ms.)
+  asm volatile("s_nop 3\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
                :
                : "v"(voff), "s"(r), "s"(soff), "{m0}"(lds)
                : "memory");
