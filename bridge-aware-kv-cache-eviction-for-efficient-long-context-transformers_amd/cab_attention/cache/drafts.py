@@ -16,6 +16,7 @@ One step of a loop over static buffers ``[B, H_kv, N, D]`` per layer::
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Sequence
 
 import torch
@@ -23,6 +24,11 @@ import torch
 from .. import _native as nat
 
 _SIZES = {torch.bfloat16: 2, torch.float16: 2, torch.float32: 4}
+
+
+@functools.lru_cache(maxsize=1024)
+def _four_strides(*strides: tuple):
+    return tuple(nat.stride_array(x) for x in strides)
 
 
 def _writable(fn: str, *caches: torch.Tensor) -> None:
@@ -42,11 +48,11 @@ def append_drafts(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cac
     would lie behind the cache's N, and those of a sequence of negative length, are
     not written. The new rows must not be views of the caches.
     """
-    if k.dim() != 4 or v.shape != k.shape:
+    new, shape = k.shape, k_cache.shape
+    if len(new) != 4 or v.shape != new:
         raise ValueError("k and v must be two [B, H, n, D] tensors")
-    B, H, n, D = k.shape
-    shape = k_cache.shape
-    if len(shape) != 4 or v_cache.shape != shape or shape[:2] != (B, H) or shape[3] != D:
+    B, H, n, D = new
+    if len(shape) != 4 or v_cache.shape != shape or (shape[0], shape[1], shape[3]) != (B, H, D):
         raise ValueError(f"k_cache and v_cache must be [{B}, {H}, N, {D}]; got {tuple(shape)} and "
                          f"{tuple(v_cache.shape)}")
     dt = k.dtype
@@ -60,12 +66,11 @@ def append_drafts(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cac
     if counts is not None:
         nat.plain_index("append_drafts", k, counts)
         counts = nat.index32(counts, "counts", (B,))
-    arr = nat.stride_array
+    strides = _four_strides(k.stride(), v.stride(), k_cache.stride(), v_cache.stride())
     with nat.at_index(dev):
         st = nat.load().cab_kv_append_at(
             k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), es, B, H, n, D,
-            shape[2], arr(k.stride()), arr(v.stride()), arr(k_cache.stride()), arr(v_cache.stride()),
-            lengths.data_ptr(), nat.ptr(counts), nat.raw_stream(dev))
+            shape[2], *strides, lengths.data_ptr(), nat.ptr(counts), nat.raw_stream(dev))
     if st:
         nat.check("cab_kv_append_at", st)
     nat.wrote(k_cache, v_cache)

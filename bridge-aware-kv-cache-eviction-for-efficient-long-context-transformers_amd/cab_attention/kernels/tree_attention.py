@@ -60,6 +60,7 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, parents: t
         if nat.closed(out):
             raise RuntimeError("tree_attention: out is an inference tensor; write to it in "
                                "inference mode")
+        nat.wrote(out)
     q, k, v = nat.aligned_rows(q), nat.aligned_rows(k), nat.aligned_rows(v)
     lse = q.new_empty((B, H, T), dtype=torch.float32) if return_lse else None
     if scale is None:

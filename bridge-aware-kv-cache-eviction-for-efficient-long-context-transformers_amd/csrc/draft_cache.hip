@@ -203,6 +203,7 @@ extern "C" cab_status_t cab_kv_commit(void* const* tensors, int32_t n_tensors,
                   length0 <= rows,
               CAB_ESHAPE, "%s: problem too large", fn);
   CAB_REQUIRE(strides[3] == 1, CAB_ESHAPE, "%s: the last-dim stride must be 1", fn);
+  CAB_REQUIRE(path_stride == 0 || path_stride >= nodes, CAB_ESHAPE, "%s: bad path stride", fn);
   CAB_REQUIRE(new_lengths == nullptr || new_lengths != lengths, CAB_EINVAL,
               "%s: the new lengths cannot be written over the old ones", fn);
   const int64_t es = element_bytes;

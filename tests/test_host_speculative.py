@@ -49,7 +49,7 @@ def test_commit_validation(lib):
     one = (ctypes.c_void_p * 2)(FAKE, FAKE + 4096)
     call = lambda **w: lib.cab_kv_commit(
         w.get("t", one), w.get("nt", 2), w.get("es", 2), w.get("B", 1), w.get("H", 2), w.get("N", 90), 64,
-        w.get("st", st), w.get("len", FAKE), w.get("l0", 0), w.get("path", FAKE), 5, 5, FAKE,
+        w.get("st", st), w.get("len", FAKE), w.get("l0", 0), w.get("path", FAKE), 5, w.get("ps", 5), FAKE,
         w.get("c0", 0), w.get("new", FAKE + 64), None)
     assert call(es=3) == nat.CAB_EDTYPE
     assert call(nt=0) == nat.CAB_ESHAPE
@@ -58,6 +58,7 @@ def test_commit_validation(lib):
     assert call(l0=91) == nat.CAB_ESHAPE
     assert call(c0=-1) == nat.CAB_EINVAL
     assert call(path=None) == nat.CAB_EINVAL
+    assert call(ps=4) == nat.CAB_ESHAPE
     assert call(t=(ctypes.c_void_p * 2)(FAKE, None)) == nat.CAB_EINVAL
     assert call(t=(ctypes.c_void_p * 2)(FAKE, FAKE)) == nat.CAB_EINVAL
     assert b"twice" in lib.cab_last_error()
