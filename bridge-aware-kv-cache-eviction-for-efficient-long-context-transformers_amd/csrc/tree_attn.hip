@@ -798,6 +798,10 @@ struct TreePlan {
 // 19.7, but 16 sequences of 32768 keys 208 -> 238, and 20 rows, 8 of 16384 65 -> 72.
 constexpr int FEW_ROWS = 32, FEWER_ROWS = 16;
 constexpr int64_t LONG_LIST = int64_t{1} << 18;
+// Lists up to which 129 to 256 rows go in two tiles of 128 with stretches twice as long, which
+// halves the partials (us, one tile of 256 -> so: 8 units of 500 keys 21.5 -> 18.4, of 8128
+// 33.6 -> 30.5, 16 of up to 5936 32.1 -> 28.5; 8 of 65472 97 -> 119).
+constexpr int64_t BRIEF_LIST = int64_t{1} << 17;
 // Workgroups that share the list: one a CU (rows_kernel; 512: 4 rows, 16 x 32768 keys 202 us
 // against 198, fp32, 256 rows of 4032 keys 84 against 70), or as many as the registers
 // allow: one of 8 waves, two of 4 (256: 64 rows, 8 x 8192 keys 54 us against 49).
@@ -817,12 +821,13 @@ TreePlan tree_plan(cab_dtype_t dtype, int64_t B, int64_t H, int64_t Hkv, int64_t
     p.least = 1;
     keys = QUAD;
   } else {
-    p.tile = p.R <= 64 ? 64 : p.R <= 128 ? 128 : 256;
+    const bool halves = p.R > 128 && p.R <= 256 && p.units * most <= BRIEF_LIST;
+    p.tile = p.R <= 64 ? 64 : p.R <= 128 || halves ? 128 : 256;
     p.row_tiles = ceil_div(p.R, p.tile);
     // (two tiles a workgroup at least; four of the small ones at D = 128 in all but short
     // lists: 64 rows of 8 x 8176 keys 19.9 us against 22.1, 20 of 8 x 595 15.1 against 12.9)
     p.least = p.tile < 256 && D == 128 && p.units * most > 512 * TILE ? 4 : 2;
-    if (p.tile < 256) slots = SMALL_TILE_WGS;
+    if (p.tile < 256 && !halves) slots = SMALL_TILE_WGS;
     keys = TILE;
   }
   // No more workgroups than the longest contexts have stretches.

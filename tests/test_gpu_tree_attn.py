@@ -112,6 +112,21 @@ def test_long_context_of_one_length(cuda, dt, H, T):
     close(*got, want, dt)
 
 
+@pytest.mark.parametrize("dt,D,H,T,N", [("bf16", 128, 4, 35, 66200), ("fp16", 64, 5, 30, 66000),
+                                        ("bf16", 64, 2, 16, 140000), ("fp16", 128, 1, 20, 140000)])
+def test_long_lists(cuda, dt, D, H, T, N):
+    """Lists past the sizes that send 129 to 256 rows to tiles of 128 and 17 to 32 to tiles: two
+    heads of K and V and contexts of very unlike lengths."""
+    from cab_attention.kernels import tree_attention
+    B, Hkv = 2, 2
+    q, k, v = rand((B, H * Hkv, T, D), dt, 1, 1.3), rand((B, Hkv, N, D), dt, 2), rand((B, Hkv, N, D), dt, 3)
+    parents, n = trees(B, T, "tree", 4), [N - T, 700]
+    want = S.tree_attention(np64(q), np64(k), np64(v), parents, n)
+    got = tree_attention(q.to(cuda), k.to(cuda), v.to(cuda), torch.tensor(parents).to(cuda),
+                         torch.tensor(n).to(cuda), return_lse=True)
+    close(*got, want, dt)
+
+
 @pytest.mark.parametrize("dt", list(DT))
 @pytest.mark.parametrize("T", [6, 40])
 def test_unseen_values_reach_nobody(cuda, dt, T):
