@@ -133,6 +133,19 @@ def test_tree_attention_validation(lib):
     assert call(B=0) == nat.CAB_OK
 
 
+def test_tree_attention_refuses_an_out_whose_rows_overlap(lib):
+    qs, ks = s4(8 * 16 * 128, 16 * 128, 128, 1), s4(2 * 500 * 128, 500 * 128, 128, 1)
+    call = lambda os, T=16, wsb=0: lib.cab_tree_attn_fwd(
+        FAKE, FAKE, FAKE, nat.CAB_BF16, 2, 8, 2, T, 500, 128, qs, ks, ks, os, FAKE, 0, None, 484, 0.1,
+        FAKE, None, FAKE, wsb, None)
+    assert call(s4(0, 16 * 128, 128, 1)) == nat.CAB_ESHAPE
+    assert call(s4(8 * 16 * 128, 0, 128, 1)) == nat.CAB_ESHAPE
+    assert call(s4(8 * 16 * 128, 16 * 128, 64, 1)) == nat.CAB_ESHAPE
+    # (the next check refuses these: a single row has no stride)
+    assert call(qs) == nat.CAB_EWORKSPACE
+    assert call(s4(8 * 128, 128, 0, 1), T=1) == nat.CAB_EWORKSPACE
+
+
 def test_python_refusals():
     from cab_attention.cache import append_drafts, commit_drafts
     from cab_attention.kernels import tree_attention, verify_drafts
