@@ -22,8 +22,8 @@
 // tile (operand reads, products, maxima, exponentials, products), of which two waves a
 // SIMD overlap little. Measured, 32 query heads on 8, D = 128, bf16: one token of 16
 // sequences of up to 32768 keys 191 + 5.6 us (contexts + join; some 6.8 TB/s of K and V); a
-// tree of 64 over 65472 keys 84 + 12 us (816 TFLOP/s), over 8128 23 + 12 us, of which the
-// partials of 256 workgroups (33 MB out and in) are about a third.
+// tree of 64 over 65472 keys 84 + 12 us (816 TFLOP/s), over 8128 22.6 + 8.6 us, of which the
+// partials of 256 workgroups (17 MB out and in) are some 5.
 #include "attn_common.h"
 
 namespace cab {
