@@ -32,6 +32,8 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, parents: t
         scale: defaults to ``1/sqrt(D)``.
 
     What a node does not see cannot reach its output, not even as a NaN or an infinity.
+    A node that is there and whose scores have no softmax (a NaN or +inf among them, or
+    all -inf) has NaN for its output and its log-sum-exp.
     Returns the output ``[B, H, T, D]``, with ``return_lse`` also the fp32 natural-log
     log-sum-exp ``[B, H, T]``.
     """

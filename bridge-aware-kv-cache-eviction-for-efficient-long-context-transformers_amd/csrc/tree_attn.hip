@@ -769,7 +769,7 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
       o[e] *= f;
 #pragma unroll
       for (int off = LG; off < 64; off <<= 1) o[e] += shfl_xor_f32(o[e], off);
-      o[e] *= l == 0.f ? 0.f : 1.0f / l;
+      o[e] *= 1.0f / l;  // (l 0, all scores -inf: 0 / 0)
     }
   }
   if (grp != 0) return;
@@ -781,8 +781,17 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
     *reinterpret_cast<u32x4*>(op) = u32x4{pack2<BF16>(o[0], o[1]), pack2<BF16>(o[2], o[3]),
                                           pack2<BF16>(o[4], o[5]), pack2<BF16>(o[6], o[7])};
   }
-  if (at == 0 && a.lse)
-    a.lse[id] = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
+  // -inf is for absent nodes alone: a node that is there and has no softmax (a score of NaN or
+  // +inf, or all of them -inf: l is NaN or 0) has NaN for both results. l's bits are tested
+  // because this file is compiled with -fno-honor-nans.
+  if (at == 0 && a.lse) {
+    int32_t bits = __builtin_bit_cast(int32_t, l);
+    asm("" : "+v"(bits));  // (or the test is made one of floats)
+    const float sum = (m + __log2f(l)) * 0.69314718055994531f;
+    uint32_t x = bits > 0 && bits <= 0x7f800000 ? __builtin_bit_cast(uint32_t, sum) : 0x7fc00000u;
+    if (!present) x = 0xff800000u;
+    reinterpret_cast<uint32_t*>(a.lse)[id] = x;
+  }
 }
 
 // How a problem is cut. tile: rows of a tile_kernel workgroup (0: rows_kernel).

@@ -474,7 +474,8 @@ cab_status_t cab_kv_commit(void* const* tensors, int32_t n_tensors, int32_t elem
  * see nothing and are seen by nobody). out[b,h,i] = softmax_s(q_i . k_s * scale) v_s
  * over those keys (0 for no node), lse[b,h,i] the natural-log log-sum-exp of the
  * scaled scores (-inf for no node), lse may be NULL. Keys a node does not see do
- * not reach it whatever they hold.
+ * not reach it whatever they hold. A node that is there and whose scores have no softmax
+ * (a NaN or +inf among them, or all -inf) has NaN for both.
  * q, out: [B,H,T,D]; k, v: [B,H_kv,N,D] (strides); H % H_kv == 0; D == 64 or 128;
  * T <= 256; bf16, fp16 (products of 16-bit operands, P rounded to 16 bits, sums in
  * fp32) or fp32 (fp32 throughout). Token strides of k and v in [0, 2^25] bytes.
