@@ -50,7 +50,7 @@ struct TreeArgs {
   // Partials. Workgroup x's of unit u is number x + u: down the list either x or u goes
   // up by one from one partial to the next.
   float* po;  // [number][R][D]
-  float* pm;  // [number][R] maxima of the scores * c
+  float* pm;  // [number][R] level_of the maximum score
   float* pl;  // [number][R] row sums
 };
 
@@ -154,6 +154,25 @@ __device__ __forceinline__ void over_stretch(const TreeArgs& a, int x, F f) {
   }
 }
 
+// What weights are relative to, 2^(s c - level), for the maximum m: m c, and in fp16 15 less. There
+// weights of at most 1 would lose digits from 6e-5 and be 0 from 3e-8 down, which a long
+// context behind one large score adds up (140000 keys 17.4 below it: 0.4 % of the row sum
+// missing in O); 2^15 more, fp16's last power of two, keeps 11 bits to 1.9e-9. Beyond 2^24 the
+// level's own rounding is more than half a power of two, and nothing is added. (The factor in
+// s - m instead, one operation more a score, has no such border: 4 trees of 64 over 65472 keys 346
+// -> 355 us; levels formed anew in every step 334 -> 348, one token of 16 x 32768 209 -> 234.)
+template <cab_dtype_t DT>
+__device__ __forceinline__ float level_of(float m, float c) {
+  const float mc = m * c;
+  if constexpr (DT != CAB_F16) return mc;
+  return __builtin_fmaf(m, c, __builtin_fabsf(mc) < 16777216.f ? -15.f : 0.f);
+}
+// What sums relative to the maximum m's level are multiplied by for m1's.
+template <cab_dtype_t DT>
+__device__ __forceinline__ float relevel(float m, float level, float m1, float level1, float c) {
+  return __builtin_amdgcn_exp2f(DT == CAB_F16 ? level - level1 : (m - m1) * c);
+}
+
 // K and V are read once: non-temporal loads.
 template <typename T>
 __device__ __forceinline__ T ld_stream(const char* p) {
@@ -245,11 +264,12 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void rows_kernel(TreeAr
       }
     }
     f32x4 o[QT][NDT];
-    float l[QT], m[QT];  // l: of this lane's keys alone
+    float l[QT], m[QT], level[QT];  // l: of this lane's keys alone
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       l[qt] = 0.f;
       m[qt] = M_EMPTY;
+      level[qt] = level_of<DT>(M_EMPTY, c);
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt) o[qt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -304,18 +324,19 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void rows_kernel(TreeAr
         colmax2(mx, mdup);
         if (__builtin_amdgcn_ballot_w64(mx > m[qt]) != 0) {
           const float mn = fmaxf(mx, m[qt]);
-          const float alpha = __builtin_amdgcn_exp2f((m[qt] - mn) * c);
+          const float upto = level_of<DT>(mn, c);
+          const float alpha = relevel<DT>(m[qt], level[qt], mn, upto, c);
           l[qt] *= alpha;
 #pragma unroll
           for (int dt = 0; dt < NDT; ++dt) o[qt][dt] *= alpha;
           m[qt] = mn;
+          level[qt] = upto;
         }
-        const float nmc = -m[qt] * c;
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            sc[qt][tt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qt][tt][r], c, nmc));
+            sc[qt][tt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qt][tt][r], c, -level[qt]));
         const f32x4 s2 = sc[qt][0] + sc[qt][1];
         l[qt] += (s2[0] + s2[1]) + (s2[2] + s2[3]);
         if constexpr (!F32)
@@ -381,7 +402,8 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void rows_kernel(TreeAr
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       const float mm = fmaxf(fmaxf(sm[0][qt][l16], sm[1][qt][l16]), fmaxf(sm[2][qt][l16], sm[3][qt][l16]));
-      const float f = __builtin_amdgcn_exp2f((m[qt] - mm) * c);
+      const float upto = level_of<DT>(mm, c);
+      const float f = relevel<DT>(m[qt], level[qt], mm, upto, c);
       if (g == 0) sl[w][qt][l16] = l[qt] * f;
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt) merge[w][dt * 64 + lane] = o[qt][dt] * f;
@@ -397,7 +419,7 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void rows_kernel(TreeAr
       }
       const int row = row0 + 16 * qt + static_cast<int>(threadIdx.x);
       if (threadIdx.x < 16 && row < a.R) {
-        a.pm[part * a.R + row] = mm * c;
+        a.pm[part * a.R + row] = upto;
         a.pl[part * a.R + row] = (sl[0][qt][l16] + sl[1][qt][l16]) + (sl[2][qt][l16] + sl[3][qt][l16]);
       }
       if (qt + 1 < QT) __syncthreads();
@@ -500,11 +522,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void tile_kernel(TreeArgs a) {
       }
     }
     f32x4 o[QT][NDT];  // [dt][r]: d = 16 dt + 4 g + r
-    float l[QT], m[QT];
+    float l[QT], m[QT], level[QT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       l[qt] = 0.f;
       m[qt] = M_EMPTY;
+      level[qt] = level_of<DT>(M_EMPTY, c);
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt) o[qt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -560,18 +583,19 @@ __global__ __launch_bounds__(64 * WAVES, 2) void tile_kernel(TreeArgs a) {
       for (int qt = 0; qt < QT; ++qt) {
         if (__builtin_amdgcn_ballot_w64(mx[qt] > m[qt]) != 0) {
           const float mn = fmaxf(mx[qt], m[qt]);
-          const float alpha = __builtin_amdgcn_exp2f((m[qt] - mn) * c);
+          const float upto = level_of<DT>(mn, c);
+          const float alpha = relevel<DT>(m[qt], level[qt], mn, upto, c);
           l[qt] *= alpha;
 #pragma unroll
           for (int dt = 0; dt < NDT; ++dt) o[qt][dt] *= alpha;
           m[qt] = mn;
+          level[qt] = upto;
         }
-        const float nmc = -m[qt] * c;
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            sc[qt][tt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qt][tt][r], c, nmc));
+            sc[qt][tt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qt][tt][r], c, -level[qt]));
         const f32x4 s4 = (sc[qt][0] + sc[qt][1]) + (sc[qt][2] + sc[qt][3]);
         l[qt] += (s4[0] + s4[1]) + (s4[2] + s4[3]);
 #pragma unroll
@@ -611,7 +635,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void tile_kernel(TreeArgs a) {
       for (int dt = 0; dt < NDT; ++dt)
         *reinterpret_cast<f32x4*>(a.po + x * HD + 16 * dt + 4 * g) = o[qt][dt];
       if (g == 0) {
-        a.pm[x] = m[qt] * c;
+        a.pm[x] = level[qt];
         a.pl[x] = l[qt];
       }
     }

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import spec_oracle as S
-from test_gpu_tree_attn import ATOL, DT, LSE_ATOL, np64, rand
+from test_gpu_tree_attn import ATOL, DT, LSE_ATOL, np64, rand, trees
 
 pytestmark = pytest.mark.gpu
 
@@ -92,3 +92,55 @@ def test_totals_of_a_commit(cuda):
     totals = key_scores(q, k, lse, causal=True)
     assert not torch.isinf(totals).any() and torch.isnan(totals[0, 0, :39]).all()
     assert torch.isfinite(totals[0, 1]).all()
+
+
+@pytest.mark.parametrize("dt,sink", [("fp16", 34.8125), ("bf16", 34.75)])
+@pytest.mark.parametrize("H,T", [(1, 4), (2, 10), (4, 10), (5, 20), (10, 20)])
+def test_small_weights_add_up(cuda, dt, sink, H, T):
+    """One score 17.4 above 140000 others, whose V alone is not 0, in as many sequences as keep
+    a context in one workgroup's stretch: a weight of 2.8e-8 each, together 0.4 % of the row. All
+    weights are alike, so each result is n w / (1 + n w) for the n keys it sees; it is off by
+    half a step of a weight's rounding and half a step of its own, and by fp32 sums: l's of 2188
+    tiles onto 1 (2^-24 each, 1.4e-4), O's of twice as many products (2^-24 of it, 2.6e-4)."""
+    B, N, D, length = 512, 140000 + T, 64, 140000
+    from cab_attention.kernels import tree_attention
+    k = torch.zeros((1, 1, N, D), dtype=DT[dt], device=cuda)
+    v = torch.ones_like(k)
+    k[0, 0, 0, 0], v[0, 0, 0] = sink, 0
+    q = torch.zeros((B, H, T, D), dtype=DT[dt], device=cuda)
+    q[..., 0] = 4
+    parents = torch.arange(-1, T - 1, dtype=torch.int32, device=cuda)
+    out, lse = tree_attention(q, k.expand(B, 1, N, D), v.expand(B, 1, N, D), parents, return_lse=True)
+    w = np.exp(-4 * sink / 8)
+    n = length - 1 + np.arange(1, T + 1)  # a chain: node i sees i + 1 drafts
+    rel = torch.finfo(DT[dt]).eps
+    want = np.broadcast_to((n * w / (1 + n * w))[:, None], (T, D))
+    np.testing.assert_allclose(np64(out), np.broadcast_to(want, out.shape), rtol=rel + 4e-4, atol=0)
+    np.testing.assert_allclose(np64(lse), np.broadcast_to(4 * sink / 8 + np.log1p(n * w), lse.shape),
+                               atol=1.4e-4, rtol=0)
+
+
+@pytest.mark.parametrize("H,T", ROWS)
+@pytest.mark.parametrize("big", [1000, 9632, 9648, 9664, 30000])
+def test_large_fp16_scores(cuda, H, T, big):
+    """Scores of 1e5 to 1e8 in fp16, around the border past which weights are not scaled
+    up: keys of a few scores that fp32 holds exactly, one or two maxima away from each other,
+    the larger ones late. (The context's weights are all relative to one rounded level; a log-sum-exp
+    has five roundings of the score's size.)"""
+    from cab_attention.kernels import tree_attention
+    N, D = 1000 + T, 64
+    g = torch.Generator().manual_seed(T)
+    q, k = torch.zeros((1, H, T, D)), torch.zeros((1, 1, N, D))
+    q[..., 0], k[..., 0] = big, big
+    step = 64.0 if big > 20000 else 8.0  # a multiple of the step of big^2 in fp32
+    q[..., 1] = 1
+    k[..., 1] = step * torch.randint(0, 3, (N,), generator=g)
+    k[:, :, 700:1000, 1] += 8 * step  # (later, larger; the drafts weigh little)
+    v = rand((1, 1, N, D), "fp16", 3)
+    q, k = q.half(), k.half()
+    parents = trees(1, T, "tree", T)
+    want = S.tree_attention(np64(q), np64(k), np64(v), parents, [1000])
+    out, lse = tree_attention(q.to(cuda), k.to(cuda), v.to(cuda), torch.tensor(parents).int().to(cuda),
+                              torch.tensor([1000], dtype=torch.int32).to(cuda), return_lse=True)
+    np.testing.assert_allclose(np64(out), want[0], atol=ATOL["fp16"], rtol=0)
+    np.testing.assert_allclose(np64(lse), want[1], rtol=5 * 2 ** -24, atol=1e-5)
