@@ -134,12 +134,18 @@ def _commit(caches, lengths, length, path, counts, count, new, dev, es, columns=
     nat.wrote(*caches)
 
 
-def commit_rows(caches: Sequence[torch.Tensor], path: torch.Tensor, length: int, count: int) -> None:
-    """:func:`commit_drafts` for contiguous buffers of one length, ``length`` rows before
-    the drafts, of which every sequence keeps ``count`` (int32 path ``[B, T]``, or ``[T]`` for
-    all). Rows of any dtype whose bytes are a multiple of 4."""
-    ref = caches[0]
-    dev = nat.plain_index("commit", path, *caches)
-    _writable("commit", *caches)
-    _commit(caches, None, length, path, None, count, None, dev, 4,
-            ref.shape[3] * ref.element_size() // 4)
+def commit_rows(groups: Sequence[tuple], count: int) -> None:
+    """:func:`commit_drafts` for groups ``(caches, path, length)`` of contiguous buffers of
+    one shape and length, ``length`` rows before the drafts, of which every sequence keeps
+    ``count`` (int32 path ``[B, T]``, or ``[T]`` for all). Rows of any dtype whose bytes are
+    a multiple of 4. All groups are checked before the first row moves."""
+    devs = []
+    for caches, path, _ in groups:
+        devs.append(nat.plain_index("commit", path, *caches))
+        _writable("commit", *caches)
+        if caches[0].shape[0] > 65535 or len(caches) > 4096:
+            raise ValueError("commit takes up to 65535 sequences and 2048 layers of one geometry")
+    for (caches, path, length), dev in zip(groups, devs):
+        ref = caches[0]
+        _commit(caches, None, length, path, None, count, None, dev, 4,
+                ref.shape[3] * ref.element_size() // 4)

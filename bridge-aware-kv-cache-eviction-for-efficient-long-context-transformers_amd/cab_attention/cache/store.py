@@ -31,6 +31,7 @@ below which they never evict.
 
 from __future__ import annotations
 
+import math
 from typing import Any, Callable, Dict, List, Optional, Tuple
 
 import torch
@@ -108,7 +109,8 @@ class LayeredKV:
     def commit(self, path: torch.Tensor, count: int):
         """Keeps ``count`` of every present layer's drafted rows: those at ``path[b, :count]``
         (int32 ``[B, T]`` or ``[T]``, ascending), moved to the front of the drafts; the
-        other drafts are dropped. One launch per 64 tensors of one geometry."""
+        other drafts are dropped. One launch per 64 tensors of one geometry, on the GPU
+        only. What is refused leaves the store as it was."""
         present = [L for L in self.layers if L is not None]
         drafts = {L.drafted for L in present}
         if len(drafts) != 1 or drafts == {0}:
@@ -120,11 +122,14 @@ class LayeredKV:
         groups: Dict[tuple, List[_Layer]] = {}
         for L in present:
             groups.setdefault((tuple(L.k.shape), L.k.dtype, L.k.device, L.length), []).append(L)
-        for (shape, _, dev, length), members in groups.items() if count else ():
-            if path.dim() == 2 and path.shape[0] != shape[0]:
-                raise ValueError(f"path must be [{shape[0]}, {T}]; got {list(path.shape)}")
-            rows = nat.index32(path.to(dev), "path", tuple(path.shape))
-            commit_rows([L.k for L in members] + [L.v for L in members], rows, length, count)
+        if path.dim() == 2:
+            for shape, _, _, _ in groups:
+                if path.shape[0] != shape[0]:
+                    raise ValueError(f"path must be [{shape[0]}, {T}]; got {list(path.shape)}")
+        if count:
+            commit_rows([([L.k for L in members] + [L.v for L in members],
+                          nat.index32(path.to(dev), "path", tuple(path.shape)), length)
+                         for (_, _, dev, length), members in groups.items()], count)
         for L in present:
             L.length += count
             L.drafted = 0
@@ -289,31 +294,51 @@ class EvictingCache:
 
         query, lse: layer 0's queries ``[B, H, T, D]`` of the drafts and
         ``tree_attention``'s log-sum-exp ``[B, H, T]`` (``scale`` as there): the accepted
-        tokens' attention is added to the importance totals, as ``update``'s weights are."""
+        tokens' attention is added to the importance totals, as ``update``'s weights are.
+
+        A call that is refused leaves rows, lengths, drafts, totals and statistics as they
+        were. GPU only."""
         if (query is None) != (lse is None):
             raise ValueError("query and lse come together")
-        if query is not None:
-            if (query.dim() != 4 or query.shape[2] != path.shape[-1] or lse.shape != query.shape[:3]
-                    or query.shape[3] not in (64, 128) or self._store.view(0)[0] is None):
-                raise ValueError("query must be [B, H, T, D] of layer 0 with D = 64 or 128, lse "
-                                 f"[B, H, T] with T = {path.shape[-1]}")
         count = int(count)
+        if query is not None:
+            # (everything key_scores would refuse, before a row moves)
+            self._check_queries(path, query, lse, scale)
+            # The accepted path is a plain causal chain behind the context once committed.
+            rows = path.to(device=query.device, dtype=torch.int64).reshape(-1, path.shape[-1])
+            rows = rows[:, :max(count, 0)].clamp(0, path.shape[-1] - 1)  # (a padded path reads some row)
+            rows = rows.expand(query.shape[0], rows.shape[1])[:, None, :, None]
+            query = torch.take_along_dim(query, rows, 2)
+            lse = torch.take_along_dim(lse, rows[..., 0], 2)
         self._store.commit(path, count)
         if count == 0:
             return
         if query is not None:
-            # The accepted path is a plain causal chain behind the context now.
-            rows = path.to(device=query.device, dtype=torch.int64).reshape(-1, path.shape[-1])
-            rows = rows[:, :count].clamp(0, path.shape[-1] - 1)  # (a padded path reads some row)
-            rows = rows.expand(query.shape[0], count)[:, None, :, None]
             keys, _ = self._store.view(0)
-            totals = key_scores(torch.take_along_dim(query, rows, 2), keys,
-                                torch.take_along_dim(lse, rows[..., 0], 2), scale, causal=True)
+            totals = key_scores(query, keys, lse, scale, causal=True)
             self.importance_tracker.add_scores(totals.sum((0, 1)), count)
         layers = [L for L in self._store.layers if L is not None]
         self.stats["total_tokens_processed"] += count * len(layers)
         self.tokens_since_last_eviction += count * len(layers)
         self._evict_if_due(max(L.length for L in layers))
+
+    def _check_queries(self, path: torch.Tensor, query: torch.Tensor, lse: torch.Tensor,
+                       scale: Optional[float]):
+        keys, _ = self._store.view(0)
+        T = path.shape[-1]
+        if (keys is None or query.dim() != 4 or query.shape[2] != T or lse.shape != query.shape[:3]
+                or query.shape[3] not in (64, 128) or query.shape[0] != keys.shape[0]
+                or query.shape[3] != keys.shape[3] or query.shape[1] % max(keys.shape[1], 1)
+                or path.dim() > 2 or (path.dim() == 2 and path.shape[0] != query.shape[0])):
+            raise ValueError("query must be [B, H, T, D] of layer 0 with D = 64 or 128, lse "
+                             f"[B, H, T] with T = {T}")
+        if query.dtype != keys.dtype or lse.dtype != torch.float32:
+            raise TypeError(f"query must be {keys.dtype} as layer 0's keys are and lse float32; got "
+                            f"{query.dtype} and {lse.dtype}")
+        nat.dtype_code(query)
+        nat.require_device(query, keys, lse)
+        if scale is not None and not (math.isfinite(scale) and scale > 0):
+            raise ValueError(f"scale must be finite and > 0; got {scale}")
 
     def _evict_if_due(self, n: int):
         due = (n > int(self.max_cache_size * 1.1)
