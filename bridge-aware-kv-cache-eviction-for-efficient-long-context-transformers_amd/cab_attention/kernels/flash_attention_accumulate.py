@@ -111,7 +111,11 @@ def key_scores(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, scale: float
     """``scores[b, h, s] (+)= sum_t exp(q_t . k_s * scale - lse[b, h, t])``
     (``cab_attn_key_scores``), with the lse of :func:`flash_attention` on the
     same q, k. bf16, fp16 or fp32."""
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError("q and k must be [B, H, N, D]")
     B, H, N_q, D = q.shape
+    if k.shape[0] != B or k.shape[3] != D:
+        raise ValueError(f"k must be [B={B}, H_kv, N_k, D={D}]; got {tuple(k.shape)}")
     H_kv, N_k = k.shape[1], k.shape[2]
     if tuple(lse.shape) != (B, H, N_q) or lse.dtype != torch.float32:
         raise ValueError(f"lse must be fp32 [B, H, N_q] = {(B, H, N_q)}")

@@ -90,6 +90,17 @@ def test_groups_are_checked_first_on_the_host(monkeypatch):
     assert not moved and [(L.length, L.drafted) for L in store.layers] == [(N, T)] * 2
 
 
+def test_key_scores_refuses_keys_of_another_batch_or_head_dim():
+    """(Its kernel would read past them.)"""
+    from cab_attention.kernels import key_scores
+    q, k, lse = torch.zeros(2, H, T, D), torch.zeros(2, HKV, N, D), torch.zeros(2, H, T)
+    for bad in (k[:1], k[..., :32], k[0]):
+        with pytest.raises(ValueError, match="k must be"):
+            key_scores(q, bad, lse)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        key_scores(q, k, lse)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("name", list(WRONG) + ["lse device", "query device", "second batch", "gradients"])
 def test_refused_commits_change_nothing(cuda, name):
