@@ -9,6 +9,7 @@
 // K and V together (3.4 us there, 2.3 for 5 drafts of one sequence), one per 64 tensors for the
 // compaction (4.9 us for 32 layers, 3.6 for 28).
 #include "cab_internal.h"
+#include "row_layout.h"
 
 namespace cab {
 namespace {
@@ -108,13 +109,6 @@ __global__ __launch_bounds__(COMMIT_THREADS) void kv_commit_kernel(CommitArgs a)
     a.new_lengths[b] = static_cast<int32_t>(len + j);
 }
 
-// Rows a kernel writes must not share memory: each stride between them spans a row.
-bool rows_apart(const int64_t* st, const int64_t* size, int64_t row) {
-  for (int d = 0; d < 3; ++d)
-    if (size[d] > 1 && (st[d] < 0 ? -st[d] : st[d]) < row) return false;
-  return true;
-}
-
 }  // namespace
 }  // namespace cab
 
@@ -152,7 +146,7 @@ extern "C" cab_status_t cab_kv_append_at(const void* k, const void* v, void* k_d
   for (int t = 0; t < 2; ++t) {
     const uintptr_t at = reinterpret_cast<uintptr_t>(src[t]) | reinterpret_cast<uintptr_t>(dst[t]);
     CAB_REQUIRE(at % es == 0, CAB_ESHAPE, "%s: pointers not aligned to their elements", fn);
-    CAB_REQUIRE(rows_apart(ds[t], size, D), CAB_ESHAPE, "%s: rows of a buffer overlap", fn);
+    CAB_REQUIRE(RowLayout(ds[t], size, D).apart, CAB_ESHAPE, "%s: rows of a buffer overlap", fn);
     a.src[t] = static_cast<const char*>(src[t]);
     a.dst[t] = static_cast<char*>(dst[t]);
     wide = wide && ss[t][3] == 1 && at % 16 == 0;
@@ -208,7 +202,7 @@ extern "C" cab_status_t cab_kv_commit(void* const* tensors, int32_t n_tensors,
               "%s: the new lengths cannot be written over the old ones", fn);
   const int64_t es = element_bytes;
   const int64_t size[3] = {B, H, rows};
-  CAB_REQUIRE(rows_apart(strides, size, D), CAB_ESHAPE, "%s: rows of a tensor overlap", fn);
+  CAB_REQUIRE(RowLayout(strides, size, D).apart, CAB_ESHAPE, "%s: rows of a tensor overlap", fn);
   CommitArgs a;
   bool wide = D * es % 16 == 0;
   for (int d = 0; d < 3; ++d) {

@@ -25,6 +25,7 @@
 // tree of 64 over 65472 keys 84 + 12 us (816 TFLOP/s), over 8128 22.6 + 8.6 us, of which the
 // partials of 256 workgroups (17 MB out and in) are some 5.
 #include "attn_common.h"
+#include "row_layout.h"
 
 namespace cab {
 namespace {
@@ -953,9 +954,7 @@ extern "C" cab_status_t cab_tree_attn_fwd(
       CAB_REQUIRE(strides[t][d] * es % 16 == 0, CAB_ESHAPE, "%s: rows must be 16-byte aligned", fn);
   }
   const int64_t out_size[3] = {B, H, T};
-  for (int d = 0; d < 3; ++d)
-    CAB_REQUIRE(out_size[d] == 1 || (o_strides[d] < 0 ? -o_strides[d] : o_strides[d]) >= D,
-                CAB_ESHAPE, "%s: rows of out overlap", fn);
+  CAB_REQUIRE(RowLayout(o_strides, out_size, D).apart, CAB_ESHAPE, "%s: rows of out overlap", fn);
   // 64 rows of K and of V are addressed by 32-bit offsets.
   const int64_t lim = int64_t{1} << 25;
   CAB_REQUIRE(k_strides[2] >= 0 && k_strides[2] * es <= lim && v_strides[2] >= 0 &&
