@@ -46,7 +46,8 @@ def append_drafts(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cac
     dtype (bf16, fp16, fp32) with a contiguous last dim. lengths, counts (``None``: n
     rows of every sequence): int32 ``[B]`` on the device (int64 is converted). Rows that
     would lie behind the cache's N, and those of a sequence of negative length, are
-    not written. The new rows must not be views of the caches.
+    not written. The new rows must not be views of the caches, nor
+    the caches share memory.
     """
     new, shape = k.shape, k_cache.shape
     if len(new) != 4 or v.shape != new:

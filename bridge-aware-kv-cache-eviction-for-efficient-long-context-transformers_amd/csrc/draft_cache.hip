@@ -156,6 +156,13 @@ extern "C" cab_status_t cab_kv_append_at(const void* k, const void* v, void* k_d
       wide = wide && a.ss[t][d] % 16 == 0 && a.ds[t][d] % 16 == 0;
     }
   }
+  // (one tensor as K and V of one buffer is written twice alike)
+  bool one = k == v && k_dst == v_dst;
+  for (int d = 0; d < 4; ++d)
+    one = one && k_strides[d] == v_strides[d] && k_dst_strides[d] == v_dst_strides[d];
+  CAB_REQUIRE(one || !rows_share(k_dst, RowLayout(k_dst_strides, size, D), v_dst,
+                                 RowLayout(v_dst_strides, size, D), es),
+              CAB_EINVAL, "%s: the buffers of K and V share memory", fn);
   if (wide) a.ss[0][3] = a.ss[1][3] = 16;
   const int64_t units = wide ? D * es / 16 : D;
   a.lengths = lengths;

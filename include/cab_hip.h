@@ -439,7 +439,7 @@ cab_status_t cab_key_sums(const void* attention, cab_dtype_t dtype, int64_t B, i
  * dim 1): sequence b's row r < counts[b] (counts NULL: r < n) goes to row
  * lengths[b] + r. Rows that would lie outside the buffer, and all rows of a
  * sequence of negative length, go nowhere. Sources and buffers must not
- * overlap.
+ * overlap, nor the two buffers (one source into one buffer as both is taken).
  *
  * cab_kv_commit keeps the accepted ones of `nodes` drafted rows in each of
  * n_tensors buffers (distinct, of one shape and stride set, every layer's K

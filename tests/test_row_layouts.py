@@ -57,3 +57,82 @@ def test_rows_of_one_tensor(lib, st):
             assert lib.cab_kv_append_at(FAKE, FAKE, FAKE, FAKE + (1 << 20), 2, 2, 3, 4, D, 4, plain, plain,
                                         k, v, FAKE, None, None) == nat.CAB_ESHAPE
             assert b"overlap" in lib.cab_last_error()
+
+
+# Pairs of [2, 3, 4] rows of 64 values (strides, offset of the second in values): which of them
+# share memory. Alike layouts are told apart place by place, others by their spans.
+FUSED = (3 * 4 * 2 * D, 4 * 2 * D, 2 * D)
+WIDE = (3 * 4 * 5 * D, 4 * 5 * D, 5 * D)
+PLAIN = (3 * 4 * D, 4 * D, D)
+HEADS_INSIDE = (3 * 4 * D, D, 3 * D)
+PAIRS = [
+    (PLAIN, PLAIN, 0, True),
+    (PLAIN, PLAIN, D, True),                     # one row on
+    (PLAIN, PLAIN, -4 * D, True),
+    (PLAIN, PLAIN, 2 * 3 * 4 * D, False),        # one behind the other
+    (PLAIN, PLAIN, -2 * 3 * 4 * D, False),
+    (PLAIN, PLAIN, 2 * 3 * 4 * D - 8, True),
+    (FUSED, FUSED, D, False),                    # K and V side by side in each row
+    (FUSED, FUSED, -D, False),
+    (FUSED, FUSED, D - 8, True),
+    (FUSED, FUSED, 2 * D, True),                 # the next row's
+    (FUSED, FUSED, 3 * D, False),
+    (WIDE, WIDE, 4 * D, False),
+    (WIDE, WIDE, 4 * D + 8, True),               # reaches into the next row
+    (WIDE, WIDE, 3 * 4 * 5 * D - 4 * D, False),
+    (HEADS_INSIDE, HEADS_INSIDE, 2 * D, True),
+    (PLAIN, HEADS_INSIDE, 0, True),
+    (PLAIN, HEADS_INSIDE, 2 * 3 * 4 * D, False),
+    (FUSED, PLAIN, D, True),                     # (their spans meet)
+]
+
+
+SHARED = [p[:3] for p in PAIRS if p[3]]
+APART = [p[:3] for p in PAIRS if not p[3]]
+
+
+@pytest.mark.parametrize("ks,vs,offset", SHARED)
+@pytest.mark.parametrize("es", [2, 4])
+def test_append_refuses_buffers_that_share(lib, ks, vs, offset, es):
+    plain = s4(*PLAIN, 1)
+    assert lib.cab_kv_append_at(FAKE, FAKE + 4096, FAKE, FAKE + es * offset, es, 2, 3, 4, D, 4, plain, plain,
+                                s4(*ks, 1), s4(*vs, 1), FAKE, None, None) == nat.CAB_EINVAL
+    assert b"share memory" in lib.cab_last_error()
+
+
+def in_one_memory(cuda, dt, ks, vs, offset):
+    """Two caches of such a layout in one tensor."""
+    import torch
+    g = torch.Generator().manual_seed(1)
+    memory = torch.randn(20000, generator=g).to(dt).to(cuda)
+    base = 8000 - offset // 2 // 8 * 8
+    view = lambda m, st, at: m.as_strided((2, 3, 4, D), (*st, 1), at)
+    return memory, lambda m: (view(m, ks, base), view(m, vs, base + offset))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ks,vs,offset", APART)
+@pytest.mark.parametrize("dt", ["bfloat16", "float32"])
+def test_append_takes_buffers_that_are_apart(cuda, dt, ks, vs, offset):
+    import torch
+    from cab_attention.cache import append_drafts
+    dt = getattr(torch, dt)
+    memory, caches = in_one_memory(cuda, dt, ks, vs, offset)
+    k, v = torch.randn((2, 2, 3, 2, D), device=cuda).to(dt)
+    want = memory.clone()
+    for cache, new in zip(caches(want), (k, v)):
+        cache[0, :, 1:3], cache[1, :, 2:4] = new[0], new[1]
+    append_drafts(k, v, *caches(memory), torch.tensor([1, 2], dtype=torch.int32, device=cuda))
+    assert torch.equal(memory, want)
+
+
+@pytest.mark.gpu
+def test_append_of_one_tensor_as_both(cuda):
+    import torch
+    from cab_attention.cache import append_drafts
+    cache, k = torch.zeros((1, 2, 9, D), device=cuda), torch.randn((1, 2, 3, D), device=cuda)
+    n = torch.tensor([4], dtype=torch.int32, device=cuda)
+    append_drafts(k, k, cache, cache, n)
+    assert torch.equal(cache[:, :, 4:7], k) and not cache[:, :, 7:].any()
+    with pytest.raises(ValueError, match="share memory"):
+        append_drafts(k, k + 1, cache, cache, n)
