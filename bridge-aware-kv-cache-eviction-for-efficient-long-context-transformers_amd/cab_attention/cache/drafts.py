@@ -84,7 +84,7 @@ def commit_drafts(caches: Sequence[torch.Tensor], lengths: torch.Tensor, path: t
     moves to row ``lengths[b] + j`` for ``j < counts[b]``. Returns the new lengths,
     int32 ``[B]``: the old ones plus the rows kept. No other row changes.
 
-    caches: distinct ``[B, H, N, D]`` tensors of one shape, dtype (bf16, fp16, fp32)
+    caches: ``[B, H, N, D]`` tensors that share no memory, of one shape, dtype (bf16, fp16, fp32)
     and stride set, with a contiguous last dim. lengths, counts: int32 ``[B]``; path:
     int32 ``[B, T]``, on the device, as :func:`verify_drafts` gives them (int64 is
     converted). A path's first ``counts[b]`` entries ascend strictly; the first one

@@ -11,6 +11,8 @@
 #include "cab_internal.h"
 #include "row_layout.h"
 
+#include <algorithm>
+
 namespace cab {
 namespace {
 
@@ -109,6 +111,29 @@ __global__ __launch_bounds__(COMMIT_THREADS) void kv_commit_kernel(CommitArgs a)
     a.new_lengths[b] = static_cast<int32_t>(len + j);
 }
 
+constexpr int MOST_TENSORS = 4096;
+
+// 1: a tensor is there twice, 2: two of them share a row, 0: neither. By rising address
+// neighbours decide, unless tensors lie in one another's gaps: there all pairs that reach each
+// other do, or, where all lie within the smallest stride (layers side by side in each
+// row), neighbours' rows.
+int tensors_share(void* const* tensors, int n, const RowLayout& layout, int64_t es) {
+  const char* t[MOST_TENSORS];
+  for (int i = 0; i < n; ++i) t[i] = static_cast<const char*>(tensors[i]);
+  std::sort(t, t + n);
+  for (int i = 1; i < n; ++i)
+    if (t[i] == t[i - 1]) return 1;
+  if (layout.empty) return 0;
+  const int64_t step = layout.dims ? layout.st[layout.dims - 1] : INT64_MAX / es;
+  const bool side_by_side = t[n - 1] - t[0] <= (step - layout.row) * es;
+  for (int i = 0; i < n; ++i)
+    for (int j = i + 1; j < n && t[j] - t[i] < layout.extent * es; ++j) {
+      if (side_by_side ? t[j] - t[i] < layout.row * es : layout.meets((t[j] - t[i]) / es)) return 2;
+      if (side_by_side) break;
+    }
+  return 0;
+}
+
 }  // namespace
 }  // namespace cab
 
@@ -194,7 +219,7 @@ extern "C" cab_status_t cab_kv_commit(void* const* tensors, int32_t n_tensors,
   clear_error();
   CAB_REQUIRE(element_bytes == 2 || element_bytes == 4, CAB_EDTYPE,
               "%s: element size %d unsupported (2 or 4)", fn, (int)element_bytes);
-  CAB_REQUIRE(n_tensors >= 1 && n_tensors <= 4096 && B >= 0 && H >= 1 && rows >= 0 && D >= 1 &&
+  CAB_REQUIRE(n_tensors >= 1 && n_tensors <= MOST_TENSORS && B >= 0 && H >= 1 && rows >= 0 && D >= 1 &&
                   nodes >= 0,
               CAB_ESHAPE, "%s: bad shape", fn);
   CAB_REQUIRE(length0 >= 0 && count0 >= 0, CAB_EINVAL, "%s: negative length or count", fn);
@@ -209,7 +234,8 @@ extern "C" cab_status_t cab_kv_commit(void* const* tensors, int32_t n_tensors,
               "%s: the new lengths cannot be written over the old ones", fn);
   const int64_t es = element_bytes;
   const int64_t size[3] = {B, H, rows};
-  CAB_REQUIRE(RowLayout(strides, size, D).apart, CAB_ESHAPE, "%s: rows of a tensor overlap", fn);
+  const RowLayout layout(strides, size, D);
+  CAB_REQUIRE(layout.apart, CAB_ESHAPE, "%s: rows of a tensor overlap", fn);
   CommitArgs a;
   bool wide = D * es % 16 == 0;
   for (int d = 0; d < 3; ++d) {
@@ -221,9 +247,12 @@ extern "C" cab_status_t cab_kv_commit(void* const* tensors, int32_t n_tensors,
     CAB_REQUIRE(at != 0, CAB_EINVAL, "%s: null tensor", fn);
     CAB_REQUIRE(at % es == 0, CAB_ESHAPE, "%s: pointers not aligned to their elements", fn);
     wide = wide && at % 16 == 0;
-    // (moved twice, a tensor's rows would be moved from where they went)
-    for (int x = 0; x < t; ++x)
-      CAB_REQUIRE(tensors[x] != tensors[t], CAB_EINVAL, "%s: a tensor is listed twice", fn);
+  }
+  // (moved twice, a row would be moved from where it went)
+  switch (tensors_share(tensors, n_tensors, layout, es)) {
+    case 0: break;
+    case 1: CAB_REQUIRE(false, CAB_EINVAL, "%s: a tensor is listed twice", fn);
+    default: CAB_REQUIRE(false, CAB_EINVAL, "%s: two tensors share memory", fn);
   }
   const int64_t units = wide ? D * es / 16 : D;
   a.lengths = lengths;

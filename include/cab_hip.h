@@ -442,8 +442,8 @@ cab_status_t cab_key_sums(const void* attention, cab_dtype_t dtype, int64_t B, i
  * overlap, nor the two buffers (one source into one buffer as both is taken).
  *
  * cab_kv_commit keeps the accepted ones of `nodes` drafted rows in each of
- * n_tensors buffers (distinct, of one shape and stride set, every layer's K
- * and V; `tensors` is a host array): with len = lengths[b] (lengths NULL:
+ * n_tensors buffers (sharing no memory, of one shape and stride set, every layer's
+ * K and V; `tensors` is a host array): with len = lengths[b] (lengths NULL:
  * length0), row len + path[b][j] moves to row len + j for j < counts[b]
  * (counts NULL: count0), and new_lengths[b] (may be NULL) = len + rows kept.
  * Other rows stay as they are. Entries of a path ascend strictly; the first

@@ -136,3 +136,54 @@ def test_append_of_one_tensor_as_both(cuda):
     assert torch.equal(cache[:, :, 4:7], k) and not cache[:, :, 7:].any()
     with pytest.raises(ValueError, match="share memory"):
         append_drafts(k, k + 1, cache, cache, n)
+
+
+def commit_status(lib, st, addresses, es=2):
+    ptrs = (ctypes.c_void_p * len(addresses))(*addresses)
+    return lib.cab_kv_commit(ptrs, len(addresses), es, 2, 3, 4, D, s4(*st, 1), FAKE, 0, FAKE, 5, 5, FAKE, 0,
+                             FAKE + 64, None)
+
+
+@pytest.mark.parametrize("st,offset", [(a, o) for a, b, o in SHARED if a == b and o])
+@pytest.mark.parametrize("es", [2, 4])
+def test_commit_refuses_tensors_that_share(lib, st, offset, es):
+    far = [FAKE + es * 100000 * (i + 1) for i in range(5)]
+    for at in ([FAKE, FAKE + es * offset], far + [far[2] + es * offset], [far[3] - es * offset] + far):
+        assert commit_status(lib, st, at, es) == nat.CAB_EINVAL
+        assert b"share memory" in lib.cab_last_error()
+    assert commit_status(lib, st, far + [far[0]], es) == nat.CAB_EINVAL
+    assert b"twice" in lib.cab_last_error()
+    # Side by side in each row, but for one that is not.
+    if st == WIDE:
+        row = [FAKE + es * D * i for i in (3, 0, 4, 1)]
+        assert commit_status(lib, st, row + [FAKE + es * (2 * D + 8)], es) == nat.CAB_EINVAL
+        assert b"share memory" in lib.cab_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("st,offset", [(a, o) for a, b, o in APART if a == b])
+@pytest.mark.parametrize("dt", ["bfloat16", "float32"])
+def test_commit_takes_tensors_that_are_apart(cuda, dt, st, offset):
+    import torch
+    from cab_attention.cache import commit_drafts
+    memory, caches = in_one_memory(cuda, getattr(torch, dt), st, st, offset)
+    want = memory.clone()
+    for c in caches(want):
+        c[0, :, 1:3], c[1, :, 0] = c[0][:, [2, 3]].clone(), c[1][:, 1].clone()
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)
+    path = i32([[1, 2, -1], [1, -1, -1]])
+    assert commit_drafts(caches(memory), i32([1, 0]), path, i32([2, 1])).tolist() == [3, 1]
+    assert torch.equal(memory, want)
+
+
+@pytest.mark.gpu
+def test_commit_of_layers_side_by_side(cuda):
+    """70 layers' rows in one tensor [B, H, N, layer, D]: two launches."""
+    import torch
+    from cab_attention.cache import commit_drafts
+    memory = torch.randn((2, 1, 9, 70, D), device=cuda)
+    want = memory.clone()
+    want[0, :, 5], want[1, :, 2] = memory[0, :, 7], memory[1, :, 3]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)
+    new = commit_drafts(memory.unbind(3), i32([4, 2]), i32([[0, 3, -1, -1], [1, -1, -1, -1]]), i32([2, 1]))
+    assert new.tolist() == [6, 3] and torch.equal(memory, want)
