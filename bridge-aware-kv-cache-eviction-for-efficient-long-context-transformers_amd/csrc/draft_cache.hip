@@ -167,11 +167,12 @@ extern "C" cab_status_t cab_kv_append_at(const void* k, const void* v, void* k_d
   const int64_t* ss[2] = {k_strides, v_strides};
   const int64_t* ds[2] = {k_dst_strides, v_dst_strides};
   const int64_t size[3] = {B, H, rows};
+  const RowLayout layout[2] = {RowLayout(k_dst_strides, size, D), RowLayout(v_dst_strides, size, D)};
   bool wide = D * es % 16 == 0;
   for (int t = 0; t < 2; ++t) {
     const uintptr_t at = reinterpret_cast<uintptr_t>(src[t]) | reinterpret_cast<uintptr_t>(dst[t]);
     CAB_REQUIRE(at % es == 0, CAB_ESHAPE, "%s: pointers not aligned to their elements", fn);
-    CAB_REQUIRE(RowLayout(ds[t], size, D).apart, CAB_ESHAPE, "%s: rows of a buffer overlap", fn);
+    CAB_REQUIRE(layout[t].apart, CAB_ESHAPE, "%s: rows of a buffer overlap", fn);
     a.src[t] = static_cast<const char*>(src[t]);
     a.dst[t] = static_cast<char*>(dst[t]);
     wide = wide && ss[t][3] == 1 && at % 16 == 0;
@@ -185,9 +186,8 @@ extern "C" cab_status_t cab_kv_append_at(const void* k, const void* v, void* k_d
   bool one = k == v && k_dst == v_dst;
   for (int d = 0; d < 4; ++d)
     one = one && k_strides[d] == v_strides[d] && k_dst_strides[d] == v_dst_strides[d];
-  CAB_REQUIRE(one || !rows_share(k_dst, RowLayout(k_dst_strides, size, D), v_dst,
-                                 RowLayout(v_dst_strides, size, D), es),
-              CAB_EINVAL, "%s: the buffers of K and V share memory", fn);
+  CAB_REQUIRE(one || !rows_share(k_dst, layout[0], v_dst, layout[1], es), CAB_EINVAL,
+              "%s: the buffers of K and V share memory", fn);
   if (wide) a.ss[0][3] = a.ss[1][3] = 16;
   const int64_t units = wide ? D * es / 16 : D;
   a.lengths = lengths;
