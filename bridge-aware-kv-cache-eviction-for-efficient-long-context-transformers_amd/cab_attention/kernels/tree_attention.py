@@ -30,6 +30,7 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, parents: t
         lengths: int32 ``[B]`` on the device, in ``[0, N - T]`` (others count as the
             nearest one inside). ``None``: the drafts are the last T rows.
         scale: defaults to ``1/sqrt(D)``.
+        out: where the output goes, like q; q itself, or memory of none of the inputs.
 
     What a node does not see cannot reach its output, not even as a NaN or an infinity.
     A node that is there and whose scores have no softmax (a NaN or +inf among them, or

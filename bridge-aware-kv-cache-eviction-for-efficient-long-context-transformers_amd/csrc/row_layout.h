@@ -7,7 +7,7 @@
 namespace cab {
 
 // Rows of `row` elements at three strides: the dims of more than one place, by falling stride.
-// `apart`: each stride spans what the smaller ones cover, so that no two rows share an element.
+// `extent`: elements from the first to behind the last. `apart`: each stride spans what the smaller ones cover, so that no two rows share an element.
 // (Sufficient; of layouts that torch's views make, only overlapping ones fail it.)
 struct RowLayout {
   int64_t st[3], size[3], row, low = 0, extent;  // elements; low: of the first one, from the pointer
@@ -27,13 +27,15 @@ struct RowLayout {
       st[at] = s;
       size[at] = sizes[d];
     }
+    // (past 2^60 elements nothing is addressed: counts as not apart)
+    constexpr int64_t FAR = int64_t{1} << 60;
     extent = row;
     for (int d = dims - 1; d >= 0; --d) {
-      // (past 2^60 elements nothing is addressed: counts as not apart)
-      apart = apart && st[d] >= extent && st[d] <= ((int64_t{1} << 60) - extent) / (size[d] - 1);
-      if (apart) extent += (size[d] - 1) * st[d];
+      const bool far = extent >= FAR || st[d] > (FAR - extent) / (size[d] - 1);
+      apart = apart && !far && st[d] >= extent;
+      extent = far ? FAR : extent + (size[d] - 1) * st[d];
     }
-    for (int d = 0; d < 3 && apart; ++d)
+    for (int d = 0; d < 3 && extent < FAR; ++d)
       if (sizes[d] > 1 && strides[d] < 0) low += (sizes[d] - 1) * strides[d];
   }
 
@@ -45,7 +47,7 @@ struct RowLayout {
 
   // Whether rows of a tensor laid out so and of one `diff` elements further on share an element:
   // diff is then a sum of places times strides, less than a row off. As strides span what is
-  // below them, only the two nearest numbers of places come into question at each.
+  // below them (the rows are apart), only the two nearest numbers of places can be it.
   bool meets(int64_t diff, int d = 0) const {
     if (d == dims) return diff < row && -diff < row;
     const int64_t k = diff / st[d] - (diff % st[d] < 0);
@@ -55,14 +57,14 @@ struct RowLayout {
   }
 };
 
-// Whether two tensors of rows that are apart (a known layout each, elements of es bytes) may
-// share memory: exact for layouts that are alike, else whether their spans meet.
+// Whether two tensors (a layout each, elements of es bytes) may share memory: exact for rows
+// that are apart and laid out alike, else whether their spans meet.
 inline bool rows_share(const void* a, const RowLayout& x, const void* b, const RowLayout& y, int64_t es) {
   if (x.empty || y.empty) return false;
   const int64_t from_a = static_cast<int64_t>(reinterpret_cast<uintptr_t>(a)) + x.low * es;
   const int64_t from_b = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b)) + y.low * es;
   if (from_a + x.extent * es <= from_b || from_b + y.extent * es <= from_a) return false;
-  return !x.same_as(y) || x.meets((from_b - from_a) / es);
+  return !x.apart || !x.same_as(y) || x.meets((from_b - from_a) / es);
 }
 
 }  // namespace cab

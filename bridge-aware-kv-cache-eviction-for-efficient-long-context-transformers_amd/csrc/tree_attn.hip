@@ -954,7 +954,8 @@ extern "C" cab_status_t cab_tree_attn_fwd(
       CAB_REQUIRE(strides[t][d] * es % 16 == 0, CAB_ESHAPE, "%s: rows must be 16-byte aligned", fn);
   }
   const int64_t out_size[3] = {B, H, T};
-  CAB_REQUIRE(RowLayout(o_strides, out_size, D).apart, CAB_ESHAPE, "%s: rows of out overlap", fn);
+  const RowLayout rows(o_strides, out_size, D);
+  CAB_REQUIRE(rows.apart, CAB_ESHAPE, "%s: rows of out overlap", fn);
   // 64 rows of K and of V are addressed by 32-bit offsets.
   const int64_t lim = int64_t{1} << 25;
   CAB_REQUIRE(k_strides[2] >= 0 && k_strides[2] * es <= lim && v_strides[2] >= 0 &&
@@ -963,6 +964,15 @@ extern "C" cab_status_t cab_tree_attn_fwd(
   const TreePlan pl = tree_plan(dtype, B, H, H_kv, T, N, D);
   CAB_REQUIRE(workspace && workspace_bytes >= pl.bytes && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
               CAB_EWORKSPACE, "%s: workspace needs %zu bytes, 16-byte aligned", fn, pl.bytes);
+  // join_kernel reads q's rows and the drafts' of k and v while it writes: q's own rows alone may
+  // be written over.
+  const int64_t kv_size[3] = {B, H_kv, N};
+  bool over_q = out == q;
+  for (int d = 0; d < 3; ++d) over_q = over_q && (out_size[d] == 1 || q_strides[d] == o_strides[d]);
+  CAB_REQUIRE((over_q || !rows_share(out, rows, q, RowLayout(q_strides, out_size, D), es)) &&
+                  !rows_share(out, rows, k, RowLayout(k_strides, kv_size, D), es) &&
+                  !rows_share(out, rows, v, RowLayout(v_strides, kv_size, D), es),
+              CAB_EINVAL, "%s: out shares memory with an input (only q itself may be out)", fn);
   JoinArgs j;
   TreeArgs& a = j.t;
   a.q = static_cast<const char*>(q);

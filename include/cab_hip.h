@@ -476,7 +476,8 @@ cab_status_t cab_kv_commit(void* const* tensors, int32_t n_tensors, int32_t elem
  * scaled scores (-inf for no node), lse may be NULL. Keys a node does not see do
  * not reach it whatever they hold. A node that is there and whose scores have no softmax
  * (a NaN or +inf among them, or all -inf) has NaN for both.
- * q, out: [B,H,T,D]; k, v: [B,H_kv,N,D] (strides); H % H_kv == 0; D == 64 or 128;
+ * q, out: [B,H,T,D]; k, v: [B,H_kv,N,D] (strides); out is q itself or shares no
+ * memory with the inputs; H % H_kv == 0; D == 64 or 128;
  * T <= 256; bf16, fp16 (products of 16-bit operands, P rounded to 16 bits, sums in
  * fp32) or fp32 (fp32 throughout). Token strides of k and v in [0, 2^25] bytes.
  * parents: int32, parents_stride 0 (one tree for all) or entries from one sequence's

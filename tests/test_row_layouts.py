@@ -187,3 +187,50 @@ def test_commit_of_layers_side_by_side(cuda):
     i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)
     new = commit_drafts(memory.unbind(3), i32([4, 2]), i32([[0, 3, -1, -1], [1, -1, -1, -1]]), i32([2, 1]))
     assert new.tolist() == [6, 3] and torch.equal(memory, want)
+
+
+def tree_status(lib, q, k, v, out, q_st, kv_st, out_st, T=4):
+    """tree_attention of [2, 3, T, D] queries over [2, 3, 40, D] caches, everything else right (a call
+    that is not refused would be launched: only for refusals)."""
+    return lib.cab_tree_attn_fwd(q, k, v, nat.CAB_F32, 2, 3, 3, T, 40, D, s4(*q_st, 1), s4(*kv_st, 1),
+                                 s4(*kv_st, 1), s4(*out_st, 1), FAKE, 0, None, 0, 0.1, out, None, FAKE,
+                                 1 << 40, None)
+
+
+def test_tree_attention_refuses_an_out_among_its_inputs(lib):
+    cache, size = (3 * 40 * D, 40 * D, D), 2 * 3 * 40 * D * 4
+    q, k, v, far = FAKE, FAKE + (1 << 24), FAKE + (1 << 25), FAKE + (1 << 26)
+    heads = (4 * 3 * D, D, 3 * D)
+    expanded = (0, 40 * D, D)
+    for out, q_st, kv_st, out_st in (
+            (q, PLAIN, cache, heads),              # q's memory in another order
+            (q + 4 * D, PLAIN, cache, PLAIN),      # a row on
+            (k, PLAIN, cache, PLAIN), (v, PLAIN, cache, PLAIN),
+            (k + size - 256, PLAIN, cache, PLAIN), # its last row
+            (k + size // 2 - 256, PLAIN, expanded, PLAIN),
+            (far - 4 * D, (0, 0, 0), cache, PLAIN)):
+        at = far if q_st == (0, 0, 0) else q
+        assert tree_status(lib, at, k, v, out, q_st, kv_st, out_st) == nat.CAB_EINVAL
+        assert b"out shares memory" in lib.cab_last_error()
+
+
+@pytest.mark.gpu
+def test_tree_attention_writes_over_q(cuda):
+    """out may be q itself, and lie beside q and between the caches' rows."""
+    import torch
+    from cab_attention.kernels import tree_attention
+    for dt, H, T in ((torch.float32, 2, 5), (torch.bfloat16, 4, 30), (torch.float16, 4, 64)):
+        fused = torch.randn((2, T, 3 * H, D), device=cuda).to(dt)
+        q, beside = fused[:, :, :H].transpose(1, 2), fused[:, :, H:2 * H].transpose(1, 2)
+        k, v = (torch.randn((2, 2, 400, D), device=cuda).to(dt) for _ in range(2))
+        up = torch.tensor([-1] + [i // 2 for i in range(T - 1)], dtype=torch.int32, device=cuda)
+        want = tree_attention(q, k, v, up)
+        rest = fused[:, :, 2 * H:].clone()
+        assert torch.equal(tree_attention(q, k, v, up, out=beside), want) and torch.equal(beside, want)
+        assert torch.equal(tree_attention(q, k, v, up, out=q), want) and torch.equal(q, want)
+        assert torch.equal(fused[:, :, 2 * H:], rest)
+        with pytest.raises(ValueError, match="shares memory"):
+            tree_attention(q, k, v, up, out=fused[:, :, 1:H + 1].transpose(1, 2))
+        if H == 2:
+            with pytest.raises(ValueError, match="shares memory"):
+                tree_attention(q, k, v, up, out=k[:, :, 100:100 + T])
