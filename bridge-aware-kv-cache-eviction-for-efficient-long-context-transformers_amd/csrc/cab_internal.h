@@ -187,10 +187,10 @@ __device__ __forceinline__ void bdma16_untracked(const sgpr_rsrc_t& r, uint32_t 
       __builtin_amdgcn_readfirstlane(static_cast<int>(reinterpret_cast<uintptr_t>(l))));
   // M0 (the LDS base of the load) and the scalars are inputs the compiler sets, whose wait
   // states it does not count for an asm block: one after an M0 write, five after a vector
-  // instruction (make_sgpr_rsrc's readfirstlane) wrote a scalar the load reads. Four here and
-  // the M0 write before them are five. (Three more than the M0 write alone needs: the
-  // block-sparse executor 3.40 -> 3.42 ms.)
-  asm volatile("s_nop 3\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
+  // instruction wrote a scalar the load reads (make_sgpr_rsrc's readfirstlane, a spilled scalar's
+  // readlane; without them rows of tree attention were wrong). All five are in the block, whatever
+  // precedes it. (The block-sparse executor: 3.39 ms with four and an M0 write, 3.41 with five.)
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
                :
                : "v"(voff), "s"(r), "s"(soff), "{m0}"(lds)
                : "memory");

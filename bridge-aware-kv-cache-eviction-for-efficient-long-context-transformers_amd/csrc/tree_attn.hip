@@ -440,18 +440,7 @@ __device__ __forceinline__ uint32_t tile_offset(uint32_t row, uint32_t chunk) {
 
 // Grid: 1-D over (row tile fastest, workgroup), neighbours on one XCD, so that a
 // stretch's row tiles find its K and V in one L2.
-// bdma16_untracked for operands that may come out of a vector lane (a spilled scalar, a
-// readfirstlane): a load reads such a scalar rightly five wait states after it was
-// written, which the compiler does not count inside an asm block.
-__device__ __forceinline__ void dma16(const sgpr_rsrc_t& r, uint32_t voff, uint32_t soff, const void* l) {
-  const uint32_t lds = static_cast<uint32_t>(
-      __builtin_amdgcn_readfirstlane(static_cast<int>(reinterpret_cast<uintptr_t>(l))));
-  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
-               :
-               : "v"(voff), "s"(r), "s"(soff), "{m0}"(lds)
-               : "memory");
-}
-
+//
 // Tiles go to LDS without passing through registers, the next one in flight while one is
 // computed (2 and 3 in flight measured 2 to 4 % slower). A wave waits for its own
 // loads of a tile, and the workgroup's barrier makes that everybody's; the same
@@ -498,12 +487,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void tile_kernel(TreeArgs a) {
         char* kt = &lds[slot][0][(n * WAVES + w) * 1024];
         char* vt = &lds[slot][1][(n * WAVES + w) * 1024];
         if (left >= TILE) {
-          dma16(kr, koff, ks, kt);
-          dma16(vr, voff, vs, vt);
+          bdma16_untracked(kr, koff, ks, kt);
+          bdma16_untracked(vr, voff, vs, vt);
         } else {
           const bool in = static_cast<int>(lrow) + n * ROWS < left;
-          dma16(kr, in ? koff + ks : END, 0, kt);
-          dma16(vr, in ? voff + vs : END, 0, vt);
+          bdma16_untracked(kr, in ? koff + ks : END, 0, kt);
+          bdma16_untracked(vr, in ? voff + vs : END, 0, vt);
         }
       }
     };
