@@ -380,6 +380,11 @@ __device__ __forceinline__ unsigned long long merge_argmax(const RowStats* st, i
   return key;
 }
 
+// Sums and weights are off by 1e-7 of the row's, so what is left after rejections, by
+// subtraction, by up to that over its share: below this share it is summed anew (a pass over
+// the row, which one node in 16 needs at most).
+constexpr double LEAST_LEFT = 1.0 / 16;
+
 // STATS: rows' statistics are there. Where the walk ended is left for pick_kernel.
 template <cab_dtype_t DT, int MODE, bool STATS>
 __global__ __launch_bounds__(WALK_THREADS) void walk_kernel(VerifyArgs a) {
@@ -479,6 +484,8 @@ __global__ __launch_bounds__(WALK_THREADS) void walk_kernel(VerifyArgs a) {
     } else if constexpr (MODE == POINT) {
       if (first >= 0) softmax_of(0, node, lrow, m, s);
       left = s;
+      double base = s;     // what the row's last pass gave
+      int rejected = 0;    // tokens in gone
       for (int i = first; i >= 0 && taken < 0; i = next_child(node, i)) {
         const int x = token[i];
         if (x < 0) continue;
@@ -488,11 +495,26 @@ __global__ __launch_bounds__(WALK_THREADS) void walk_kernel(VerifyArgs a) {
           before = before || ballot64(j < i && parent[j] == node && token[j] == x) != 0;
         }
         if (before) continue;
+        if (left < base * LEAST_LEFT) {
+          __syncthreads();  // (gone is there)
+          double c = 0.0;
+          over_row<DT, 4, THREADS>(lrow, a.V, [&](int at, const float* v, auto n) {
+            const uint32_t out_of = gone_mask<decltype(n)::value>(gone, rejected, at);
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < decltype(n)::value; ++k) sum += out_of >> k & 1 ? 0.f : weight(v[k], m, a);
+            c += sum;
+          });
+          base = left = block_sum<THREADS>(c, sh);
+        }
         const float e = weight(value[i], m, a);
-        if (static_cast<double>(uniform[i]) * left < static_cast<double>(e))
+        if (static_cast<double>(uniform[i]) * left < static_cast<double>(e)) {
           taken = i;
-        else
+        } else {
           left = fmax(left - static_cast<double>(e), 0.0);
+          if (tid == 0) gone[rejected] = x;
+          ++rejected;
+        }
       }
     } else {
       qrow = drafts + node * a.ds[1];
