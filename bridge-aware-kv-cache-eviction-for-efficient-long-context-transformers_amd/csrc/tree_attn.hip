@@ -870,7 +870,8 @@ bool tree_sizes(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t N, int64_t
   return B >= 1 && Hkv >= 1 && H >= Hkv && H % Hkv == 0 && T >= 1 && T <= MAX_NODES && N >= T &&
          N <= INT32_MAX - 1024 && (D == 64 || D == 128) && H <= 65535 && B <= 65535 &&
          B * Hkv <= INT32_MAX / 2 / ceil_div(N, TILE) && H / Hkv * T <= 65535 &&
-         H * T <= (int64_t{1} << 26) / B;  // (join_kernel's threads: 64 a row)
+         // (join_kernel's threads, 64 a row in workgroups of four: fewer than 2^32)
+         H * T <= ((int64_t{1} << 26) - 4) / B;
 }
 
 template <cab_dtype_t DT, int HD>

@@ -234,3 +234,17 @@ def test_tree_attention_writes_over_q(cuda):
         if H == 2:
             with pytest.raises(ValueError, match="shares memory"):
                 tree_attention(q, k, v, up, out=k[:, :, 100:100 + T])
+
+
+def test_tree_attention_of_the_most_rows(lib):
+    """B H T = 2^26 rows need one thread more than a launch takes, and the three numbers below it
+    as many."""
+    ws = lib.cab_tree_attn_workspace_bytes
+    st = s4(64, 64, 64, 1)
+    for B, H, T in ((1 << 13, 1 << 7, 1 << 6), (1 << 10, 1 << 8, 1 << 8), (8191, 8193, 1), (18631, 3602, 1)):
+        assert B * H * T in (1 << 26, (1 << 26) - 1, (1 << 26) - 2)
+        assert ws(nat.CAB_BF16, B, H, H, T, T, D) == 0
+        assert lib.cab_tree_attn_fwd(FAKE, FAKE, FAKE, nat.CAB_BF16, B, H, H, T, T, D, st, st, st, st, FAKE, 0,
+                                     None, 0, 0.1, FAKE, None, FAKE, 1 << 40, None) == nat.CAB_ESHAPE
+        assert b"too large" in lib.cab_last_error()
+    assert 16380 * 4097 == (1 << 26) - 4 and ws(nat.CAB_BF16, 16380, 4097, 4097, 1, 1, D) > 0
