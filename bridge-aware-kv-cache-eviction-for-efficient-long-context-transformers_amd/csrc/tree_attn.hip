@@ -6,8 +6,8 @@
 //  1. The context has no mask: every row of a unit sees all of it. The contexts of all
 //     units, cut into pieces of as many keys as a workgroup takes at a time, make one
 //     list, and each workgroup takes an equal stretch of it, whatever the lengths. Of
-//     each unit that its stretch touches it leaves one partial (maximum m, row sum l,
-//     unnormalised O) per row:
+//     each unit that its stretch touches it leaves one partial (the maximum's level m,
+//     row sum l, unnormalised O) per row:
 //     - rows_kernel (few rows, and fp32, on the fp32 matrix instructions): every wave walks
 //       its own 32-key steps, K and V straight from memory into matrix operands;
 //     - tile_kernel (more rows, 16 bits): 64-key tiles of K and V in LDS, read by all
@@ -15,8 +15,15 @@
 //     Both compute S^T = K Q^T, an online softmax in the log2 domain (maxima, sums and O
 //     in fp32, P rounded to 16 bits as the operand of O^T += V^T P^T).
 //  2. join_kernel, one wave per row, merges the row's partials and adds the drafts it
-//     sees, found by walking its ancestors: a node has few of them, and no other
-//     draft's K or V is touched, so nothing a row does not see can reach it.
+//     sees, found by walking its ancestors: no other draft's K or V is touched, so nothing
+//     a row does not see can reach it. A tree's node has few of them; in a chain of T
+//     nodes a row has up to T, and the rows' work together grows with T^2.
+//
+// P goes to 16 bits because the matrix instructions take it so (fp32 ones run at a seventh of
+// the rate): half a step of each weight, which with the output's own rounding is an error of
+// 1.9e-3 to 2.1e-3 of the outputs in bf16 where that rounding alone is 1.65e-3 (fp16 2.5e-4,
+// 2.1e-4). Nothing in a result depends on the order in which workgroups run: the same bits
+// again for the same sizes and lengths.
 //
 // Bound: HBM (the context's K and V, read once) for few rows; for many the chain of one
 // tile (operand reads, products, maxima, exponentials, products), of which two waves a
@@ -174,7 +181,7 @@ __device__ __forceinline__ float relevel(float m, float level, float m1, float l
   return __builtin_amdgcn_exp2f(DT == CAB_F16 ? level - level1 : (m - m1) * c);
 }
 
-// K and V are read once: non-temporal loads.
+// Non-temporal loads: K and V are read once, but in fp32 by every 32 rows of a unit.
 template <typename T>
 __device__ __forceinline__ T ld_stream(const char* p) {
   return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
@@ -370,7 +377,9 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void rows_kernel(TreeAr
 
     const int end = min((len + STEP - 1) / STEP, 4 * (piece + pieces));
     int step = 4 * piece + w;
-    if constexpr (F32 || QT * HD > 128) {  // (two register sets would spill)
+    // (Two register sets spill with 32 rows of 128 in 16 bits. In fp32, one workgroup a CU,
+    // they would not; one set is what the figures here are of.)
+    if constexpr (F32 || QT * HD > 128) {
       SR x;
       for (; step < end; step += 4) {
         load(step, x);

@@ -5,7 +5,8 @@
 // number:
 //   greedy (temperature 0): the child whose token is the row's argmax;
 //   point (no draft logits): a child x is accepted if r Z < p(x), where Z is what the
-//     siblings rejected before it have left of p (their tokens' weights become 0);
+//     siblings rejected before it have left of p (their tokens' weights become 0): the row's
+//     sum less theirs, or, where that is little of it, the sum of the others;
 //   draft, with q = softmax(draft_logits[node] / temperature): each rejection leaves
 //     max(p - q, 0) / c of p. As max(max(y, 0) - z, 0) = max(y - z, 0) for z >= 0, the
 //     residual after any number of rejections is max(p - a q, 0) / c with two numbers:
@@ -729,8 +730,9 @@ VerifyPlan verify_plan(cab_dtype_t dtype, int mode, int64_t B, int64_t T, int64_
   const int64_t es = static_cast<int64_t>(dtype_size(dtype)), rows = B * T, sides = mode == DRAFT ? 2 : 1;
   // (stats_kernel's threads: 256 a slice, within 32 bits)
   p.stats = rows * sides <= STATS_BYTES / (V * es) && rows <= (int64_t{1} << 23);
-  // At most 64 slices a row (one wave merges them), and no more than fill the chip: a
-  // slice is at least `loads` 16-byte loads a thread. (32 trees of 32 rows: 2048 workgroups
+  // Slices of up to `loads` 16-byte loads a thread (rows just past a whole number of them are
+  // cut evenly: half as many in the worst case), longer ones where that were more than 64 a
+  // row (one wave merges them) or more than fill the chip. (32 trees of 32 rows: 2048 workgroups
   // of statistics 68 us the call, 4096 60, 16384 62; 512 that pick 60, 1024 58, 2048 59.)
   auto cut = [&](int64_t loads, int64_t units, int64_t fill, int64_t& n, int64_t& size) {
     n = ceil_div(V, SLICE_THREADS * loads * 16 / es);
