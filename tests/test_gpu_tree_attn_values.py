@@ -144,3 +144,30 @@ def test_large_fp16_scores(cuda, H, T, big):
                               torch.tensor([1000], dtype=torch.int32).to(cuda), return_lse=True)
     np.testing.assert_allclose(np64(out), want[0], atol=ATOL["fp16"], rtol=0)
     np.testing.assert_allclose(np64(lse), want[1], rtol=5 * 2 ** -24, atol=1e-5)
+
+
+@pytest.mark.parametrize("H,T", ROWS)
+@pytest.mark.parametrize("late", [True, False])
+def test_fp16_scores_across_the_levels_border(cuda, H, T, late):
+    """Scores of 2^24 / log2(e) less and more a few, the larger ones in the later keys or the
+    earlier: sums taken on one side of the border are carried over to the other. (Each score is
+    a whole number that fp32 sums exactly: 11629072 + 8 i + j.)"""
+    N, D = 1300 + T, 64
+    g = torch.Generator().manual_seed(T)
+    q, k = torch.zeros((1, H, T, D)), torch.zeros((1, 1, N, D))
+    q[..., :3] = torch.tensor([9640.0, 2.0, 8.0])
+    k[..., 0] = 9640
+    low = torch.tensor([51488.0, 5.0]) + torch.stack([torch.zeros(N), torch.randint(0, 3, (N,), generator=g)], 1)
+    high = torch.tensor([51520.0, 0.0]) + torch.stack([torch.zeros(N), torch.randint(0, 2, (N,), generator=g)], 1)
+    first = (torch.arange(N) < 650)[:, None]
+    k[0, 0, :, 1:3] = torch.where(first == late, low, high)
+    k[:, :, 1300:, 1] = 0  # (the drafts weigh nothing)
+    v = rand((1, 1, N, D), "fp16", 3)
+    q, k = q.half(), k.half()
+    s = np64(k)[0, 0, :1300] @ np64(q)[0, 0, 0] / 8
+    assert np.unique(s).tolist() == [11629077, 11629078, 11629079, 11629080, 11629081]
+    parents = trees(1, T, "tree", T)
+    want = S.tree_attention(np64(q), np64(k), np64(v), parents, [1300])
+    out, lse = run(cuda, q, k, v, parents, [1300])
+    np.testing.assert_allclose(out, want[0], atol=ATOL["fp16"], rtol=0)
+    np.testing.assert_allclose(lse, want[1], rtol=5 * 2 ** -24, atol=1e-5)
