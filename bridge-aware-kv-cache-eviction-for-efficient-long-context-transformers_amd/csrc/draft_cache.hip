@@ -115,8 +115,8 @@ constexpr int MOST_TENSORS = 4096;
 
 // 1: a tensor is there twice, 2: two of them share a row, 0: neither. By rising address
 // neighbours decide, unless tensors lie in one another's gaps: there all pairs that reach each
-// other do, or, where all lie within the smallest stride (layers side by side in each
-// row), neighbours' rows.
+// other do, or, where all lie within the smallest stride and the others are multiples of it
+// (layers side by side in each row), neighbours' rows.
 int tensors_share(void* const* tensors, int n, const RowLayout& layout, int64_t es) {
   const char* t[MOST_TENSORS];
   for (int i = 0; i < n; ++i) t[i] = static_cast<const char*>(tensors[i]);
@@ -125,7 +125,8 @@ int tensors_share(void* const* tensors, int n, const RowLayout& layout, int64_t 
     if (t[i] == t[i - 1]) return 1;
   if (layout.empty) return 0;
   const int64_t step = layout.dims ? layout.st[layout.dims - 1] : INT64_MAX / es;
-  const bool side_by_side = t[n - 1] - t[0] <= (step - layout.row) * es;
+  bool side_by_side = t[n - 1] - t[0] <= (step - layout.row) * es;
+  for (int d = 0; d < layout.dims; ++d) side_by_side = side_by_side && layout.st[d] % step == 0;
   for (int i = 0; i < n; ++i)
     for (int j = i + 1; j < n && t[j] - t[i] < layout.extent * es; ++j) {
       if (side_by_side ? t[j] - t[i] < layout.row * es : layout.meets((t[j] - t[i]) / es)) return 2;

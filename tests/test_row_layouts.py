@@ -65,7 +65,11 @@ FUSED = (3 * 4 * 2 * D, 4 * 2 * D, 2 * D)
 WIDE = (3 * 4 * 5 * D, 4 * 5 * D, 5 * D)
 PLAIN = (3 * 4 * D, 4 * D, D)
 HEADS_INSIDE = (3 * 4 * D, D, 3 * D)
+UNEVEN = (60 * D, 18 * D, 5 * D)                 # the next head is three rows' places and 3 D on
 PAIRS = [
+    (UNEVEN, UNEVEN, 3 * D, True),
+    (UNEVEN, UNEVEN, 2 * D, False),
+    (UNEVEN, UNEVEN, -4 * D, False),
     (PLAIN, PLAIN, 0, True),
     (PLAIN, PLAIN, D, True),                     # one row on
     (PLAIN, PLAIN, -4 * D, True),
