@@ -31,19 +31,14 @@
 // sequences of up to 32768 keys 191 + 5.6 us (contexts + join; some 6.8 TB/s of K and V); a
 // tree of 64 over 65472 keys 84 + 12 us (816 TFLOP/s), over 8128 22.6 + 8.6 us, of which the
 // partials of 256 workgroups (17 MB out and in) are some 5.
-#include "attn_common.h"
+#include "decode_common.h"
 #include "row_layout.h"
 
 namespace cab {
 namespace {
 
 constexpr int MAX_NODES = 256;
-constexpr int STEP = 32;        // keys of a wave's step in rows_kernel
-constexpr int QUAD = 4 * STEP;  // its pieces: a step for each of four waves
-constexpr int TILE = 64;        // tile_kernel's pieces
-// Pieces a workgroup of an even cut, up to which stretches begin anew with every unit (us, so
-// -> running on: 256 rows, 8 units of 8128 keys 33.5 -> 40.7, of 65472 99 -> 104).
-constexpr int FEW_PIECES = 32;
+constexpr int TILE = 64;  // tile_kernel's pieces (rows_kernel's: QUAD)
 
 struct TreeArgs {
   const char* q;
@@ -62,191 +57,14 @@ struct TreeArgs {
   float* pl;  // [number][R] row sums
 };
 
-__device__ __forceinline__ int context_length(const int32_t* lengths, int64_t length0, int64_t most,
-                                              int b) {
-  const int64_t n = lengths ? lengths[b] : length0;
-  return static_cast<int>(n < 0 ? 0 : n < most ? n : most);
-}
-
-// Sums over lanes 0 .. lane of a wave (lane moves within rows of 16, then row by row).
-__device__ __forceinline__ int wave_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15, 31
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
-  return x;
-}
-__device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
-
-// A lane's context lengths of sequences lane, lane + 64, ..; the first is kept.
-struct Lengths {
-  const TreeArgs& a;
-  int first;
-  __device__ __forceinline__ explicit Lengths(const TreeArgs& args) : a(args), first(0) {
-    if (lane_id() < a.B) first = context_length(a.lengths, a.length0, a.most, lane_id());
-  }
-  __device__ __forceinline__ int mine(int b0) const {  // of sequence b0 + lane, 0 past the last
-    if (b0 == 0) return first;
-    return b0 + lane_id() < a.B ? context_length(a.lengths, a.length0, a.most, b0 + lane_id()) : 0;
-  }
-  __device__ __forceinline__ int of(int b) const {  // b: the same in every lane
-    return __builtin_amdgcn_readfirstlane(
-        b < 64 ? __builtin_amdgcn_readlane(first, b) : context_length(a.lengths, a.length0, a.most, b));
-  }
-};
-
-__device__ __forceinline__ int round_to(int x, int grain) { return (x + grain - 1) / grain * grain; }
-
-// How the list is cut: pieces a workgroup takes, and what a unit's share of the list is
-// rounded up to. An even cut takes ceil(pieces / workgroups), and its stretches run on
-// from one unit into the next. Where that is only a few pieces, beginning a second part
-// costs as much as the pieces: then stretches begin anew with every unit, and are as
-// long as it takes for the workgroups to suffice.
-struct Cut {
-  int per, grain;
-};
-template <int KEYS>
-__device__ __forceinline__ int pieces_of(int length) { return (length + KEYS - 1) / KEYS; }
-
-template <int KEYS>
-__device__ __forceinline__ Cut list_cut(const TreeArgs& a, const Lengths& len) {
-  int all = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) all += wave_sum(pieces_of<KEYS>(len.mine(b0)));
-  int per = max(a.least, (all * a.Hkv + a.wgs - 1) / a.wgs);
-  if (per > FEW_PIECES || a.B * a.Hkv > a.wgs / 4) return Cut{per, 1};
-  for (;; ++per) {  // (ends: one a unit suffice)
-    int parts = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64)
-      parts += wave_sum((pieces_of<KEYS>(len.mine(b0)) + per - 1) / per);
-    if (parts * a.Hkv <= a.wgs) return Cut{per, per};
-  }
-}
-
-// f(sequence, head, first piece, pieces, length) for each part of workgroup x's stretch.
-template <int KEYS, typename F>
-__device__ __forceinline__ void over_stretch(const TreeArgs& a, int x, F f) {
-  const Lengths len(a);
-  const Cut cut = list_cut<KEYS>(a, len);
-  int at = x * cut.per;
-  int before = 0, b = -1, n = 0;  // n: the sequence's pieces, rounded up
-  for (int b0 = 0; b0 < a.B && b < 0; b0 += 64) {
-    const int mine = round_to(pieces_of<KEYS>(len.mine(b0)), cut.grain), upto = wave_scan(mine);
-    const uint64_t past = ballot64((before + upto) * a.Hkv > at);
-    if (past) {
-      const int i = __builtin_ctzll(past);
-      b = b0 + i;
-      n = __builtin_amdgcn_readlane(mine, i);
-      before += __builtin_amdgcn_readlane(upto, i) - n;
-    } else {
-      before += __builtin_amdgcn_readlane(upto, 63);
-    }
-  }
-  if (b < 0) return;  // past the list's end
-  at -= before * a.Hkv;
-  int head = at / n, piece = at - head * n;
-  for (int left = cut.per; left > 0;) {
-    const int length = len.of(b);
-    const int take = min(left, n - piece), there = pieces_of<KEYS>(length) - piece;
-    f(b, head, piece, min(take, there), length);  // (a rounded share ends in less than a stretch)
-    left -= take;
-    piece = 0;
-    if (++head == a.Hkv) {
-      head = 0;
-      do {
-        if (++b == a.B) return;
-        n = round_to(pieces_of<KEYS>(len.of(b)), cut.grain);
-      } while (n == 0);
-    }
-  }
-}
-
-// What weights are relative to, 2^(s c - level), for the maximum m: m c, and in fp16 15 less. There
-// weights of at most 1 would lose digits from 6e-5 and be 0 from 3e-8 down, which a long
-// context behind one large score adds up (140000 keys 17.4 below it: 0.4 % of the row sum
-// missing in O); 2^15 more, fp16's last power of two, keeps 11 bits to 1.9e-9. Beyond 2^24 the
-// level's own rounding is more than half a power of two, and nothing is added. (The factor in
-// s - m instead, one operation more a score, has no such border: 4 trees of 64 over 65472 keys 346
-// -> 355 us; levels formed anew in every step 334 -> 348, one token of 16 x 32768 209 -> 234.)
-template <cab_dtype_t DT>
-__device__ __forceinline__ float level_of(float m, float c) {
-  const float mc = m * c;
-  if constexpr (DT != CAB_F16) return mc;
-  return __builtin_fmaf(m, c, __builtin_fabsf(mc) < 16777216.f ? -15.f : 0.f);
-}
-// What sums relative to the maximum m's level are multiplied by for m1's.
-template <cab_dtype_t DT>
-__device__ __forceinline__ float relevel(float m, float level, float m1, float level1, float c) {
-  return __builtin_amdgcn_exp2f(DT == CAB_F16 ? level - level1 : (m - m1) * c);
-}
-
-// Non-temporal loads: K and V are read once, but in fp32 by every 32 rows of a unit.
-template <typename T>
-__device__ __forceinline__ T ld_stream(const char* p) {
-  return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
-}
-
-// A lane's K and V values of one 32-key step (l16 = lane % 16, g = lane / 16).
-// K: rows 16 tt + l16, 16 bytes at 64 j + 16 g. V: rows 16 tt + 4 g + r (number 4 tt
-// + r), values (D / 16) l16 ..: output tile dt takes the dt-th of them, so that its row
-// i is d = (D / 16) i + dt.
-template <cab_dtype_t DT, int HD>
-struct StepRegs {
-  static constexpr int ES = DT == CAB_F32 ? 4 : 2;
-  static constexpr int NJ = HD * ES / 64;
-  static constexpr int VB = HD / 16 * ES;
-  static constexpr int NV = VB / 8;
-  u32x4 k[2][NJ];
-  u32x2 v[8][NV];
-};
-
-template <cab_dtype_t DT, int HD, bool TAIL>
-__device__ __forceinline__ void load_step(StepRegs<DT, HD>& x, const char* kp, const char* vp,
-                                          uint32_t krow, uint32_t vrow, int left, int l16, int g) {
-  using SR = StepRegs<DT, HD>;
-#pragma unroll
-  for (int tt = 0; tt < 2; ++tt) {
-    const bool in = !TAIL || 16 * tt + l16 < left;
-#pragma unroll
-    for (int j = 0; j < SR::NJ; ++j) {
-      x.k[tt][j] = u32x4{0u, 0u, 0u, 0u};
-      if (in) x.k[tt][j] = ld_stream<u32x4>(kp + ((16u * tt + l16) * krow + 64u * j + 16u * g));
-    }
-  }
-#pragma unroll
-  for (int r = 0; r < 8; ++r) {
-    const int key = 16 * (r >> 2) + 4 * g + (r & 3);
-    const bool in = !TAIL || key < left;
-    const char* p = vp + (static_cast<uint32_t>(key) * vrow + SR::VB * l16);
-    if constexpr (SR::NV == 1) {
-      x.v[r][0] = u32x2{0u, 0u};
-      if (in) x.v[r][0] = ld_stream<u32x2>(p);
-    } else {
-#pragma unroll
-      for (int n = 0; n < SR::NV; n += 2) {
-        u32x4 y = {0u, 0u, 0u, 0u};
-        if (in) y = ld_stream<u32x4>(p + 8 * n);
-        x.v[r][n] = u32x2{y[0], y[1]};
-        x.v[r][n + 1] = u32x2{y[2], y[3]};
-      }
-    }
-  }
-}
-
-__device__ __forceinline__ f32x4 mfma4(float a, float b, const f32x4& c) {
-  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
-}
-
 // Grid: (workgroups, row tiles of 16 QT rows).
 template <cab_dtype_t DT, int HD, int QT>
 __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void rows_kernel(TreeArgs a) {
-  constexpr bool F32 = DT == CAB_F32, BF16 = DT == CAB_BF16;
+  constexpr bool F32 = DT == CAB_F32;
   constexpr int NDT = HD / 16;
   using SR = StepRegs<DT, HD>;
   constexpr int NJ = SR::NJ;
-  __shared__ f32x4 merge[4][NDT * 64];  // one query tile's O^T per wave
-  __shared__ float sm[4][QT][16], sl[4][QT][16];
+  __shared__ RowMerge<DT, HD, QT> merge;
 
   const int row0 = blockIdx.y * (16 * QT);
   const int w = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
@@ -271,16 +89,8 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void rows_kernel(TreeAr
         if (r < a.R) qr[qt][j] = *reinterpret_cast<const u32x4*>(qp + 64 * j + 16 * g);
       }
     }
-    f32x4 o[QT][NDT];
-    float l[QT], m[QT], level[QT];  // l: of this lane's keys alone
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-      l[qt] = 0.f;
-      m[qt] = M_EMPTY;
-      level[qt] = level_of<DT>(M_EMPTY, c);
-#pragma unroll
-      for (int dt = 0; dt < NDT; ++dt) o[qt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+    RowState<DT, HD, QT> rows;
+    rows.clear(c);
 
     auto load = [&](int step, SR& x) {
       const int left = len - STEP * step;
@@ -293,86 +103,7 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void rows_kernel(TreeAr
     };
     auto compute = [&](int step, const SR& x) {
       const int left = len - STEP * step;
-      f32x4 sc[QT][2];  // [qt][tt][r]: key 16 tt + 4 g + r, row 16 qt + l16
-#pragma unroll
-      for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt) sc[qt][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < NJ; ++j)
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt) {
-            if constexpr (F32) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t kx = x.k[tt][j][e], qx = qr[qt][j][e];
-                sc[qt][tt] = mfma4(__uint_as_float(kx), __uint_as_float(qx), sc[qt][tt]);
-              }
-            } else {
-              sc[qt][tt] = mfma16<BF16>(x.k[tt][j], qr[qt][j], sc[qt][tt]);
-            }
-          }
-      if (left < STEP) {
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-          for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (16 * tt + 4 * g + r >= left) sc[qt][tt][r] = -INFINITY;
-      }
-      u32x4 pb[QT];
-#pragma unroll
-      for (int qt = 0; qt < QT; ++qt) {
-        const float m0 = fmaxf(fmaxf(sc[qt][0][0], sc[qt][0][1]), fmaxf(sc[qt][0][2], sc[qt][0][3]));
-        const float m1 = fmaxf(fmaxf(sc[qt][1][0], sc[qt][1][1]), fmaxf(sc[qt][1][2], sc[qt][1][3]));
-        float mx = fmaxf(m0, m1), mdup = mx;
-        colmax2(mx, mdup);
-        if (__builtin_amdgcn_ballot_w64(mx > m[qt]) != 0) {
-          const float mn = fmaxf(mx, m[qt]);
-          const float upto = level_of<DT>(mn, c);
-          const float alpha = relevel<DT>(m[qt], level[qt], mn, upto, c);
-          l[qt] *= alpha;
-#pragma unroll
-          for (int dt = 0; dt < NDT; ++dt) o[qt][dt] *= alpha;
-          m[qt] = mn;
-          level[qt] = upto;
-        }
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            sc[qt][tt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qt][tt][r], c, -level[qt]));
-        const f32x4 s2 = sc[qt][0] + sc[qt][1];
-        l[qt] += (s2[0] + s2[1]) + (s2[2] + s2[3]);
-        if constexpr (!F32)
-          pb[qt] = u32x4{pack2<BF16>(sc[qt][0][0], sc[qt][0][1]), pack2<BF16>(sc[qt][0][2], sc[qt][0][3]),
-                         pack2<BF16>(sc[qt][1][0], sc[qt][1][1]), pack2<BF16>(sc[qt][1][2], sc[qt][1][3])};
-      }
-#pragma unroll
-      for (int dt = 0; dt < NDT; ++dt) {
-        if constexpr (F32) {
-#pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            const uint32_t vx = x.v[r][dt >> 1][dt & 1];
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
-              o[qt][dt] = mfma4(__uint_as_float(vx), sc[qt][r >> 2][r & 3], o[qt][dt]);
-          }
-        } else {
-          u32x4 vo;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t lo = x.v[2 * e][dt >> 2][(dt >> 1) & 1];
-            const uint32_t hi = x.v[2 * e + 1][dt >> 2][(dt >> 1) & 1];
-            vo[e] = __builtin_amdgcn_perm(hi, lo, dt & 1 ? 0x07060302u : 0x05040100u);
-          }
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt) o[qt][dt] = mfma16<BF16>(vo, pb[qt], o[qt][dt]);
-        }
-      }
+      rows.step(x, qr, c, left < STEP, [&](int tt, int r) { return 16 * tt + 4 * g + r < left; });
     };
 
     const int end = min((len + STEP - 1) / STEP, 4 * (piece + pieces));
@@ -399,41 +130,24 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void rows_kernel(TreeAr
       }
     }
 
-    // Merge of the four waves: common maximum, then the scaled O^T and sums in wave order.
     const int64_t part = static_cast<int64_t>(blockIdx.x) + b * a.Hkv + hk;
-    __syncthreads();  // (the last part's merge has been read)
+    merge.run(
+        rows, w, lane, c,
+        [&](int qt, int e, const f32x4& y) {
+          const int dt = e >> 6, ll = e & 63, row = row0 + 16 * qt + (ll & 15);
+          if (row < a.R) {
+            float* po = a.po + (part * a.R + row) * HD;
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-      l[qt] += shfl_xor_f32(l[qt], 16);
-      l[qt] += shfl_xor_f32(l[qt], 32);
-      if (g == 0) sm[w][qt][l16] = m[qt];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-      const float mm = fmaxf(fmaxf(sm[0][qt][l16], sm[1][qt][l16]), fmaxf(sm[2][qt][l16], sm[3][qt][l16]));
-      const float upto = level_of<DT>(mm, c);
-      const float f = relevel<DT>(m[qt], level[qt], mm, upto, c);
-      if (g == 0) sl[w][qt][l16] = l[qt] * f;
-#pragma unroll
-      for (int dt = 0; dt < NDT; ++dt) merge[w][dt * 64 + lane] = o[qt][dt] * f;
-      __syncthreads();
-      for (int e = threadIdx.x; e < NDT * 64; e += 256) {
-        const int dt = e >> 6, ll = e & 63, row = row0 + 16 * qt + (ll & 15);
-        const f32x4 y = (merge[0][e] + merge[1][e]) + (merge[2][e] + merge[3][e]);
-        if (row < a.R) {
-          float* po = a.po + (part * a.R + row) * HD;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) po[NDT * (4 * (ll >> 4) + r) + dt] = y[r];
-        }
-      }
-      const int row = row0 + 16 * qt + static_cast<int>(threadIdx.x);
-      if (threadIdx.x < 16 && row < a.R) {
-        a.pm[part * a.R + row] = upto;
-        a.pl[part * a.R + row] = (sl[0][qt][l16] + sl[1][qt][l16]) + (sl[2][qt][l16] + sl[3][qt][l16]);
-      }
-      if (qt + 1 < QT) __syncthreads();
-    }
+            for (int r = 0; r < 4; ++r) po[NDT * (4 * (ll >> 4) + r) + dt] = y[r];
+          }
+        },
+        [&](int qt, float level, float sum) {
+          const int row = row0 + 16 * qt + static_cast<int>(threadIdx.x);
+          if (row < a.R) {
+            a.pm[part * a.R + row] = level;
+            a.pl[part * a.R + row] = sum;
+          }
+        });
   });
 }
 
@@ -652,27 +366,6 @@ struct JoinArgs {
   float* lse;
 };
 
-// Eight values of a row in fp32.
-template <cab_dtype_t DT>
-__device__ __forceinline__ void load8(const char* p, float* x) {
-  if constexpr (DT == CAB_F32) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 16);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = a[i];
-      x[4 + i] = b[i];
-    }
-  } else {
-    const u32x4 a = *reinterpret_cast<const u32x4*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t w = a[i >> 1];
-      const uint16_t h = static_cast<uint16_t>(i & 1 ? w >> 16 : w);
-      x[i] = DT == CAB_BF16 ? bf16_to_f32(h) : f16_to_f32(h);
-    }
-  }
-}
-
 // One wave per row; groups of D / 8 lanes, each lane eight of the row's values. A group
 // takes every G-th partial and every G-th ancestor. KEYS: of the context's pieces.
 template <cab_dtype_t DT, int HD, int KEYS>
@@ -690,7 +383,7 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
   const int b = static_cast<int>(bh / a.H), h = static_cast<int>(bh - static_cast<int64_t>(b) * a.H);
   const int hk = h / ta.group;
   // The row's line: the node and its ancestors. A node that ends nowhere is absent.
-  const Lengths lens(ta);
+  const Lengths<TreeArgs> lens(ta);
   float q[8];
   load8<DT>(ta.q + b * ta.qs[0] + h * ta.qs[1] + node * ta.qs[2] + at * 8 * ES, q);
   const int32_t* parents = a.parents + b * a.parents_ld;
