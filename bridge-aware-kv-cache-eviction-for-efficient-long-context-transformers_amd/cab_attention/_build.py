@@ -53,6 +53,7 @@ def _hipcc() -> str:
 EXTRA_FLAGS = {
     "sparse_attn.hip": ["-Xarch_device", "-fno-honor-nans"],
     "tree_attn.hip": ["-Xarch_device", "-fno-honor-nans"],
+    "paged_attn.hip": ["-Xarch_device", "-fno-honor-nans"],
 }
 
 

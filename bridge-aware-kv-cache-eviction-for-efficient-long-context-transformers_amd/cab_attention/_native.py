@@ -21,7 +21,7 @@ from torch.utils._device import DeviceContext
 # host-sanitized one that tests/test_host_sanitizers.py runs the ABI checks on).
 LIB_PATH = pathlib.Path(os.environ.get("CAB_HIP_LIB") or
                         pathlib.Path(__file__).resolve().with_name("libcab_hip.so"))
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 CAB_OK, CAB_EINVAL, CAB_EDTYPE, CAB_ESHAPE, CAB_EWORKSPACE, CAB_EHIP = range(6)
 CAB_F32, CAB_F16, CAB_BF16 = 0, 1, 2
@@ -104,6 +104,21 @@ SIGNATURES = {
                                          _ptr, ctypes.c_size_t, _ptr]),
     "cab_verify_drafts_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, _i64, _i64, _i64,
                                                             ctypes.c_int, ctypes.c_int]),
+    "cab_rotary": (ctypes.c_int, [_i32, ctypes.POINTER(_ptr), ctypes.POINTER(_ptr), ctypes.c_int, _i64,
+                                  _i64x4, _i64, _i64, _i64x4, _i64x4, _ptr, _i64, _ptr, _i64,
+                                  ctypes.c_int, _f32, ctypes.c_int, _ptr]),
+    "cab_paged_append": (ctypes.c_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, ctypes.c_int, _i64, _i64,
+                                        _i64, _i64, _i64, _i64, _i64, _i64x4, _i64x4, _i64x4, _i64x4,
+                                        _i64x4, _i64x4, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _i64,
+                                        _ptr, _i64, ctypes.c_int, _f32, _ptr]),
+    "cab_paged_attn_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "cab_paged_attn_fwd": (ctypes.c_int, [_ptr, _ptr, _ptr, ctypes.c_int, _i64, _i64, _i64, _i64, _i64,
+                                          _i64, _i64x4, _i64x4, _i64x4, _i64x4, _ptr, _i64, _i64, _ptr,
+                                          _f32, _ptr, _ptr, _ptr, ctypes.c_size_t, _ptr]),
+    "cab_adjust_logits": (ctypes.c_int, [_ptr, _ptr, ctypes.c_int, _i64, _i64, _i64, _i64x4, _i64x4,
+                                         _ptr, _i64, _i64, _ptr, _ptr, _ptr, _f32, _ptr, _f32, _ptr,
+                                         _f32, _ptr, _ptr, _i64, _i64, _ptr, _i64x4, _ptr, _ptr,
+                                         _i64, _ptr]),
     "cab_token_frc": (ctypes.c_int, [_ptr, ctypes.c_int, _i64, _i64, _ptr, _ptr, _ptr, _ptr]),
     "cab_attention_symmetrize": (ctypes.c_int, [_ptr, ctypes.c_int, _i64, _i64, _i64, _i64, _i64x4,
                                                 _ptr, _i64, _ptr]),
@@ -295,6 +310,20 @@ def index32(t: torch.Tensor, name: str, shape: tuple) -> torch.Tensor:
         # (values past 32 bits stay out of range instead of wrapping round)
         t = t.clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32)
     return t if t.is_contiguous() else t.contiguous()
+
+
+def table32(t: torch.Tensor, name: str, rows: int):
+    """``(t, columns, row stride)``: ``t [rows, columns]`` as int32 whose rows are contiguous (itself
+    where it is one: a step of a server takes the first rows and columns of a larger table)."""
+    if t.dim() != 2 or t.shape[0] != rows:
+        raise ValueError(f"{name} must be [{rows}, columns]; got {list(t.shape)}")
+    if t.dtype is not torch.int32:
+        t = index32(t, name, t.shape)
+    columns, ld = t.shape[1], t.stride(0)
+    if (columns > 1 and t.stride(1) != 1) or (rows > 1 and 0 < ld < columns):
+        t = t.contiguous()
+        ld = columns
+    return t, columns, ld if rows > 1 else 0
 
 
 def wrote(*tensors: torch.Tensor) -> None:

@@ -14,6 +14,7 @@ import torch
 from torch import nn
 
 from .coarse_predictor import CoarseCurvaturePredictor
+from .kernels.rotary import Rotary
 from .kernels.sparse_attention import (SUPPORTED_BLOCK_SIZES, SUPPORTED_HEAD_DIMS,
                                        block_sparse_attention)
 
@@ -30,12 +31,14 @@ class CABAttention(nn.Module):
         lambda_redundancy: FRC redundancy weight.
         causal: token-causal attention (the predictor keeps only j <= i).
         qkv_bias: bias of the QKV projection.
+        rotary: turns queries and keys by their positions before blocks are chosen
+            (a :class:`Rotary` for this head dim); ``None``: none are.
         predictor_kwargs: forwarded to :class:`CoarseCurvaturePredictor`.
     """
 
     def __init__(self, dim: int, num_heads: int, block_size: int = 64, sparsity: float = 0.95,
                  lambda_redundancy: float = 0.5, causal: bool = False, qkv_bias: bool = False,
-                 **predictor_kwargs):
+                 rotary: Rotary | None = None, **predictor_kwargs):
         super().__init__()
         if dim % num_heads:
             raise ValueError(f"dim={dim} is not divisible by num_heads={num_heads}")
@@ -46,12 +49,15 @@ class CABAttention(nn.Module):
             raise ValueError(f"block_size={block_size} is not supported by the block-sparse "
                              f"executor (block_size in {SUPPORTED_BLOCK_SIZES}); "
                              "CoarseCurvaturePredictor alone accepts any block size")
+        if rotary is not None and rotary.head_dim != dim // num_heads:
+            raise ValueError(f"rotary is for heads of {rotary.head_dim} values, not {dim // num_heads}")
         self.dim = dim
         self.num_heads = num_heads
         self.head_dim = dim // num_heads
         self.causal = bool(causal)
         self.qkv = nn.Linear(dim, 3 * dim, bias=qkv_bias)
         self.proj = nn.Linear(dim, dim)
+        self.rotary = rotary
         self.predictor = CoarseCurvaturePredictor(block_size=block_size, sparsity=sparsity,
                                                   lambda_redundancy=lambda_redundancy,
                                                   causal=causal, **predictor_kwargs)
@@ -65,15 +71,21 @@ class CABAttention(nn.Module):
                                    causal=self.causal, out=out)
         return (o, pred[2]) if return_diagnostics else o
 
-    def forward(self, x: torch.Tensor, return_diagnostics: bool = False):
+    def forward(self, x: torch.Tensor, return_diagnostics: bool = False,
+                positions: torch.Tensor | None = None):
         """``x [B, N, dim]`` -> ``[B, N, dim]`` (and the predictor's
-        diagnostics dict with ``return_diagnostics``)."""
+        diagnostics dict with ``return_diagnostics``). positions: what ``rotary``
+        turns by, ``[N]`` or ``[B, N]`` (``None``: 0 .. N - 1)."""
+        if positions is not None and self.rotary is None:
+            raise ValueError("positions are for a module with rotary")
         B, N, C = x.shape
         H, Dh = self.num_heads, self.head_dim
         qkv = self.qkv(x).view(B, N, 3, H, Dh)
         q = qkv[:, :, 0].transpose(1, 2)  # [B, H, N, Dh] views, last dim contiguous
         k = qkv[:, :, 1].transpose(1, 2)
         v = qkv[:, :, 2].transpose(1, 2)
+        if self.rotary is not None:
+            q, k = self.rotary(q, k, positions)
         o = torch.empty((B, N, H, Dh), dtype=x.dtype, device=x.device)
         res = self.attend(q, k, v, return_diagnostics=return_diagnostics, out=o.transpose(1, 2))
         y = self.proj(o.view(B, N, C))

@@ -8,6 +8,9 @@ from .sparse_attention import (block_sparse_attention, block_sparse_attention_pa
 from .flash_attention_accumulate import (FlashAttentionWithAccumulation, flash_attention,
                                          flash_attention_with_cumulative_scores,
                                          get_all_cumulative_scores, key_scores, repeat_kv)
+from .adjust_logits import adjust_logits
+from .paged_attention import paged_attention
+from .rotary import Rotary
 from .tree_attention import tree_attention
 from .verify import verify_drafts
 from .token_frc import (compute_frc, compute_frc_pytorch, compute_frc_triton,
@@ -21,5 +24,6 @@ __all__ = [
     "key_scores", "flash_attention_with_cumulative_scores", "FlashAttentionWithAccumulation",
     "get_all_cumulative_scores", "repeat_kv", "compute_frc", "compute_frc_triton",
     "compute_frc_pytorch", "compute_node_strengths_triton", "compute_triangles_triton",
-    "tree_attention", "verify_drafts", "token_frc", "frc_from_keys", "symmetrize_attention",
+    "tree_attention", "verify_drafts", "Rotary", "paged_attention", "adjust_logits",
+    "token_frc", "frc_from_keys", "symmetrize_attention",
 ]

@@ -55,7 +55,7 @@ enum { CAB_NORM_NONE = 0, CAB_NORM_MINMAX = 1 };
 /* FRC combination (experiments/longbench_qa/config.py:465; test.ipynb:111-145). */
 enum { CAB_FRC_ADDITIVE = 0, CAB_FRC_MULTIPLICATIVE = 1, CAB_FRC_AUGMENTED = 2 };
 
-#define CAB_ABI_VERSION 12
+#define CAB_ABI_VERSION 13
 
 int cab_abi_version(void);
 const char* cab_last_error(void);
@@ -536,6 +536,101 @@ cab_status_t cab_verify_drafts(const void* logits, const void* draft_logits, cab
                                const float* uniforms, const float* noise, float temperature,
                                int32_t* path, int32_t* counts, int64_t* next_tokens,
                                void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Decoding over a paged cache with rotary positions (no counterparts in the
+ * reference, whose caches hold one length and take keys as they come). Tables,
+ * lengths, counts, positions: int32 device arrays, read when the work runs.
+ * Pages are [pages, H_kv, page_size, D] (any strides, last dim contiguous);
+ * row s of sequence b is place s % page_size of page table[b][s / page_size]
+ * (table_stride: entries from one sequence's row of the table to the next's;
+ * `columns` entries each). An entry outside [0, pages) is no page.
+ *
+ * cab_rotary turns pair i of the first rotary_dim values of every row of one or two tensors
+ * [B, heads[t], N, D] (4 strides each, one after the other) by positions[b][n] *
+ * turns[i] / 2^64 turns (positions_stride 0: one list for all; NULL: n), modulo
+ * 2^64 without rounding, and by `amplitude`: pair i is (i, i + rotary_dim / 2),
+ * or (2 i, 2 i + 1) if interleaved; (x, y) -> amplitude (x cos - y sin, x sin +
+ * y cos), in fp32, rounded once. inverse: by the negative angles, which is the
+ * gradient's. The other values are copied. out[t] is x[t] itself or shares no
+ * memory with the tensors. rotary_dim even, D <= 512, B * N < 2^24.
+ *
+ * cab_paged_append writes new rows k, v [B, H_kv, n, D] into pages: sequence
+ * b's row t < counts[b] (counts NULL: n) becomes its row lengths[b] + t. Rows
+ * whose page is not there, past the table, or of a sequence of negative length
+ * go nowhere. With rotary_dim > 0 k is turned as cab_rotary does it, by
+ * positions[b][t], or lengths[b] + t (positions NULL); so is q [B, H, n, D] into
+ * q_out (H 0: no q), all of its rows. Of new rows that meet in one place of a
+ * page one stays, piece by piece whichever. Nothing that is written shares memory with another
+ * tensor of the call, but q_out with q itself.
+ *
+ * cab_paged_attn_fwd: out[b,h] = softmax_s(q[b,h] . k_s * scale) v_s over sequence b's rows s <
+ * lengths[b] (taken as the nearest in [0, columns * page_size]) whose page is
+ * there, of head h / (H / H_kv); lse[b][h] (may be NULL) the natural-log log-sum-exp of the
+ * scaled scores. With no such row: 0 and -inf. Rows whose scores have no softmax (NaN or +inf among them, or
+ * all -inf) have NaN for both. What is behind a length or in no page of the sequence is
+ * not read. q, out: [B, H, 1, D], out is q itself or shares no memory with the
+ * inputs; D 64 or 128; H % H_kv == 0; 16-byte aligned rows; place strides
+ * in [0, 2^25] bytes. bf16, fp16 (P rounded to 16 bits as the products' operand, sums in fp32) or
+ * fp32. workspace: cab_paged_attn_workspace_bytes() bytes (may be 0), 16-byte aligned,
+ * overwritten.
+ *
+ * cab_adjust_logits prepares logits [B, T, V] (strides {b, t}, last dim
+ * contiguous) for the choice of the next token: with c the times token v is in
+ * history[b][prompt_lengths[b] .. lengths[b]) and (drafts given) on node t's line, which is
+ * t, its parent and so on as long as a parent is an earlier node;
+ *   if c > 0 or v is in history[b][0 .. prompt_lengths[b]):  x = x > 0 ? x / r : x r
+ *   x -= frequency c, and presence if c > 0;  x += bias of v;  v not allowed: -inf
+ * in fp32, rounded once; values of which nothing is asked pass as they are. history:
+ * int32 [B, history_len]; lengths NULL: history_len, prompt_lengths NULL: 0;
+ * tokens outside [0, V) are nobody's. r, presence, frequency: [B] arrays, or NULL and
+ * one value for all. bias_tokens, bias: [B, biases], of a token listed twice the last one counts. allowed:
+ * bit v % 32 of word v / 32 of int32 [B, T, (V + 31) / 32] (strides in words; 0: one
+ * mask for all), NULL: all. drafts: int64 [B, T], T <= 256, with parents as
+ * cab_verify_drafts takes them. out is logits itself or shares no memory with them.
+ */
+cab_status_t cab_rotary(int32_t n_tensors, const void* const* x, void* const* out,
+                        cab_dtype_t dtype, int64_t B, const int64_t* heads, int64_t N, int64_t D,
+                        const int64_t* x_strides, const int64_t* out_strides,
+                        const int32_t* positions, int64_t positions_stride, const uint64_t* turns,
+                        int64_t rotary_dim, int interleaved, float amplitude, int inverse,
+                        void* stream);
+
+cab_status_t cab_paged_append(const void* k, const void* v, void* k_pages, void* v_pages,
+                              const void* q, void* q_out, cab_dtype_t dtype, int64_t B, int64_t H,
+                              int64_t H_kv, int64_t n, int64_t D, int64_t pages, int64_t page_size,
+                              const int64_t k_strides[4], const int64_t v_strides[4],
+                              const int64_t k_page_strides[4], const int64_t v_page_strides[4],
+                              const int64_t q_strides[4], const int64_t q_out_strides[4],
+                              const int32_t* table, int64_t table_stride, int64_t columns,
+                              const int32_t* lengths, const int32_t* counts,
+                              const int32_t* positions, int64_t positions_stride,
+                              const uint64_t* turns, int64_t rotary_dim, int interleaved,
+                              float amplitude, void* stream);
+
+size_t cab_paged_attn_workspace_bytes(int64_t B, int64_t H, int64_t H_kv, int64_t columns,
+                                      int64_t page_size, int64_t D);
+
+cab_status_t cab_paged_attn_fwd(const void* q, const void* k_pages, const void* v_pages,
+                                cab_dtype_t dtype, int64_t B, int64_t H, int64_t H_kv, int64_t D,
+                                int64_t pages, int64_t page_size, const int64_t q_strides[4],
+                                const int64_t k_strides[4], const int64_t v_strides[4],
+                                const int64_t o_strides[4], const int32_t* table,
+                                int64_t table_stride, int64_t columns, const int32_t* lengths,
+                                float scale, void* out, float* lse, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
+cab_status_t cab_adjust_logits(const void* logits, void* out, cab_dtype_t dtype, int64_t B,
+                               int64_t T, int64_t V, const int64_t logit_strides[2],
+                               const int64_t out_strides[2], const int32_t* history,
+                               int64_t history_len, int64_t history_stride, const int32_t* lengths,
+                               const int32_t* prompt_lengths, const float* repetition,
+                               float repetition0, const float* presence, float presence0,
+                               const float* frequency, float frequency0,
+                               const int32_t* bias_tokens, const float* bias, int64_t biases,
+                               int64_t bias_stride, const int32_t* allowed,
+                               const int64_t allowed_strides[2], const int64_t* drafts,
+                               const int32_t* parents, int64_t parents_stride, void* stream);
 
 /*
  * Token-level Forman-Ricci curvature of a weighted directed graph A [n, n]
