@@ -63,25 +63,29 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     if v.dtype is not dt or k_pages.dtype is not dt or v_pages.dtype is not dt:
         raise TypeError("k, v and the pages must be of one dtype: bfloat16, float16 or float32")
     code = nat.dtype_code(k)
-    dev = nat.plain_index("append_paged", k, v, k_pages, v_pages, page_table, lengths)
+    given = [k, v, k_pages, v_pages, page_table, lengths]
+    for x in (counts, positions, q):
+        if x is not None:
+            given.append(x)
+    turns = None
+    if rotary is not None:
+        turns = rotary.turns
+        given.append(turns)
+    dev = nat.plain_index("append_paged", *given)
     if k_pages.is_inference() or v_pages.is_inference():
         _writable("append_paged", k_pages, v_pages)
     page_table, M, ld = nat.table32(page_table, "page_table", B)
     lengths = nat.index32(lengths, "lengths", (B,))
     if counts is not None:
-        nat.plain_index("append_paged", k, counts)
         counts = nat.index32(counts, "counts", (B,))
-    turns, dim, interleaved, amplitude, position_ld = None, 0, False, 1.0, 0
+    dim, interleaved, amplitude, position_ld = 0, False, 1.0, 0
     if rotary is not None:
         if rotary.head_dim != D:
             raise ValueError(f"rotary is for heads of {rotary.head_dim} values; got {D}")
-        nat.plain_index("append_paged", k, rotary.turns)
-        turns, dim = rotary.turns.data_ptr(), rotary.rotary_dim
-        interleaved, amplitude = rotary.interleaved, rotary.amplitude
+        dim, interleaved, amplitude = rotary.rotary_dim, rotary.interleaved, rotary.amplitude
     elif q is not None or positions is not None:
         raise ValueError("q and positions are for rotary")
     if positions is not None:
-        nat.plain_index("append_paged", k, positions)
         one = positions.dim() == 1
         positions = nat.index32(positions, "positions", (n,) if one else (B, n))
         position_ld = 0 if one else n
@@ -91,7 +95,6 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
             raise ValueError(f"q must be [{B}, H, {n}, {D}]; got {list(q.shape)}")
         if q.dtype is not dt:
             raise TypeError("q and k dtypes differ")
-        nat.plain_index("append_paged", k, q)
         if q.stride(3) != 1:
             q = q.contiguous()
         H, out = q.shape[1], torch.empty_like(q)
@@ -106,7 +109,7 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
             k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), nat.ptr(q), nat.ptr(out),
             code, B, H, H_kv, n, D, shape[0], shape[2], *strides, q_strides, out_strides,
             page_table.data_ptr(), ld, M, lengths.data_ptr(), nat.ptr(counts), nat.ptr(positions),
-            position_ld, turns, dim, interleaved, amplitude, nat.raw_stream(dev))
+            position_ld, nat.ptr(turns), dim, interleaved, amplitude, nat.raw_stream(dev))
     if st:
         nat.check("cab_paged_append", st)
     nat.wrote(k_pages, v_pages)

@@ -18,7 +18,6 @@ def _penalty(x, name: str, logits: torch.Tensor):
     B = logits.shape[0]
     if x.shape != (B,) or x.dtype is not torch.float32:
         raise ValueError(f"{name} must be a number or fp32 [{B}]; got {x.dtype} {list(x.shape)}")
-    nat.plain_index("adjust_logits", logits, x)
     return x.contiguous(), 0.0
 
 
@@ -61,24 +60,27 @@ def adjust_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
         out: where the result goes, like logits; the logits themselves, or memory of none of the
             inputs.
 
-    All arithmetic is in fp32, rounded once; values of which nothing is asked pass unchanged.
+    All arithmetic is in fp32, rounded once; values of which nothing is asked pass unchanged (a NaN
+    as a NaN).
     """
     if logits.dim() != 3:
         raise ValueError(f"logits must be [B, T, V]; got {list(logits.shape)}")
     B, T, V = logits.shape
-    dev = nat.plain_index("adjust_logits", logits)
+    given = [logits]
+    for x in (history, lengths, prompt_lengths, repetition, presence, frequency, bias_tokens, bias,
+              allowed, drafts, parents, out):
+        if x is not None and not isinstance(x, (float, int)):
+            given.append(x)
+    dev = nat.plain_index("adjust_logits", *given)
     dt = nat.dtype_code(logits)
     L = history_ld = 0
     if history is not None:
-        nat.plain_index("adjust_logits", logits, history)
         history, L, history_ld = nat.table32(history, "history", B)
     elif lengths is not None or prompt_lengths is not None:
         raise ValueError("lengths and prompt_lengths are the history's")
     if lengths is not None:
-        nat.plain_index("adjust_logits", logits, lengths)
         lengths = nat.index32(lengths, "lengths", (B,))
     if prompt_lengths is not None:
-        nat.plain_index("adjust_logits", logits, prompt_lengths)
         prompt_lengths = nat.index32(prompt_lengths, "prompt_lengths", (B,))
     repetition, repetition0 = _penalty(repetition, "repetition", logits)
     presence, presence0 = _penalty(presence, "presence", logits)
@@ -87,14 +89,12 @@ def adjust_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
         raise ValueError("bias_tokens and bias come together")
     n = bias_ld = 0
     if bias is not None:
-        nat.plain_index("adjust_logits", logits, bias_tokens, bias)
         if bias.dim() != 2 or bias.shape[0] != B or bias.dtype is not torch.float32:
             raise ValueError(f"bias must be fp32 [{B}, n]; got {bias.dtype} {list(bias.shape)}")
         n = bias_ld = bias.shape[1]
         bias_tokens, bias = nat.index32(bias_tokens, "bias_tokens", (B, n)), bias.contiguous()
     allowed_strides = None
     if allowed is not None:
-        nat.plain_index("adjust_logits", logits, allowed)
         W = -(-V // 32)
         if allowed.dtype is not torch.int32:
             raise TypeError(f"allowed must be int32 words of 32 bits; got {allowed.dtype}")
@@ -108,7 +108,6 @@ def adjust_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
         raise ValueError("drafts and parents come together")
     shared = True
     if drafts is not None:
-        nat.plain_index("adjust_logits", logits, drafts, parents)
         if drafts.shape != (B, T):
             raise ValueError(f"drafts must be {[B, T]}; got {list(drafts.shape)}")
         if drafts.dtype is not torch.int64:
@@ -123,7 +122,6 @@ def adjust_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
             raise ValueError("out must match the logits' shape and dtype")
         if out.stride(2) != 1:
             raise ValueError("out needs a contiguous last dim")
-        nat.plain_index("adjust_logits", logits, out)
         if nat.closed(out):
             raise RuntimeError("adjust_logits: out is an inference tensor; write to it in "
                                "inference mode")

@@ -183,13 +183,14 @@ class Rotary(torch.nn.Module):
                 raise ValueError("q and k must share B and N")
             if x.dtype is not q.dtype:
                 raise TypeError("q and k dtypes differ")
-        _plain("Rotary", *tensors, self.turns)
         nat.dtype_code(q)
+        given = (*tensors, self.turns) if positions is None else (*tensors, self.turns, positions)
+        record = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
+        (_plain if record else nat.plain_index)("Rotary", *given)
         if positions is not None:
-            _plain("Rotary", q, positions)
             B, N = q.shape[0], q.shape[2]
             positions = nat.index32(positions, "positions", (N,) if positions.dim() == 1 else (B, N))
-        if torch.is_grad_enabled() and any(x.requires_grad for x in tensors):
+        if record:
             out = _Turned.apply(self, positions, False, *tensors)
         else:
             out = _turn(self, positions, False, tensors)

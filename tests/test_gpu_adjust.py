@@ -236,3 +236,12 @@ def test_refusals_on_the_device(cuda):
         big = torch.zeros((1, 257, 4), device=cuda)
         adjust_logits(big, drafts=torch.zeros((1, 257), dtype=torch.int64, device=cuda),
                       parents=torch.zeros(257, dtype=torch.int32, device=cuda))
+
+
+def test_long_histories_and_lists(cuda):
+    """Histories and lists on both sides of 2^15, where counts and places share a word."""
+    for L, biases in ((32767, 5), (32768, 5), (40000, 70), (100, 32767), (100, 32768)):
+        a = setup(2, 1, 5000, L, "fp32", biases=biases)
+        a["history"][0] = 4999
+        a["lengths"][0], a["prompts"][0] = L, 0
+        check(a, call(a, cuda), "fp32")
