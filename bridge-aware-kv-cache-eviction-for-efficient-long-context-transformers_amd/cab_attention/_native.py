@@ -111,7 +111,7 @@ SIGNATURES = {
                                         _i64, _i64, _i64, _i64, _i64, _i64x4, _i64x4, _i64x4, _i64x4,
                                         _i64x4, _i64x4, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _i64,
                                         _ptr, _i64, ctypes.c_int, _f32, _ptr]),
-    "cab_paged_attn_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "cab_paged_attn_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, _i64, _i64, _i64, _i64, _i64, _i64]),
     "cab_paged_attn_fwd": (ctypes.c_int, [_ptr, _ptr, _ptr, ctypes.c_int, _i64, _i64, _i64, _i64, _i64,
                                           _i64, _i64x4, _i64x4, _i64x4, _i64x4, _ptr, _i64, _i64, _ptr,
                                           _f32, _ptr, _ptr, _ptr, ctypes.c_size_t, _ptr]),

@@ -68,7 +68,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         scale = 1.0 / math.sqrt(D)
     lib = nat.load()
     arr = nat.stride_array
-    wbytes = lib.cab_paged_attn_workspace_bytes(B, H, H_kv, M, S, D)
+    wbytes = lib.cab_paged_attn_workspace_bytes(dt, B, H, H_kv, M, S, D)
     ws = q.new_empty(wbytes, dtype=torch.uint8) if wbytes else None
     with nat.at_index(dev):
         st = lib.cab_paged_attn_fwd(

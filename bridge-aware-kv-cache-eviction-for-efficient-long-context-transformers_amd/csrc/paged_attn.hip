@@ -70,6 +70,9 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void paged_kernel(Paged
   constexpr int NDT = HD / 16;
   using SR = StepRegs<DT, HD>;
   constexpr int NJ = SR::NJ;
+  // (Two register sets spill with 32 rows of 128 in 16 bits, and gain nothing in fp32 but for 16 rows
+  // of 64: 8 x 4 heads of 5000 keys 28.0 -> 26.2 us.)
+  constexpr bool ONE_SET = F32 ? QT * HD > 64 : QT * HD > 128;
   __shared__ RowMerge<DT, HD, QT> merge;
   __shared__ int seen_by[4];
 
@@ -196,8 +199,7 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void paged_kernel(Paged
       constexpr int KEPT = 32;  // steps that a look-up holds the pages of
       int page, place;
       look_up(begin, page, place);
-      // (Two register sets spill with 32 rows of 128 in 16 bits.)
-      if constexpr (F32 || QT * HD > 128) {
+      if constexpr (ONE_SET) {
         Step x;
         int n = 0;
         for (int step = begin; step < end; step += 4) {
@@ -230,7 +232,7 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void paged_kernel(Paged
     } else {
       int page, place;
       look_up(begin, page, place);
-      if constexpr (F32 || QT * HD > 128) {
+      if constexpr (ONE_SET) {
         Step x;
         for (int step = begin; step < end; step += 4) {
           load(step, 0, page, place, x);
@@ -301,14 +303,17 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void paged_kernel(Paged
   }
 }
 
-// One wave per row; groups of D / 8 lanes, each lane eight of the row's values. A group takes
-// every G-th partial.
-template <cab_dtype_t DT, int HD>
+// WAVES waves per row; groups of D / 8 lanes, each lane eight of the row's values. A group takes
+// every G-th partial. (Four waves where rows are few, and so partials many: 28 rows of 64
+// partials JOIN4_US us.)
+template <cab_dtype_t DT, int HD, int WAVES>
 __global__ __launch_bounds__(256) void join_kernel(PagedArgs a) {
-  constexpr int LG = HD / 8, G = 64 / LG, ES = DT == CAB_F32 ? 4 : 2;
+  constexpr int LG = HD / 8, ES = DT == CAB_F32 ? 4 : 2;
+  constexpr int GROUPS = 64 / LG, G = GROUPS * WAVES;
+  __shared__ float sums[WAVES], rows[WAVES][HD];
   const int w = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
-  const int lane = lane_id(), grp = lane / LG, at = lane % LG;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + w;
+  const int lane = lane_id(), at = lane % LG, grp = lane / LG + (WAVES > 1 ? w * GROUPS : 0);
+  const int64_t id = WAVES > 1 ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + w;
   if (id >= static_cast<int64_t>(a.B) * a.H) return;
   const int b = static_cast<int>(id / a.H), h = static_cast<int>(id - static_cast<int64_t>(b) * a.H);
   const int hk = h / a.group;
@@ -331,7 +336,7 @@ __global__ __launch_bounds__(256) void join_kernel(PagedArgs a) {
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, shfl_xor_f32(m, off));
   float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, l = 0.f;
-  // (a +inf level is no -inf; only -inf itself is below the lowest finite value)
+  // (only -inf itself, no key seen, is below the lowest finite value; the same for all waves of a row)
   const bool any = m >= -3.4028234e38f;
   if (any) {
 #pragma unroll 4
@@ -350,11 +355,29 @@ __global__ __launch_bounds__(256) void join_kernel(PagedArgs a) {
 #pragma unroll
     for (int off = LG; off < 64; off <<= 1) l += shfl_xor_f32(l, off);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < 8; ++e)
 #pragma unroll
       for (int off = LG; off < 64; off <<= 1) o[e] += shfl_xor_f32(o[e], off);
-      o[e] *= 1.0f / l;
+    if constexpr (WAVES > 1) {
+      if (lane < LG) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) rows[w][8 * at + e] = o[e];
+        if (lane == 0) sums[w] = l;
+      }
+      __syncthreads();
+      l = 0.f;
+#pragma unroll
+      for (int v = 0; v < WAVES; ++v) l += sums[v];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        o[e] = 0.f;
+#pragma unroll
+        for (int v = 0; v < WAVES; ++v) o[e] += rows[v][8 * at + e];
+      }
     }
+    const float f = 1.0f / l;  // (of scores that are all -inf: 0 / 0)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] *= f;
   }
   if (grp != 0) return;
   char* op = a.out + b * a.os[0] + h * a.os[1] + at * 8 * ES;
@@ -375,18 +398,25 @@ struct PagedPlan {
   size_t off_pm, off_pl, bytes;
 };
 
-constexpr int WGS = 256;  // workgroups that share the list: one a CU
-// Places a sequence up to which a workgroup a unit does all of it.
-constexpr int64_t BRIEF = 512;
+// Workgroups that share the list: one a CU, or two where there are many units and so many parts a
+// workgroup, whose beginnings and ends the other one then fills (16 bits; us, one -> two a CU: 1024
+// units of up to 2048 keys 140 -> 130, 512 of up to 4096 129 -> 124, but 4 of 128000 57 -> 59).
+constexpr int WGS = 256;
+constexpr int64_t MANY_UNITS = 512;
+// Places a sequence up to which a workgroup does a unit alone, without partials and join; where
+// there is a unit a CU, the second number (us, list -> alone: 8 units of 608 keys 10.7 -> 9.8, 128 of
+// 1024 18.8 -> 20.2, 256 of up to 1024 28.7 -> 24.8, 1024 of up to 1024 86 -> 81, of up to 4096 256 -> 274).
+constexpr int64_t BRIEF = 640, BRIEF_FILLED = 1024;
 
-PagedPlan paged_plan(int64_t B, int64_t H, int64_t Hkv, int64_t most, int64_t D) {
+PagedPlan paged_plan(cab_dtype_t dtype, int64_t B, int64_t H, int64_t Hkv, int64_t most, int64_t D) {
   PagedPlan p;
   const int64_t group = H / Hkv;
   p.units = B * Hkv;
   p.row_tiles = ceil_div(group, group <= 16 ? 16 : 32);
-  p.direct = most <= BRIEF;
+  p.direct = most <= (p.units >= WGS ? BRIEF_FILLED : BRIEF);
   const int64_t list = p.units * ceil_div(most, QUAD);
-  p.wgs = ceil_div(WGS, p.row_tiles);
+  const int64_t slots = dtype != CAB_F32 && p.units >= MANY_UNITS ? 2 * WGS : WGS;
+  p.wgs = ceil_div(slots, p.row_tiles);
   if (p.wgs > list) p.wgs = list;
   if (p.wgs < 1) p.wgs = 1;
   const int64_t parts = p.direct ? 0 : (p.wgs + p.units) * group;
@@ -395,6 +425,8 @@ PagedPlan paged_plan(int64_t B, int64_t H, int64_t Hkv, int64_t most, int64_t D)
   p.bytes = p.off_pl + static_cast<size_t>(round_up(parts, 4)) * 4;
   return p;
 }
+
+constexpr int64_t FEW_JOINED = 256;  // rows that four waves each join
 
 bool paged_sizes(int64_t B, int64_t H, int64_t Hkv, int64_t columns, int64_t size, int64_t D) {
   return B >= 1 && B <= 65535 && Hkv >= 1 && H >= Hkv && H % Hkv == 0 && H <= 65535 && columns >= 0 &&
@@ -414,8 +446,12 @@ void launch(const PagedPlan& pl, const PagedArgs& a, bool blocks, hipStream_t s)
     else if (blocks) paged_kernel<DT, HD, 2, true><<<grid, 256, 0, s>>>(a);
     else paged_kernel<DT, HD, 2, false><<<grid, 256, 0, s>>>(a);
   }
-  if (!pl.direct)
-    join_kernel<DT, HD><<<static_cast<unsigned>(ceil_div(static_cast<int64_t>(a.B) * a.H, 4)), 256, 0, s>>>(a);
+  if (pl.direct) return;
+  const int64_t rows = static_cast<int64_t>(a.B) * a.H;
+  if (rows <= FEW_JOINED)
+    join_kernel<DT, HD, 4><<<static_cast<unsigned>(rows), 256, 0, s>>>(a);
+  else
+    join_kernel<DT, HD, 1><<<static_cast<unsigned>(ceil_div(rows, 4)), 256, 0, s>>>(a);
 }
 
 }  // namespace
@@ -423,10 +459,10 @@ void launch(const PagedPlan& pl, const PagedArgs& a, bool blocks, hipStream_t s)
 
 using namespace cab;
 
-extern "C" size_t cab_paged_attn_workspace_bytes(int64_t B, int64_t H, int64_t H_kv, int64_t columns,
+extern "C" size_t cab_paged_attn_workspace_bytes(cab_dtype_t dtype, int64_t B, int64_t H, int64_t H_kv, int64_t columns,
                                                  int64_t page_size, int64_t D) {
-  if (!paged_sizes(B, H, H_kv, columns, page_size, D)) return 0;
-  return paged_plan(B, H, H_kv, columns * page_size, D).bytes;
+  if (!valid_dtype(dtype) || !paged_sizes(B, H, H_kv, columns, page_size, D)) return 0;
+  return paged_plan(dtype, B, H, H_kv, columns * page_size, D).bytes;
 }
 
 extern "C" cab_status_t cab_paged_attn_fwd(
@@ -481,7 +517,7 @@ extern "C" cab_status_t cab_paged_attn_fwd(
                   !rows_share(out, rows, v_pages, RowLayout(v_strides, page_sizes, D), es),
               CAB_EINVAL, "%s: out shares memory with an input (only q itself may be out)", fn);
   const int64_t most = none ? 0 : columns * page_size;
-  const PagedPlan pl = paged_plan(B, H, H_kv, most, D);
+  const PagedPlan pl = paged_plan(dtype, B, H, H_kv, most, D);
   CAB_REQUIRE(pl.bytes == 0 || (workspace && workspace_bytes >= pl.bytes &&
                                 reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
               CAB_EWORKSPACE, "%s: workspace needs %zu bytes, 16-byte aligned", fn, pl.bytes);

@@ -10,10 +10,12 @@
 // of cosines is read. The top 32 bits (1.5e-9 rad) give the nearest quarter turn and a remainder
 // of at most an eighth, whose sine and cosine are Taylor polynomials to fp32's rounding.
 //
-// Bound: HBM, each row read and written once. A workgroup takes 4 tokens (1 where there are few),
-// forms their angles once for all heads (one a thread, through LDS) and then streams the
-// heads: 16 bytes of both of a pair's halves a lane, neighbouring lanes along the row, then
-// tokens, then heads.
+// Bound: HBM, each row read and written once. A workgroup takes 2 tokens (1 where there are few),
+// forms their angles once for all heads (through LDS) and streams the heads: 16 bytes of
+// both of a pair's halves a lane, neighbouring lanes along the row, then tokens, then heads; one
+// head in flight a thread, many waves. Measured, bf16, D = 128: 40 heads of 16384 tokens 63 us, 5.3 TB/s (4 tokens
+// and 4 heads in flight 75, 4 and 2 70, 2 and 1 67, so with non-temporal stores 63, loads too 62);
+// 8000 tokens into pages, 32 + 8 + 8 heads, 43 us (51); one token of 16 sequences 3.7 us.
 #include "attn_common.h"
 #include "row_layout.h"
 
@@ -21,8 +23,7 @@ namespace cab {
 namespace {
 
 constexpr int MAX_DIM = 512, MAX_PAIRS = MAX_DIM / 2;
-constexpr int TOKENS = 4;  // of a workgroup, at most
-constexpr int AHEAD = 4;   // heads loaded before the first of them is stored
+constexpr int TOKENS = 2;  // of a workgroup, at most
 constexpr int64_t MAX_ROWS = (1 << 24) - 1;  // a launch of up to 256 threads a token: below 2^32
 
 struct TurnTensor {
@@ -119,40 +120,13 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a) {
   using U = typename Unit<DT, P>::T;
   __shared__ float cosines[TOKENS * MAX_PAIRS], sines[TOKENS * MAX_PAIRS];
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.tokens;
-  for (int i = threadIdx.x; i < a.tokens * a.half; i += 256) {
-    const int r = i / a.half, j = i - r * a.half;
-    const int64_t row = row0 + r;
-    if (row >= a.rows) break;
-    const int64_t b = row / a.N;
-    const int32_t n = static_cast<int32_t>(row - b * a.N);
-    const int64_t p = a.positions ? a.positions[b * a.positions_ld + n]
-                                  : (a.lengths ? static_cast<int64_t>(a.lengths[b]) : 0) + n;
-    float s, c;
-    turn_sincos(static_cast<uint32_t>((static_cast<uint64_t>(p) * a.turns[j]) >> 32), s, c);
-    cosines[i] = c * a.amplitude;
-    sines[i] = s * (a.amplitude * a.sign);
-  }
-  __syncthreads();
-
   const int chunk = threadIdx.x % a.chunks, slot = threadIdx.x / a.chunks;
   const int lanes = 256 / a.chunks / a.tokens;  // heads side by side
   const int r = slot % a.tokens, lane = slot / a.tokens;
   const int64_t row = row0 + r;
-  if (lane >= lanes || row >= a.rows) return;
-  const int64_t b = row / a.N;
-  const int32_t n = static_cast<int32_t>(row - b * a.N);
-  // Where the row goes in the pages.
-  bool there = false;
-  int64_t page = 0, place = 0;
-  if (a.table) {
-    const int64_t len = a.lengths[b], to = len + n;
-    if (len >= 0 && to < static_cast<int64_t>(a.columns) * a.size && (!a.counts || n < a.counts[b])) {
-      const uint32_t col = static_cast<uint32_t>(to) / static_cast<uint32_t>(a.size);
-      page = a.table[b * a.table_ld + col];
-      place = to - static_cast<int64_t>(col) * a.size;
-      there = page >= 0 && page < a.pages;
-    }
-  }
+  const bool active = lane < lanes && row < a.rows;
+  const int64_t b = active ? row / a.N : 0;
+  const int32_t n = active ? static_cast<int32_t>(row - b * a.N) : 0;
   // The chunk's units.
   const int turning = a.half / P;
   int u0, u1;
@@ -163,61 +137,87 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a) {
     u0 = 2 * chunk;
     u1 = u0 + 1 < a.last ? u0 + 1 : u0;
   }
+  const int step = lanes * gridDim.y;
+  const int end = active ? a.upto[2] : 0;
+  auto tensor_of = [&](int h) { return h < a.upto[0] ? 0 : h < a.upto[1] ? 1 : 2; };
+  auto head_of = [&](int h, int t) { return t == 0 ? h : h - a.upto[t - 1]; };
+  U x, y;
+  auto fetch = [&](int h) {
+    if (h >= end) return;
+    const int t = tensor_of(h);
+    const TurnTensor& tt = a.t[t];
+    const char* from = tt.src + b * tt.ss[0] + head_of(h, t) * tt.ss[1] + n * tt.ss[2];
+    x = *reinterpret_cast<const U*>(from + u0 * static_cast<int>(sizeof(U)));
+    y = *reinterpret_cast<const U*>(from + u1 * static_cast<int>(sizeof(U)));
+  };
+  // The first head is asked for before the angles are formed.
+  int h = blockIdx.y * lanes + lane;
+  fetch(h);
+
+  for (int i = threadIdx.x; i < a.tokens * a.half; i += 256) {
+    const int q = i / a.half, j = i - q * a.half;
+    const int64_t other = row0 + q;
+    if (other >= a.rows) break;
+    const int64_t ob = other / a.N;
+    const int32_t on = static_cast<int32_t>(other - ob * a.N);
+    const int64_t p = a.positions ? a.positions[ob * a.positions_ld + on]
+                                  : (a.lengths ? static_cast<int64_t>(a.lengths[ob]) : 0) + on;
+    float s, c;
+    turn_sincos(static_cast<uint32_t>((static_cast<uint64_t>(p) * a.turns[j]) >> 32), s, c);
+    cosines[i] = c * a.amplitude;
+    sines[i] = s * (a.amplitude * a.sign);
+  }
+  // Where the row goes in the pages.
+  bool there = false;
+  int64_t page = 0, place = 0;
+  if (a.table && active) {
+    const int64_t len = a.lengths[b], to = len + n;
+    if (len >= 0 && to < static_cast<int64_t>(a.columns) * a.size && (!a.counts || n < a.counts[b])) {
+      const uint32_t col = static_cast<uint32_t>(to) / static_cast<uint32_t>(a.size);
+      page = a.table[b * a.table_ld + col];
+      place = to - static_cast<int64_t>(col) * a.size;
+      there = page >= 0 && page < a.pages;
+    }
+  }
+  lds_barrier();
   float cs[P], sn[P];
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     cs[i] = chunk < turning ? cosines[r * a.half + chunk * P + i] : 1.f;
     sn[i] = chunk < turning ? sines[r * a.half + chunk * P + i] : 0.f;
   }
-  const int step = lanes * gridDim.y;
-  for (int h0 = blockIdx.y * lanes + lane; h0 < a.upto[2]; h0 += AHEAD * step) {
-    U x[AHEAD], y[AHEAD];
-    char* to[AHEAD];
+  for (; h < end; h += step, fetch(h)) {
+    const bool in_pages = h >= a.paged;
+    if (in_pages && !there) continue;
+    if (chunk < turning && h < a.turned) {
+      float p[P], q[P], z[2 * P];
+      unpack<DT, P>(x, p);
+      unpack<DT, P>(y, q);
+      if constexpr (INTERLEAVED) {
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      to[i] = nullptr;
-      const int h = h0 + i * step;
-      if (h >= a.upto[2]) continue;
-      const int t = h < a.upto[0] ? 0 : h < a.upto[1] ? 1 : 2;
-      const int head = t == 0 ? h : h - a.upto[t == 1 ? 0 : 1];
-      const TurnTensor& tt = a.t[t];
-      const bool in_pages = h >= a.paged;
-      if (in_pages && !there) continue;
-      const char* from = tt.src + b * tt.ss[0] + head * tt.ss[1] + n * tt.ss[2];
-      to[i] = tt.dst + (in_pages ? page : b) * tt.ds[0] + head * tt.ds[1] +
-              (in_pages ? place : n) * tt.ds[2];
-      x[i] = *reinterpret_cast<const U*>(from + u0 * static_cast<int>(sizeof(U)));
-      y[i] = *reinterpret_cast<const U*>(from + u1 * static_cast<int>(sizeof(U)));
-    }
+        for (int e = 0; e < P; ++e) z[e] = p[e], z[P + e] = q[e];
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      if (!to[i]) continue;
-      if (chunk < turning && h0 + i * step < a.turned) {
-        float p[P], q[P], z[2 * P];
-        unpack<DT, P>(x[i], p);
-        unpack<DT, P>(y[i], q);
-        if constexpr (INTERLEAVED) {
-#pragma unroll
-          for (int e = 0; e < P; ++e) z[e] = p[e], z[P + e] = q[e];
-#pragma unroll
-          for (int e = 0; e < P; ++e) {
-            const float u = z[2 * e], v = z[2 * e + 1];
-            z[2 * e] = __builtin_fmaf(u, cs[e], -(v * sn[e]));
-            z[2 * e + 1] = __builtin_fmaf(u, sn[e], v * cs[e]);
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < P; ++e) {
-            z[e] = __builtin_fmaf(p[e], cs[e], -(q[e] * sn[e]));
-            z[P + e] = __builtin_fmaf(p[e], sn[e], q[e] * cs[e]);
-          }
+        for (int e = 0; e < P; ++e) {
+          const float u = z[2 * e], v = z[2 * e + 1];
+          z[2 * e] = __builtin_fmaf(u, cs[e], -(v * sn[e]));
+          z[2 * e + 1] = __builtin_fmaf(u, sn[e], v * cs[e]);
         }
-        x[i] = pack<DT, P>(z);
-        y[i] = pack<DT, P>(z + P);
+      } else {
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+          z[e] = __builtin_fmaf(p[e], cs[e], -(q[e] * sn[e]));
+          z[P + e] = __builtin_fmaf(p[e], sn[e], q[e] * cs[e]);
+        }
       }
-      *reinterpret_cast<U*>(to[i] + u0 * static_cast<int>(sizeof(U))) = x[i];
-      *reinterpret_cast<U*>(to[i] + u1 * static_cast<int>(sizeof(U))) = y[i];
+      x = pack<DT, P>(z);
+      y = pack<DT, P>(z + P);
     }
+    const int t = tensor_of(h);
+    const TurnTensor& tt = a.t[t];
+    char* to = tt.dst + (in_pages ? page : b) * tt.ds[0] + head_of(h, t) * tt.ds[1] +
+               (in_pages ? place : n) * tt.ds[2];
+    __builtin_nontemporal_store(x, reinterpret_cast<U*>(to + u0 * static_cast<int>(sizeof(U))));
+    __builtin_nontemporal_store(y, reinterpret_cast<U*>(to + u1 * static_cast<int>(sizeof(U))));
   }
 }
 

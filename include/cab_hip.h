@@ -608,8 +608,8 @@ cab_status_t cab_paged_append(const void* k, const void* v, void* k_pages, void*
                               const uint64_t* turns, int64_t rotary_dim, int interleaved,
                               float amplitude, void* stream);
 
-size_t cab_paged_attn_workspace_bytes(int64_t B, int64_t H, int64_t H_kv, int64_t columns,
-                                      int64_t page_size, int64_t D);
+size_t cab_paged_attn_workspace_bytes(cab_dtype_t dtype, int64_t B, int64_t H, int64_t H_kv,
+                                      int64_t columns, int64_t page_size, int64_t D);
 
 cab_status_t cab_paged_attn_fwd(const void* q, const void* k_pages, const void* v_pages,
                                 cab_dtype_t dtype, int64_t B, int64_t H, int64_t H_kv, int64_t D,

@@ -87,9 +87,10 @@ def test_append_validation(lib):
 
 def test_attention_validation(lib):
     ws = lib.cab_paged_attn_workspace_bytes
-    need = ws(3, 8, 2, 500, 16, 128)
-    assert need > 0
-    assert ws(3, 8, 3, 500, 16, 128) == 0 and ws(3, 8, 2, 500, 16, 96) == 0 and ws(3, 8, 2, 1 << 30, 16, 64) == 0
+    need = ws(nat.CAB_BF16, 3, 8, 2, 500, 16, 128)
+    assert need > 0 and ws(9, 3, 8, 2, 500, 16, 128) == 0
+    assert ws(0, 3, 8, 3, 500, 16, 128) == 0 and ws(0, 3, 8, 2, 500, 16, 96) == 0
+    assert ws(0, 3, 8, 2, 1 << 30, 16, 64) == 0
     qs, pool = arr(8 * 128, 128, 128, 1), arr(2 * 16 * 128, 16 * 128, 128, 1)
     call = lambda **w: lib.cab_paged_attn_fwd(
         w.get("q", FAKE), w.get("k", FAKE + (1 << 32)), FAKE + (1 << 33), w.get("dt", nat.CAB_BF16),
