@@ -67,9 +67,9 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     for x in (counts, positions, q):
         if x is not None:
             given.append(x)
-    turns = None
+    turns, plan, position_ld = None, (0, False, 1.0), 0
     if rotary is not None:
-        turns = rotary.turns
+        plan, turns = rotary.plan()
         given.append(turns)
     dev = nat.plain_index("append_paged", *given)
     if k_pages.is_inference() or v_pages.is_inference():
@@ -78,11 +78,9 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     lengths = nat.index32(lengths, "lengths", (B,))
     if counts is not None:
         counts = nat.index32(counts, "counts", (B,))
-    dim, interleaved, amplitude, position_ld = 0, False, 1.0, 0
     if rotary is not None:
         if rotary.head_dim != D:
             raise ValueError(f"rotary is for heads of {rotary.head_dim} values; got {D}")
-        dim, interleaved, amplitude = rotary.rotary_dim, rotary.interleaved, rotary.amplitude
     elif q is not None or positions is not None:
         raise ValueError("q and positions are for rotary")
     if positions is not None:
@@ -109,7 +107,7 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
             k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), nat.ptr(q), nat.ptr(out),
             code, B, H, H_kv, n, D, shape[0], shape[2], *strides, q_strides, out_strides,
             page_table.data_ptr(), ld, M, lengths.data_ptr(), nat.ptr(counts), nat.ptr(positions),
-            position_ld, nat.ptr(turns), dim, interleaved, amplitude, nat.raw_stream(dev))
+            position_ld, nat.ptr(turns), *plan, nat.raw_stream(dev))
     if st:
         nat.check("cab_paged_append", st)
     nat.wrote(k_pages, v_pages)

@@ -53,7 +53,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     page_table, M, ld = nat.table32(page_table, "page_table", B)
     lengths = nat.index32(lengths, "lengths", (B,))
     if out is None:
-        out = q.new_empty((B, H, 1, D))
+        out = torch.empty_like(q)
     else:
         if out.shape != q.shape or out.dtype is not q.dtype:
             raise ValueError("out must match q's shape and dtype")

@@ -6,15 +6,21 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
-from fractions import Fraction
 from typing import Optional
 
 import torch
 
 from .. import _native as nat
 
-# pi to 10^-53: turns are formed to the last of 64 bits.
-_PI = Fraction(314159265358979323846264338327950288419716939937510582, 10 ** 53)
+# 2 pi 10^53: turns are formed to the last of 64 bits.
+_TWO_PI = 628318530717958647692528676655900576839433879875021164
+
+
+def _turns(x: float) -> int:
+    """``x / (2 pi)`` modulo 1 in units of 2^-64, as the int64 of the same bits."""
+    n, d = x.as_integer_ratio()
+    t = ((n << 65) * 10 ** 53 // (d * _TWO_PI) + 1) // 2 % (1 << 64)
+    return t - (1 << 64) if t >> 63 else t
 
 
 def _frequencies(dim: int, base: float, scaling: Optional[dict]):
@@ -74,7 +80,8 @@ def _plain(fn: str, *tensors: torch.Tensor) -> None:
         raise RuntimeError(f"{fn} takes plain tensors outside transforms, tracing and modes")
 
 
-def _turn(rotary: "Rotary", positions, inverse: bool, tensors):
+def _turn(plan: tuple, turns: torch.Tensor, positions, inverse: bool, tensors):
+    """plan: (rotary_dim, interleaved, amplitude)."""
     tensors = [x if x.stride(3) == 1 else x.contiguous() for x in tensors]
     outs = [torch.empty_like(x) for x in tensors]
     n = len(tensors)
@@ -87,8 +94,7 @@ def _turn(rotary: "Rotary", positions, inverse: bool, tensors):
             nat.dtype_code(tensors[0]), B, nat.stride_array(tuple(x.shape[1] for x in tensors)), N, D,
             _joined(*[x.stride() for x in tensors]), _joined(*[x.stride() for x in outs]),
             nat.ptr(positions), 0 if positions is None or positions.dim() == 1 else N,
-            rotary.turns.data_ptr(), rotary.rotary_dim, rotary.interleaved, rotary.amplitude, inverse,
-            nat.raw_stream(dev))
+            turns.data_ptr(), *plan, inverse, nat.raw_stream(dev))
     if st:
         nat.check("cab_rotary", st)
     return outs
@@ -98,24 +104,24 @@ class _Turned(torch.autograd.Function):
     """One or two tensors turned together. A rotation's gradient is the rotation back."""
 
     @staticmethod
-    def forward(ctx, rotary, positions, inverse, *tensors):
-        ctx.rotary, ctx.inverse = rotary, inverse
+    def forward(ctx, plan, turns, positions, inverse, *tensors):
+        ctx.plan, ctx.inverse = plan, inverse
         ctx.set_materialize_grads(False)
         # (changed in place before the backward pass: an error, not other angles)
-        ctx.save_for_backward(rotary.turns, positions)
-        return tuple(_turn(rotary, positions, inverse, [x.detach() for x in tensors]))
+        ctx.save_for_backward(turns, positions)
+        return tuple(_turn(plan, turns, positions, inverse, [x.detach() for x in tensors]))
 
     @staticmethod
     def backward(ctx, *grads):
-        _, positions = ctx.saved_tensors
-        at = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[3 + i]]
+        turns, positions = ctx.saved_tensors
+        at = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[4 + i]]
         out = [None] * len(grads)
         if at:
             given = [grads[i] for i in at]
             _plain("Rotary's gradient", *given)
-            for i, x in zip(at, _Turned.apply(ctx.rotary, positions, not ctx.inverse, *given)):
+            for i, x in zip(at, _Turned.apply(ctx.plan, turns, positions, not ctx.inverse, *given)):
                 out[i] = x
-        return (None, None, None, *out)
+        return (None, None, None, None, *out)
 
 
 class Rotary(torch.nn.Module):
@@ -165,13 +171,19 @@ class Rotary(torch.nn.Module):
         self.interleaved = bool(interleaved)
         self.scaling = dict(scaling) if scaling else None
         self.frequencies, self.amplitude = _frequencies(self.rotary_dim, self.base, self.scaling)
-        turns = [round(Fraction(x) / (2 * _PI) * 2 ** 64) % 2 ** 64 for x in self.frequencies]
-        self.register_buffer("turns", torch.tensor([x - 2 ** 64 if x >= 2 ** 63 else x for x in turns],
-                                                   dtype=torch.int64), persistent=False)
+        self.register_buffer("turns", torch.tensor([_turns(x) for x in self.frequencies], dtype=torch.int64),
+                             persistent=False)
 
     def extra_repr(self) -> str:
         return (f"head_dim={self.head_dim}, rotary_dim={self.rotary_dim}, base={self.base}, "
                 f"interleaved={self.interleaved}, scaling={self.scaling}")
+
+    def plan(self):
+        """``((rotary_dim, interleaved, amplitude), turns)``, what the kernels take."""
+        turns = self.turns
+        if turns.dtype is not torch.int64 or turns.numel() != self.rotary_dim // 2:
+            raise RuntimeError("Rotary: the turns buffer has been converted; make a new module")
+        return (self.rotary_dim, self.interleaved, self.amplitude), turns
 
     def forward(self, q: torch.Tensor, k: Optional[torch.Tensor] = None,
                 positions: Optional[torch.Tensor] = None):
@@ -184,14 +196,15 @@ class Rotary(torch.nn.Module):
             if x.dtype is not q.dtype:
                 raise TypeError("q and k dtypes differ")
         nat.dtype_code(q)
-        given = (*tensors, self.turns) if positions is None else (*tensors, self.turns, positions)
+        plan, turns = self.plan()
+        given = (*tensors, turns) if positions is None else (*tensors, turns, positions)
         record = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
         (_plain if record else nat.plain_index)("Rotary", *given)
         if positions is not None:
             B, N = q.shape[0], q.shape[2]
             positions = nat.index32(positions, "positions", (N,) if positions.dim() == 1 else (B, N))
         if record:
-            out = _Turned.apply(self, positions, False, *tensors)
+            out = _Turned.apply(plan, turns, positions, False, *tensors)
         else:
-            out = _turn(self, positions, False, tensors)
+            out = _turn(plan, turns, positions, False, tensors)
         return out[0] if k is None else (out[0], out[1])

@@ -23,6 +23,8 @@
 namespace cab {
 namespace {
 
+constexpr float NO_KEY = -1.f;  // (a sum of weights is 0 or more, or NaN)
+
 struct PagedArgs {
   const char* q;
   const char* k;
@@ -43,8 +45,8 @@ struct PagedArgs {
   float* lse;     // [B, H], may be null
   // Partials; workgroup x's of unit u is number x + u.
   float* po;  // [number][group][D]
-  float* pm;  // [number][group] level of the maximum score, -inf: no key seen
-  float* pl;  // [number][group] row sums
+  float* pm;  // [number][group] level of the maximum score
+  float* pl;  // [number][group] row sums, NO_KEY where none was seen
 };
 
 // x / d for x d < 2^64.
@@ -285,7 +287,7 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void paged_kernel(Paged
           const bool any = (seen_by[0] | seen_by[1] | seen_by[2] | seen_by[3]) != 0;
           if (!whole) {
             a.pm[part * a.group + row] = any ? level : -INFINITY;
-            a.pl[part * a.group + row] = sum;
+            a.pl[part * a.group + row] = any ? sum : NO_KEY;
           } else if (a.lse) {
             const int64_t at = static_cast<int64_t>(b) * a.H + static_cast<int64_t>(hk) * a.group + row;
             reinterpret_cast<uint32_t*>(a.lse)[at] = lse_bits(any, level, sum);
@@ -331,13 +333,18 @@ __global__ __launch_bounds__(256) void join_kernel(PagedArgs a) {
   const int parts = pieces ? (start + pieces - 1) / cut.per - first + 1 : 0;
   if (parts == 1) return;  // (finished by the workgroup that had all of it)
   const int64_t row = (static_cast<int64_t>(first) + b * a.Hkv + hk) * a.group + (h - hk * a.group);
+  // (whether a key was seen goes by bits: levels may be NaN, and comparisons of those say anything)
   float m = -INFINITY;
-  for (int x = lane; x < parts; x += 64) m = fmaxf(m, a.pm[row + static_cast<int64_t>(x) * a.group]);
+  bool some = false;
+  for (int x = lane; x < parts; x += 64) {
+    const int64_t y = row + static_cast<int64_t>(x) * a.group;
+    m = fmaxf(m, a.pm[y]);
+    some = some || reinterpret_cast<const uint32_t*>(a.pl)[y] != __builtin_bit_cast(uint32_t, NO_KEY);
+  }
+  const bool any = ballot64(some) != 0;  // (the same for all waves of a row)
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, shfl_xor_f32(m, off));
   float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, l = 0.f;
-  // (only -inf itself, no key seen, is below the lowest finite value; the same for all waves of a row)
-  const bool any = m >= -3.4028234e38f;
   if (any) {
 #pragma unroll 4
     for (int x = grp; x < parts; x += G) {

@@ -198,6 +198,14 @@ def test_one_token_a_thousand_times(cuda):
     assert float(got[0, 0, 17]) == -1001.0 and not got[0, 0, :17].any() and not got[0, 0, 18:].any()
 
 
+def test_one_token_in_a_vocabulary(cuda):
+    x = torch.ones((2, 1, 9), device=cuda)[:, :, ::5][:, :, :1]
+    out = torch.zeros((2, 1, 9), device=cuda)[:, :, ::5][:, :, 1:]
+    h = torch.zeros((2, 3), dtype=torch.int32, device=cuda)
+    assert adjust_logits(x, h, frequency=2.0, out=out) is out and (out == -5.0).all()
+    assert (adjust_logits(x, h, frequency=2.0) == -5.0).all()
+
+
 def test_empty_calls(cuda):
     for shape in ((0, 1, 10), (2, 0, 10), (2, 1, 0)):
         assert adjust_logits(torch.empty(shape, device=cuda)).shape == shape

@@ -249,3 +249,53 @@ def test_refusals_on_the_device(cuda):
             ((q.double(), k.double(), v.double(), table, n), {}, TypeError, "dtype")):
         with pytest.raises(error, match=match):
             paged_attention(*args, **kw)
+
+
+@pytest.mark.parametrize("dt", list(DT))
+def test_scores_without_a_softmax_over_parts(cuda, dt):
+    """The same where several workgroups share the sequence: NaN or infinite keys in any part, a NaN
+    query, NaN in a V row, all scores -inf, and pages gone but for one part."""
+    host, (q, k, v, table, n) = setup(2, 4, 2, 64, 16, [3000, 2500], dt, cuda)
+    clean = paged_attention(q, k, v, table, n, return_lse=True)
+    check(host, clean, [3000, 2500], dt)
+    q = q.clone()
+    q[..., 0] = 1.0
+    clean = paged_attention(q, k, v, table, n, return_lse=True)
+    for key in (0, 1500, 2999):
+        page, place = int(table[0, key // 16]), key % 16
+        for value in (float("nan"), float("inf")):
+            k2 = k.clone()
+            k2[page, 0, place, 0] = value
+            out, lse = paged_attention(q, k2, v, table, n, return_lse=True)
+            assert torch.isnan(out[0, :2]).all() and torch.isnan(lse[0, :2]).all()
+            assert torch.equal(out[0, 2:], clean[0][0, 2:]) and torch.equal(out[1], clean[0][1])
+            assert torch.equal(lse[0, 2:], clean[1][0, 2:]) and torch.equal(lse[1], clean[1][1])
+        v2 = v.clone()
+        v2[page, 0, place, 9] = float("nan")
+        out, lse = paged_attention(q, k, v2, table, n, return_lse=True)
+        assert torch.isnan(out[0, :2, 0, 9]).all() and torch.equal(lse, clean[1])
+        assert int(torch.isnan(out).sum()) == 2
+    k2 = k.clone()
+    k2[table[0].long(), 0, :, 0] = -float("inf")
+    out, lse = paged_attention(q, k2, v, table, n, return_lse=True)
+    assert torch.isnan(out[0, :2]).all() and torch.isnan(lse[0, :2]).all() and torch.equal(out[0, 2:], clean[0][0, 2:])
+    q2 = q.clone()
+    q2[1, 3, 0, 5] = float("nan")
+    out, lse = paged_attention(q2, k, v, table, n, return_lse=True)
+    assert torch.isnan(out[1, 3]).all() and torch.isnan(lse[1, 3]).all()
+    assert torch.equal(out[0], clean[0][0]) and torch.equal(out[1, :3], clean[0][1, :3])
+    for kept in (0, 90, 187):  # one page left of sequence 0
+        t = table.clone()
+        t[0] = -1
+        t[0, kept] = table[0, kept]
+        got = paged_attention(q, k, v, t, n, return_lse=True)
+        check((q.cpu(), host[1], host[2], t.cpu().numpy()), got, [3000, 2500], dt)
+
+
+def test_values_that_are_infinite(cuda):
+    """An infinity in a V row that is seen is the output's."""
+    host, (q, k, v, table, n) = setup(1, 2, 1, 64, 16, [40], "bf16", cuda)
+    v2 = v.clone()
+    v2[int(table[0, 1]), 0, 3, 7] = -float("inf")
+    out = paged_attention(q, k, v2, table, n)
+    assert torch.isneginf(out[0, :, 0, 7]).all() and int((~torch.isfinite(out)).sum()) == 2

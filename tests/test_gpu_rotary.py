@@ -253,3 +253,19 @@ def test_attention_module(cuda, dt):
         assert not torch.equal(module(x), plain(x))
         zero = torch.zeros(300, dtype=torch.int32, device=cuda)
         assert torch.equal(module(x, positions=zero), plain(x))
+
+
+def test_backward_after_the_module_moved(cuda):
+    """What the forward pass took is kept for the backward pass, whatever becomes of the module."""
+    rot = Rotary(64).to(cuda)
+    x = rand((1, 2, 5, 64), "fp32", 1).to(cuda).requires_grad_()
+    g = rand((1, 2, 5, 64), "fp32", 2).to(cuda)
+    (want,) = torch.autograd.grad(rot(x), x, g)
+    y = rot(x)
+    rot.cpu()
+    rot.amplitude = 3.0
+    (got,) = torch.autograd.grad(y, x, g)
+    assert torch.equal(got, want)
+    rot.turns = rot.turns.float().to(cuda)
+    with pytest.raises(RuntimeError, match="turns"):
+        rot(x)
