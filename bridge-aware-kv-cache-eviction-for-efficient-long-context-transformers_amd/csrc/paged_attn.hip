@@ -17,6 +17,12 @@
 // offset a lane. Of other sizes a lane looks up one key of the step, one step ahead, and
 // the lanes that load the key's parts fetch its row from there.
 // Rows past the length or without a page are not read: zeros take their place, scores -inf.
+//
+// Bound: HBM (K and V, read once); short caches: the latency of a start, a few steps and a merge.
+// Measured, D = 128: 16 sequences of up to 32768 keys, 32 heads on 8, bf16, pages of 16, 200 + 4.8 us
+// (contexts + join; 6.7 TB/s of K and V; with pages in order, or of 64, the same within 4 %); one of 128000
+// keys, 28 heads on 4, fp16, 44 + 5.3; one of 600, 10, alone. fp32, D = 64, pages of 24: 3 x 12 heads of up to
+// 5003 keys 18.7 + 4.2.
 #include "decode_common.h"
 #include "row_layout.h"
 
@@ -307,7 +313,7 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void paged_kernel(Paged
 
 // WAVES waves per row; groups of D / 8 lanes, each lane eight of the row's values. A group takes
 // every G-th partial. (Four waves where rows are few, and so partials many: 28 rows of 64
-// partials JOIN4_US us.)
+// partials 7.5 -> 5.3 us.)
 template <cab_dtype_t DT, int HD, int WAVES>
 __global__ __launch_bounds__(256) void join_kernel(PagedArgs a) {
   constexpr int LG = HD / 8, ES = DT == CAB_F32 ? 4 : 2;
