@@ -78,6 +78,11 @@ CASES = [  # B, H, H_kv, S, lengths
     (70, 2, 1, 16, [(37 * i) % 200 for i in range(70)]),   # more than 64 sequences
     (80, 4, 4, 16, [600 + (91 * i) % 50 for i in range(80)]),  # units over workgroups' borders
     (2, 4, 2, 16, [-7, 5]),                   # a negative length
+    (3, 2, 1, 16, [639, 640, 641]),           # around what a workgroup takes whole of a few units
+    (64, 8, 4, 16, [1024 - 16 * (i % 3) for i in range(64)]),  # the same of a unit a CU
+    (70, 4, 2, 16, [(97 * i) % 1100 for i in range(70)]),      # a list of more than 64 sequences
+    (130, 4, 4, 16, [(31 * i) % 1200 for i in range(130)]),    # and of two workgroups a CU
+    (40, 40, 1, 16, [(211 * i) % 900 for i in range(40)]),     # three row tiles over one list
 ]
 
 
