@@ -413,22 +413,26 @@ struct PagedPlan {
 
 // Workgroups that share the list: one a CU, or two where there are many units and so many parts a
 // workgroup, whose beginnings and ends the other one then fills (16 bits; us, one -> two a CU: 1024
-// units of up to 2048 keys 140 -> 130, 512 of up to 4096 129 -> 124, but 4 of 128000 57 -> 59).
+// units of up to 2048 keys 140 -> 130, 512 of up to 4096 129 -> 124, but 4 of 128000 57 -> 59), or rows are
+// of 64, whose steps leave half as many bytes in flight (128 units of up to 32768 keys 150 -> 118, 8 of
+// 128000 67 -> 53, of 4096 10.4 both).
 constexpr int WGS = 256;
 constexpr int64_t MANY_UNITS = 512;
-// Places a sequence up to which a workgroup does a unit alone, without partials and join; where
-// there is a unit a CU, the second number (us, list -> alone: 8 units of 608 keys 10.7 -> 9.8, 128 of
-// 1024 18.8 -> 20.2, 256 of up to 1024 28.7 -> 24.8, 1024 of up to 1024 86 -> 81, of up to 4096 256 -> 274).
-constexpr int64_t BRIEF = 640, BRIEF_FILLED = 1024;
+// Places a sequence up to which a workgroup does a unit alone, without partials and join: of 16 bits,
+// of fp32 (as values of a row's length, whose matrix instructions take seven times as long), and where there
+// is a unit a CU (us, list -> alone: 16 bits, D = 128, 8 units of 608 keys 10.7 -> 9.8, 128 of 1024 18.8 -> 20.2,
+// 256 of up to 1024 28.7 -> 24.8, 1024 of up to 1024 86 -> 81, of up to 4096 256 -> 274; fp32, 8 units, D = 128, 200
+// keys 13.7 -> 13.5, 400 14.8 -> 20.1; D = 64, 400 10.6 both; 256 units, D = 128, of up to 1000 55 -> 51).
+constexpr int64_t BRIEF = 640, BRIEF_VALUES = 25600, BRIEF_FILLED = 1024;
 
 PagedPlan paged_plan(cab_dtype_t dtype, int64_t B, int64_t H, int64_t Hkv, int64_t most, int64_t D) {
   PagedPlan p;
   const int64_t group = H / Hkv;
   p.units = B * Hkv;
   p.row_tiles = ceil_div(group, group <= 16 ? 16 : 32);
-  p.direct = most <= (p.units >= WGS ? BRIEF_FILLED : BRIEF);
+  p.direct = most <= (p.units >= WGS ? BRIEF_FILLED : dtype == CAB_F32 ? BRIEF_VALUES / D : BRIEF);
   const int64_t list = p.units * ceil_div(most, QUAD);
-  const int64_t slots = dtype != CAB_F32 && p.units >= MANY_UNITS ? 2 * WGS : WGS;
+  const int64_t slots = dtype != CAB_F32 && (D == 64 || p.units >= MANY_UNITS) ? 2 * WGS : WGS;
   p.wgs = ceil_div(slots, p.row_tiles);
   if (p.wgs > list) p.wgs = list;
   if (p.wgs < 1) p.wgs = 1;

@@ -79,6 +79,11 @@ CASES = [  # B, H, H_kv, S, lengths
     (80, 4, 4, 16, [600 + (91 * i) % 50 for i in range(80)]),  # units over workgroups' borders
     (2, 4, 2, 16, [-7, 5]),                   # a negative length
     (3, 2, 1, 16, [639, 640, 641]),           # around what a workgroup takes whole of a few units
+    (3, 2, 1, 16, [0, 640, 600]),
+    (2, 2, 1, 16, [200, 130]),                # the same in fp32, D = 128
+    (2, 2, 1, 8, [208, 7]),
+    (2, 2, 1, 16, [400, 130]),                # and D = 64
+    (2, 2, 1, 8, [408, 390]),
     (64, 8, 4, 16, [1024 - 16 * (i % 3) for i in range(64)]),  # the same of a unit a CU
     (70, 4, 2, 16, [(97 * i) % 1100 for i in range(70)]),      # a list of more than 64 sequences
     (130, 4, 4, 16, [(31 * i) % 1200 for i in range(130)]),    # and of two workgroups a CU
