@@ -3,12 +3,34 @@ reference decodes over caches of one length that lie in one piece, and has no co
 
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional
 
 import torch
 
 from .. import _native as nat
+
+
+@functools.lru_cache(maxsize=1024)
+def _checked(q, kv, v, q_dtype, k_dtype, v_dtype):
+    """``(B, H, D, P, H_kv, S)`` of the shapes, once for each set of them (a step of a decoding
+    loop asks the same per layer)."""
+    if len(q) != 4 or q[2] != 1 or len(kv) != 4 or v != kv:
+        raise ValueError("q must be [B, H, 1, D], k_pages and v_pages two [P, H_kv, S, D]")
+    if kv[3] != q[3]:
+        raise ValueError(f"k_pages and v_pages must be [P, H_kv, S, D={q[3]}]; got {list(kv)}")
+    if not (q_dtype is k_dtype is v_dtype):
+        raise TypeError("q, k_pages and v_pages dtypes differ")
+    return q[0], q[1], q[3], kv[0], kv[1], kv[2]
+
+
+@functools.lru_cache(maxsize=1024)
+def _layout(dt, sizes, columns, *strides):
+    """The workspace's bytes and the strides as C integers."""
+    B, H, D, _, H_kv, S = sizes
+    need = nat.load().cab_paged_attn_workspace_bytes(dt, B, H, H_kv, columns, S, D)
+    return need, tuple(nat.stride_array(x) for x in strides)
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -39,15 +61,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     Returns the output ``[B, H, 1, D]``, with ``return_lse`` also the fp32 natural-log
     log-sum-exp ``[B, H, 1]``.
     """
-    shape = k_pages.shape
-    if q.dim() != 4 or q.shape[2] != 1 or len(shape) != 4 or v_pages.shape != shape:
-        raise ValueError("q must be [B, H, 1, D], k_pages and v_pages two [P, H_kv, S, D]")
-    B, H, _, D = q.shape
-    P, H_kv, S, _ = shape
-    if shape[3] != D:
-        raise ValueError(f"k_pages and v_pages must be [P, H_kv, S, D={D}]; got {list(shape)}")
-    if not (q.dtype is k_pages.dtype is v_pages.dtype):
-        raise TypeError("q, k_pages and v_pages dtypes differ")
+    sizes = _checked(q.shape, k_pages.shape, v_pages.shape, q.dtype, k_pages.dtype, v_pages.dtype)
+    B, H, D, P, H_kv, S = sizes
     dev = nat.plain_index("paged_attention", q, k_pages, v_pages, page_table, lengths)
     dt = nat.dtype_code(q)
     page_table, M, ld = nat.table32(page_table, "page_table", B)
@@ -66,16 +81,14 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     lse = q.new_empty((B, H, 1), dtype=torch.float32) if return_lse else None
     if scale is None:
         scale = 1.0 / math.sqrt(D)
-    lib = nat.load()
-    arr = nat.stride_array
-    wbytes = lib.cab_paged_attn_workspace_bytes(dt, B, H, H_kv, M, S, D)
+    wbytes, strides = _layout(dt, sizes, M, q.stride(), k_pages.stride(), v_pages.stride(),
+                              out.stride())
     ws = q.new_empty(wbytes, dtype=torch.uint8) if wbytes else None
     with nat.at_index(dev):
-        st = lib.cab_paged_attn_fwd(
+        st = nat.load().cab_paged_attn_fwd(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), dt, B, H, H_kv, D, P, S,
-            arr(q.stride()), arr(k_pages.stride()), arr(v_pages.stride()), arr(out.stride()),
-            page_table.data_ptr(), ld, M, lengths.data_ptr(), scale, out.data_ptr(), nat.ptr(lse),
-            nat.ptr(ws), wbytes, nat.raw_stream(dev))
+            *strides, page_table.data_ptr(), ld, M, lengths.data_ptr(), scale, out.data_ptr(),
+            nat.ptr(lse), nat.ptr(ws), wbytes, nat.raw_stream(dev))
     if st:
         nat.check("cab_paged_attn_fwd", st)
     return (out, lse) if return_lse else out
