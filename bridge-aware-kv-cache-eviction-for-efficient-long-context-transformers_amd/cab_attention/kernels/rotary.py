@@ -12,14 +12,14 @@ import torch
 
 from .. import _native as nat
 
-# 2 pi 10^53: turns are formed to the last of 64 bits.
-_TWO_PI = 628318530717958647692528676655900576839433879875021164
+# 2^150 / (2 pi), from 2 pi to 53 digits: turns are formed to the last of 64 bits.
+_TURN = (10 ** 53 << 150) // 628318530717958647692528676655900576839433879875021164
 
 
 def _turns(x: float) -> int:
     """``x / (2 pi)`` modulo 1 in units of 2^-64, as the int64 of the same bits."""
-    n, d = x.as_integer_ratio()
-    t = ((n << 65) * 10 ** 53 // (d * _TWO_PI) + 1) // 2 % (1 << 64)
+    n, d = x.as_integer_ratio()  # (d: a power of two)
+    t = (n * _TURN >> d.bit_length() + 84) + 1 >> 1 & (1 << 64) - 1
     return t - (1 << 64) if t >> 63 else t
 
 
@@ -119,7 +119,10 @@ class _Turned(torch.autograd.Function):
         if at:
             given = [grads[i] for i in at]
             _plain("Rotary's gradient", *given)
-            for i, x in zip(at, _Turned.apply(ctx.plan, turns, positions, not ctx.inverse, *given)):
+            back = (ctx.plan, turns, positions, not ctx.inverse)
+            # (recorded only for gradients of gradients)
+            turned = _Turned.apply(*back, *given) if torch.is_grad_enabled() else _turn(*back, given)
+            for i, x in zip(at, turned):
                 out[i] = x
         return (None, None, None, None, *out)
 
