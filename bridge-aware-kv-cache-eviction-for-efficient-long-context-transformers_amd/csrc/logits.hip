@@ -368,14 +368,17 @@ extern "C" cab_status_t cab_adjust_logits(
                   T <= INT32_MAX / 2,
               CAB_ESHAPE, "%s: problem too large", fn);
   const bool tree = drafts != nullptr, with_bias = biases > 0;
-  // The longest stretch that leaves some four workgroups a CU.
+  // The longest stretch that leaves a workgroup a CU, and as many groups of a tree's nodes, each of
+  // which counts the history anew, as make three of them. (us, with 4 for both -> so: 8 rows of
+  // 128000, histories of 8000, 7.5 -> 5.2; trees of 26 x 50001 10.0 -> 8.4; 4 x 64 x 32000 22.8 -> 17.1;
+  // 8 x 32 x 128000 35.8 -> 32.7; two groups a CU there 34.6, 4 x 26 x 50001 14.0 -> 15.6.)
   // (in a tree the T nodes of a line are counted too)
   const int places = !with_bias ? NO_PLACES
                      : history_len + (tree ? T : 0) < HALF && biases < HALF ? HALVES : WORDS;
   int64_t stretch = places == WORDS ? 4096 : 8192;  // (at most 64 KB of LDS)
-  while (stretch > 1024 && ceil_div(V, stretch) * T < ceil_div(1024, B)) stretch /= 2;
+  while (stretch > 1024 && ceil_div(V, stretch) * T < ceil_div(256, B)) stretch /= 2;
   const int64_t stretches = ceil_div(V, stretch);
-  int64_t groups = ceil_div(1024, B);
+  int64_t groups = ceil_div(768, B);
   groups = ceil_div(groups, stretches);
   if (groups > T) groups = T;
   const int64_t nodes = ceil_div(T, groups);

@@ -443,7 +443,9 @@ PagedPlan paged_plan(cab_dtype_t dtype, int64_t B, int64_t H, int64_t Hkv, int64
   return p;
 }
 
-constexpr int64_t FEW_JOINED = 256;  // rows that four waves each join
+// Rows up to which four waves join each (us, one -> four: 32 rows, 128000 keys 46.6 -> 43.4, 256 of up to
+// 16000 73 -> 65, 512 of up to 8000 63 -> 65).
+constexpr int64_t FEW_JOINED = 256;
 
 bool paged_sizes(int64_t B, int64_t H, int64_t Hkv, int64_t columns, int64_t size, int64_t D) {
   return B >= 1 && B <= 65535 && Hkv >= 1 && H >= Hkv && H % Hkv == 0 && H <= 65535 && columns >= 0 &&
