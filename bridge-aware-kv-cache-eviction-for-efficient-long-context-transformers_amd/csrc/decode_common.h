@@ -215,6 +215,24 @@ __device__ __forceinline__ f32x4 mfma4(float a, float b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
+// Two weights' upper 16 bits (rounded towards 0), as fp32 again, and the least rest that is no zero.
+template <bool BF16>
+__device__ __forceinline__ uint32_t cut2(float lo, float hi) {
+  if constexpr (BF16)
+    return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo, hi));
+}
+template <bool BF16>
+__device__ __forceinline__ float low_half(uint32_t x) {
+  return BF16 ? __uint_as_float(x << 16) : f16_to_f32(static_cast<uint16_t>(x));
+}
+template <bool BF16>
+__device__ __forceinline__ float high_half(uint32_t x) {
+  return BF16 ? __uint_as_float(x & 0xffff0000u) : f16_to_f32(static_cast<uint16_t>(x >> 16));
+}
+template <bool BF16> constexpr float LEAST = BF16 ? 0x1p-120f : 0x1p-24f;
+
 // QT tiles of 16 query rows and what they have seen, of one wave (l16 = lane % 16: a
 // tile's row, g = lane / 16).
 template <cab_dtype_t DT, int HD, int QT>
@@ -237,8 +255,10 @@ struct RowState {
     }
   }
 
-  // 32 keys; with `some`, of those alone for which in(tt, r) (key 16 tt + 4 g + r).
-  template <typename F>
+  // 32 keys; with `some`, of those alone for which in(tt, r) (key 16 tt + 4 g + r). BOTH: 16-bit weights
+  // as two operands, the upper bits cut off and the rest, so that only the output's rounding is
+  // left (the rest of a weight is never 0: times an infinite V that would be NaN).
+  template <bool BOTH = false, typename F>
   __device__ __forceinline__ void step(const SR& x, const u32x4 (&qr)[QT][NJ], float c, bool some, F in) {
     f32x4 sc[QT][2];  // [qt][tt][r]: key 16 tt + 4 g + r, row 16 qt + l16
 #pragma unroll
@@ -270,7 +290,7 @@ struct RowState {
           for (int r = 0; r < 4; ++r)
             if (!in(tt, r)) sc[qt][tt][r] = -INFINITY;
     }
-    u32x4 pb[QT];
+    u32x4 pb[QT], rest[QT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       const float m0 = fmaxf(fmaxf(sc[qt][0][0], sc[qt][0][1]), fmaxf(sc[qt][0][2], sc[qt][0][3]));
@@ -294,9 +314,22 @@ struct RowState {
           sc[qt][tt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qt][tt][r], c, -level[qt]));
       const f32x4 s2 = sc[qt][0] + sc[qt][1];
       l[qt] += (s2[0] + s2[1]) + (s2[2] + s2[3]);
-      if constexpr (!F32)
+      if constexpr (!F32 && BOTH) {
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int r = 0; r < 4; r += 2) {
+            const float a = sc[qt][tt][r], b = sc[qt][tt][r + 1];
+            const uint32_t cut = cut2<BF16>(a, b);
+            pb[qt][2 * tt + r / 2] = cut;
+            rest[qt][2 * tt + r / 2] =
+                pack2<BF16>(fmaxf(a - low_half<BF16>(cut), fminf(a, LEAST<BF16>)),
+                            fmaxf(b - high_half<BF16>(cut), fminf(b, LEAST<BF16>)));
+          }
+      } else if constexpr (!F32) {
         pb[qt] = u32x4{pack2<BF16>(sc[qt][0][0], sc[qt][0][1]), pack2<BF16>(sc[qt][0][2], sc[qt][0][3]),
                        pack2<BF16>(sc[qt][1][0], sc[qt][1][1]), pack2<BF16>(sc[qt][1][2], sc[qt][1][3])};
+      }
     }
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) {
@@ -317,7 +350,10 @@ struct RowState {
           vo[e] = __builtin_amdgcn_perm(hi, lo, dt & 1 ? 0x07060302u : 0x05040100u);
         }
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) o[qt][dt] = mfma16<BF16>(vo, pb[qt], o[qt][dt]);
+        for (int qt = 0; qt < QT; ++qt) {
+          o[qt][dt] = mfma16<BF16>(vo, pb[qt], o[qt][dt]);
+          if constexpr (BOTH) o[qt][dt] = mfma16<BF16>(vo, rest[qt], o[qt][dt]);
+        }
       }
     }
   }

@@ -5,8 +5,10 @@
 //  1. The contexts of all units, cut into pieces of 128 keys, make one list of which each
 //     workgroup takes an equal stretch. Every wave walks its own 32-key steps, K and V straight
 //     from the pages into matrix operands (S^T = K Q^T, online softmax in the log2 domain,
-//     O^T += V^T P^T; maxima, sums and O in fp32, P rounded to 16 bits as the operand, half a step
-//     of each weight; fp32 on the fp32 matrix instructions). A part that is all of a unit
+//     O^T += V^T P^T; maxima, sums and O in fp32; P as two 16-bit operands, its upper bits and
+//     the rest, so that bf16 outputs are as near as their own rounding, 1.7e-3 in place of
+//     1.9e-3 in norm; the second product costs 0.3 us of 10 at 600 keys and nothing that shows at
+//     long contexts; fp32 on the fp32 matrix instructions). A part that is all of a unit
 //     is finished there; of the others one partial (level, row sum, O) is left per row.
 //  2. join_kernel, one wave per row, merges the partials. Where one workgroup a unit does
 //     (paged_plan), there are none and it is not launched.
@@ -19,10 +21,10 @@
 // Rows past the length or without a page are not read: zeros take their place, scores -inf.
 //
 // Bound: HBM (K and V, read once); short caches: the latency of a start, a few steps and a merge.
-// Measured, D = 128: 16 sequences of up to 32768 keys, 32 heads on 8, bf16, pages of 16, 200 + 4.8 us
-// (contexts + join; 6.7 TB/s of K and V; with pages in order, or of 64, the same within 4 %); one of 128000
-// keys, 28 heads on 4, fp16, 44 + 5.3; one of 600, 10, alone. fp32, D = 64, pages of 24: 3 x 12 heads of up to
-// 5003 keys 18.7 + 4.2.
+// Measured, D = 128: 16 sequences of up to 32768 keys, 32 heads on 8, bf16, pages of 16, 202 + 4.7 us
+// (contexts + join; 6.6 TB/s of K and V; with pages in order, or of 64, the same within 4 %); one of 128000
+// keys, 28 heads on 4, fp16, 45 + 5.2; one of 600, 10.4, alone. fp32, D = 64, pages of 24: 3 x 12 heads of up to
+// 5003 keys 19.1 + 4.2.
 #include "decode_common.h"
 #include "row_layout.h"
 
@@ -200,7 +202,7 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void paged_kernel(Paged
     auto compute = [&](const Step& s) __attribute__((always_inline)) {
       const uint64_t some = __builtin_amdgcn_ballot_w64(s.in != 255u);
       seen |= static_cast<int>(__builtin_amdgcn_ballot_w64(s.in != 0) != 0);
-      rows.step(s.x, qr, c, some != 0, [&](int tt, int r) { return (s.in >> (4 * tt + r) & 1u) != 0; });
+      rows.template step<true>(s.x, qr, c, some != 0, [&](int tt, int r) { return (s.in >> (4 * tt + r) & 1u) != 0; });
     };
 
     if constexpr (BLOCKS) {

@@ -302,10 +302,28 @@ def test_scores_without_a_softmax_over_parts(cuda, dt):
         check((q.cpu(), host[1], host[2], t.cpu().numpy()), got, [3000, 2500], dt)
 
 
-def test_values_that_are_infinite(cuda):
-    """An infinity in a V row that is seen is the output's."""
-    host, (q, k, v, table, n) = setup(1, 2, 1, 64, 16, [40], "bf16", cuda)
-    v2 = v.clone()
-    v2[int(table[0, 1]), 0, 3, 7] = -float("inf")
-    out = paged_attention(q, k, v2, table, n)
-    assert torch.isneginf(out[0, :, 0, 7]).all() and int((~torch.isfinite(out)).sum()) == 2
+@pytest.mark.parametrize("dt", list(DT))
+def test_values_that_are_infinite(cuda, dt):
+    """An infinity in a V row that is seen is the output's, whole and over parts."""
+    for n in (40, 3000):
+        host, (q, k, v, table, m) = setup(1, 2, 1, 64, 16, [n], dt, cuda)
+        q.zero_()  # all weights alike, and a power of two relative to the level: nothing left of them
+        v2 = v.clone()
+        v2[int(table[0, 1]), 0, 3, 7] = -float("inf")
+        out = paged_attention(q, k, v2, table, m)
+        assert torch.isneginf(out[0, :, 0, 7]).all() and int((~torch.isfinite(out)).sum()) == 2
+
+
+# An output's own rounding, and what is left of the weights': 16-bit weights in two parts keep 16 bits
+# (bf16: 8 and 8, a step of 2^-16 of the weight) or 22 (fp16).
+@pytest.mark.parametrize("dt, rest", [("bf16", 2.0 ** -15), ("fp16", 2.0 ** -20), ("fp32", 0.0)])
+@pytest.mark.parametrize("case", [(2, 8, 2, 16, [600, 31]), (2, 8, 2, 16, [5000, 700]), (2, 8, 1, 24, [900, 7])], ids=str)
+def test_only_the_output_is_rounded(cuda, case, dt, rest):
+    B, H, Hkv, S, lengths = case
+    host, args = setup(B, H, Hkv, 128, S, lengths, dt, cuda)
+    out, _ = P.attention(*(np64(x) for x in host[:3]), host[3], lengths)
+    mean, _ = P.attention(np64(host[0]), np64(host[1]), np.abs(np64(host[2])), host[3], lengths)
+    # (and of fp32 sums of D + some 256 terms, 2^-24 each of the mean of |v|)
+    off = np.abs(np64(paged_attention(*args)) - out)
+    assert (off <= np.abs(out) * torch.finfo(DT[dt]).eps / 2 * (1 + 1e-6) + mean * (rest + 400 * 2.0 ** -24)
+            + torch.finfo(DT[dt]).tiny).all()
