@@ -16,15 +16,17 @@
 // Pages. Of sizes in whole 16 keys, a 16-key block lies in one page: a lane of the wave looks up
 // one block each of the next 32 steps, and a step takes its two blocks' pages out of the lanes as
 // scalars, so that no load waits for the table and addresses are a scalar base and a fixed
-// offset a lane. Of other sizes a lane looks up one key of the step, one step ahead, and
-// the lanes that load the key's parts fetch its row from there.
+// offset a lane. Of other sizes the blocks are of 8, 4, 2 or 1 keys, which divide the size, and
+// the lanes that load a key's parts fetch its block's page from the lane that holds it (a
+// look-up of 32 keys a step, one step ahead: 100 keys in pages of 24 6.8 us, of which 5.5 are left;
+// 16 sequences of up to 32768 in pages of 8 260, 243).
 // Rows past the length or without a page are not read: zeros take their place, scores -inf.
 //
 // Bound: HBM (K and V, read once); short caches: the latency of a start, a few steps and a merge.
 // Measured, D = 128: 16 sequences of up to 32768 keys, 32 heads on 8, bf16, pages of 16, 202 + 4.7 us
 // (contexts + join; 6.6 TB/s of K and V; with pages in order, or of 64, the same within 4 %); one of 128000
 // keys, 28 heads on 4, fp16, 45 + 5.2; one of 600, 10.4, alone. fp32, D = 64, pages of 24: 3 x 12 heads of up to
-// 5003 keys 19.1 + 4.2.
+// 5003 keys 18.5 + 4.2.
 #include "decode_common.h"
 #include "row_layout.h"
 
@@ -44,7 +46,8 @@ struct PagedArgs {
   const int32_t* table;
   int64_t table_ld;
   int32_t pages, size;
-  uint64_t magic;  // 2^64 / (size, or its blocks) rounded up; 0: by 1
+  int32_t shift;   // a block of 2^shift keys lies in one page
+  uint64_t magic;  // 2^64 / (blocks of a page) rounded up; 0: by 1
   int32_t group, H;
   int32_t direct;  // a workgroup a unit
   float c;         // scale * log2(e)
@@ -116,25 +119,19 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void paged_kernel(Paged
     const int end = min((len + STEP - 1) / STEP, 4 * (piece + pieces));
     const int begin = 4 * piece + w;
 
-    // Pages of this wave's steps. BLOCKS: lane 2 i + tt holds that of block tt of step
-    // from + 4 i. Else lane i holds the page, and the place in it, of key i % 32 of step `from`.
+    // Pages of this wave's steps: lane (i << per) + j holds that of block j of step from + 4 i, and the
+    // block's place in it.
+    const int shift = BLOCKS ? 4 : a.shift, per = 5 - shift;
+    const int kept = 64 >> per;  // steps that a look-up serves
     auto look_up = [&](int from, int& page, int& place) {
       page = -1;
       place = 0;
-      if constexpr (BLOCKS) {
-        const int block = 2 * (from + 4 * (lane >> 1)) + (lane & 1);
-        if (from + 4 * (lane >> 1) < end && 16 * block < len) {
-          const uint32_t col = divided(block, a.magic);
-          page = table[col];
-          place = 16 * (block - col * (a.size >> 4));
-        }
-      } else {
-        const int key = STEP * from + (lane & 31);
-        if (from < end && key < len) {
-          const uint32_t col = divided(key, a.magic);
-          page = table[col];
-          place = key - col * a.size;
-        }
+      const int step = from + 4 * (lane >> per);
+      const int block = (step << per) + (lane & ((1 << per) - 1));
+      if (step < end && block << shift < len) {
+        const uint32_t col = divided(block, a.magic);
+        page = table[col];
+        place = (block - col * (a.size >> shift)) << shift;
       }
       if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pages)) page = -1;
     };
@@ -179,20 +176,22 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void paged_kernel(Paged
       } else {
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
-          const int p = __shfl(page, 16 * tt + l16, 64), at = __shfl(place, 16 * tt + l16, 64);
+          const int key = 16 * tt + l16, from = (slot << per) + (key >> shift);
+          const int p = __shfl(page, from, 64), at = __shfl(place, from, 64) + (key & ((1 << shift) - 1));
           const char* kp = kb + p * a.ks[0] + at * a.ks[2];
 #pragma unroll
           for (int j = 0; j < NJ; ++j) {
             s.x.k[tt][j] = u32x4{0u, 0u, 0u, 0u};
-            if (p >= 0) s.x.k[tt][j] = ld_stream<u32x4>(kp + 64u * j + 16u * g);
+            if (p >= 0 && key < left) s.x.k[tt][j] = ld_stream<u32x4>(kp + 64u * j + 16u * g);
           }
         }
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
           const int key = 16 * (r >> 2) + 4 * g + (r & 3);
-          const int p = __shfl(page, key, 64), at = __shfl(place, key, 64);
+          const int from = (slot << per) + (key >> shift);
+          const int p = __shfl(page, from, 64), at = __shfl(place, from, 64) + (key & ((1 << shift) - 1));
           clear_v(s.x.v[r]);
-          if (p >= 0) {
+          if (p >= 0 && key < left) {
             s.in |= 1u << r;
             load_v(s.x.v[r], vb + p * a.vs[0] + at * a.vs[2] + SR::VB * l16);
           }
@@ -205,61 +204,35 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void paged_kernel(Paged
       rows.template step<true>(s.x, qr, c, some != 0, [&](int tt, int r) { return (s.in >> (4 * tt + r) & 1u) != 0; });
     };
 
-    if constexpr (BLOCKS) {
-      constexpr int KEPT = 32;  // steps that a look-up holds the pages of
-      int page, place;
-      look_up(begin, page, place);
-      if constexpr (ONE_SET) {
-        Step x;
-        int n = 0;
-        for (int step = begin; step < end; step += 4) {
-          load(step, n, page, place, x);
-          if (++n == KEPT) {
-            n = 0;
-            look_up(step + 4, page, place);
-          }
-          compute(x);
+    int page, place;
+    look_up(begin, page, place);
+    if constexpr (ONE_SET) {
+      Step x;
+      int n = 0;
+      for (int step = begin; step < end; step += 4) {
+        load(step, n, page, place, x);
+        if (++n == kept) {
+          n = 0;
+          look_up(step + 4, page, place);
         }
-      } else {
-        // Two register sets: a step's loads are in flight while the one before it is computed.
-        Step x, y;
-        int n = 1;
-        if (begin < end) load(begin, 0, page, place, x);
-        for (int step = begin; step < end; step += 8) {
-          if (step + 4 < end) load(step + 4, n, page, place, y);
-          if (++n == KEPT) {
-            n = 0;
-            look_up(step + 8, page, place);
-          }
-          compute(x);
-          if (step + 4 < end) {
-            if (step + 8 < end) load(step + 8, n, page, place, x);
-            ++n;
-            compute(y);
-          }
-        }
+        compute(x);
       }
     } else {
-      int page, place;
-      look_up(begin, page, place);
-      if constexpr (ONE_SET) {
-        Step x;
-        for (int step = begin; step < end; step += 4) {
-          load(step, 0, page, place, x);
-          look_up(step + 4, page, place);
-          compute(x);
-        }
-      } else {
-        Step x, y;
-        load(begin, 0, page, place, x);
-        look_up(begin + 4, page, place);
-        for (int step = begin; step < end; step += 8) {
-          load(step + 4, 0, page, place, y);
+      // Two register sets: a step's loads are in flight while the one before it is computed.
+      Step x, y;
+      int n = 1;
+      if (begin < end) load(begin, 0, page, place, x);
+      for (int step = begin; step < end; step += 8) {
+        if (step + 4 < end) load(step + 4, n, page, place, y);
+        if (++n == kept) {
+          n = 0;
           look_up(step + 8, page, place);
-          compute(x);
-          load(step + 8, 0, page, place, x);
-          look_up(step + 12, page, place);
-          if (step + 4 < end) compute(y);
+        }
+        compute(x);
+        if (step + 4 < end) {
+          if (step + 8 < end) load(step + 8, n, page, place, x);
+          ++n;
+          compute(y);
         }
       }
     }
@@ -565,7 +538,8 @@ extern "C" cab_status_t cab_paged_attn_fwd(
   a.pages = static_cast<int32_t>(pages);
   a.size = static_cast<int32_t>(page_size);
   const bool blocks = page_size % 16 == 0;
-  const uint64_t by = static_cast<uint64_t>(blocks ? page_size / 16 : page_size);
+  a.shift = std::min(__builtin_ctzll(static_cast<uint64_t>(page_size)), 4);
+  const uint64_t by = static_cast<uint64_t>(page_size >> a.shift);
   a.magic = by == 1 ? 0 : ~uint64_t{0} / by + 1;
   a.group = static_cast<int32_t>(H / H_kv);
   a.H = static_cast<int32_t>(H);

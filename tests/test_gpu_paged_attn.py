@@ -113,6 +113,29 @@ def test_pages_that_are_gone(cuda, S, dt, lengths):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("S", [1, 2, 4, 8, 24, 12, 6, 5])
+def test_pages_of_other_sizes(cuda, S, dt):
+    """Sizes whose blocks of one page are of 8, 4, 2 and 1 keys: whole and in parts, pages gone."""
+    for lengths in ([70, 33, 1], [1500, 7, 1111]):
+        host, args = setup(3, 4, 2, 128, S, lengths, dt, cuda, gone=0.2)
+        check(host, paged_attention(*args, return_lse=True), lengths, dt)
+
+
+@pytest.mark.parametrize("S, n", [(16, 18500), (32, 18500), (8, 9500), (4, 5000), (3, 4000)])
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_stretches_past_a_look_up(cuda, S, n, dt):
+    """64 sequences over a few pages in any order, so that a wave takes more steps than its lanes hold the
+    pages of (32 of them with whole blocks of 16 keys, 16 of 8, 8 of 4, 2 of odd sizes)."""
+    rng = np.random.default_rng(S)
+    pool, lengths = 61, [n - 37 * b for b in range(64)]
+    table = rng.integers(-3, pool, (64, -(-n // S)))
+    q, k, v = rand((64, 2, 1, 128), dt, 1, 1.5), rand((pool, 1, S, 128), dt, 2), rand((pool, 1, S, 128), dt, 3)
+    got = paged_attention(*(x.to(cuda) for x in (q, k, v)), torch.tensor(table, device=cuda),
+                          torch.tensor(lengths, device=cuda), return_lse=True)
+    check((q, k, v, table), got, lengths, dt)
+
+
 def test_nothing_to_see(cuda):
     """All pages gone, no columns, no pages, lengths of zero: 0 and -inf, for short and long tables."""
     for columns in (3, 200):
