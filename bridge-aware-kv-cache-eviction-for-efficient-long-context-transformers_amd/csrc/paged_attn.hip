@@ -23,10 +23,10 @@
 // Rows past the length or without a page are not read: zeros take their place, scores -inf.
 //
 // Bound: HBM (K and V, read once); short caches: the latency of a start, a few steps and a merge.
-// Measured, D = 128: 16 sequences of up to 32768 keys, 32 heads on 8, bf16, pages of 16, 202 + 4.7 us
+// Measured, D = 128: 16 sequences of up to 32768 keys, 32 heads on 8, bf16, pages of 16, 203 + 4.8 us
 // (contexts + join; 6.6 TB/s of K and V; with pages in order, or of 64, the same within 4 %); one of 128000
-// keys, 28 heads on 4, fp16, 45 + 5.2; one of 600, 10.4, alone. fp32, D = 64, pages of 24: 3 x 12 heads of up to
-// 5003 keys 18.5 + 4.2.
+// keys, 28 heads on 4, fp16, 45 + 5.4; one of 600, 10.6, alone. fp32, D = 64, pages of 24: 3 x 12 heads of up to
+// 5003 keys 17.9 + 4.3.
 #include "decode_common.h"
 #include "row_layout.h"
 
