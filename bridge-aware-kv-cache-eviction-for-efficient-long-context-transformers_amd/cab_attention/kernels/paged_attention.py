@@ -67,8 +67,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     dt = nat.dtype_code(q)
     page_table, M, ld = nat.table32(page_table, "page_table", B)
     lengths = nat.index32(lengths, "lengths", (B,))
+    rows = nat.aligned_rows(q)
     if out is None:
-        out = torch.empty_like(q)
+        out = torch.empty_like(rows)
     else:
         if out.shape != q.shape or out.dtype is not q.dtype:
             raise ValueError("out must match q's shape and dtype")
@@ -77,7 +78,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             raise RuntimeError("paged_attention: out is an inference tensor; write to it in "
                                "inference mode")
         nat.wrote(out)
-    q = nat.aligned_rows(q)
+    q = rows
     lse = q.new_empty((B, H, 1), dtype=torch.float32) if return_lse else None
     if scale is None:
         scale = 1.0 / math.sqrt(D)

@@ -136,6 +136,17 @@ def test_stretches_past_a_look_up(cuda, S, n, dt):
     check((q, k, v, table), got, lengths, dt)
 
 
+def test_queries_of_any_strides(cuda):
+    """Values apart from one another, rows off 16-byte boundaries, heads and sequences broadcast."""
+    _, (q, k, v, table, n) = setup(2, 8, 2, 64, 16, [90, 33], "bf16", cuda)
+    apart = q.permute(0, 3, 1, 2).contiguous().permute(0, 2, 3, 1)
+    off = torch.zeros(2, 8, 1, 67, dtype=q.dtype, device=cuda)[..., 3:].copy_(q)
+    for x in (apart, off, q[:1].expand_as(q), q[:, :1].expand_as(q)):
+        out, lse = paged_attention(x, k, v, table, n, return_lse=True)
+        a, b = paged_attention(x.contiguous(), k, v, table, n, return_lse=True)
+        assert torch.equal(out, a) and torch.equal(lse, b)
+
+
 def test_nothing_to_see(cuda):
     """All pages gone, no columns, no pages, lengths of zero: 0 and -inf, for short and long tables."""
     for columns in (3, 200):
