@@ -215,7 +215,8 @@ __device__ __forceinline__ f32x4 mfma4(float a, float b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-// Two weights' upper 16 bits (rounded towards 0), as fp32 again, and the least rest that is no zero.
+// Two weights' upper 16 bits (rounded towards 0), as fp32 again, and the least rest that is no zero
+// (times the largest V it is 4 in bf16, 2^-8 in fp16, whose weights go up to 2^15).
 template <bool BF16>
 __device__ __forceinline__ uint32_t cut2(float lo, float hi) {
   if constexpr (BF16)
@@ -231,7 +232,7 @@ template <bool BF16>
 __device__ __forceinline__ float high_half(uint32_t x) {
   return BF16 ? __uint_as_float(x & 0xffff0000u) : f16_to_f32(static_cast<uint16_t>(x >> 16));
 }
-template <bool BF16> constexpr float LEAST = BF16 ? 0x1p-120f : 0x1p-24f;
+template <bool BF16> constexpr float LEAST = BF16 ? 0x1p-126f : 0x1p-24f;
 
 // QT tiles of 16 query rows and what they have seen, of one wave (l16 = lane % 16: a
 // tile's row, g = lane / 16).

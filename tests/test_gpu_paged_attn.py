@@ -2,6 +2,8 @@
 pieces, 16-key blocks), of pages and of row tiles (16, 32 rows a K / V head), with pages that are
 not there, and with values that must not reach a row."""
 
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -346,6 +348,20 @@ def test_values_that_are_infinite(cuda, dt):
         v2[int(table[0, 1]), 0, 3, 7] = -float("inf")
         out = paged_attention(q, k, v2, table, m)
         assert torch.isneginf(out[0, :, 0, 7]).all() and int((~torch.isfinite(out)).sum()) == 2
+
+
+def test_values_near_the_types_end(cuda):
+    """The least weights times the largest values: 300 keys of weight 1 and of V = 0, and one whose weight is a
+    power of two (nothing is left of its upper bits) and whose V is 2^127."""
+    q = torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16, device=cuda)
+    k, v = (torch.zeros(20, 1, 16, 64, dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    q[..., 0], k[3, 0, 5, 0], v[3, 0, 5] = 1.0, -112.0, 2.0 ** 127
+    table = torch.arange(20, dtype=torch.int32, device=cuda)[None]
+    n = torch.tensor([301], dtype=torch.int32, device=cuda)
+    out = paged_attention(q, k, v, table, n, scale=math.log(2.0))
+    # (an output's half step; the weight's exponent, 112 in fp32, and its power, 2^-17; the rest's 2^-126 of 2^-112)
+    want = 2.0 ** (127 - 112) / 300
+    assert (out.double() / want - 1).abs().max() <= 2.0 ** -8 + 2.0 ** -14
 
 
 # An output's own rounding, and what is left of the weights': 16-bit weights in two parts keep 16 bits
