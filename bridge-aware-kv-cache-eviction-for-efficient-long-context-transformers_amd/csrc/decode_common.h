@@ -256,10 +256,12 @@ struct RowState {
     }
   }
 
-  // 32 keys; with `some`, of those alone for which in(tt, r) (key 16 tt + 4 g + r). BOTH: 16-bit weights
-  // as two operands, the upper bits cut off and the rest, so that only the output's rounding is
-  // left (the rest of a weight is never 0: times an infinite V that would be NaN).
-  template <bool BOTH = false, typename F>
+  // 32 keys; with `some`, of those alone for which in(tt, r) (key 16 tt + 4 g + r). WHOLE: 16-bit weights
+  // as operands of their upper bits and of what those leave, so that only the output's rounding is
+  // left: two in fp16 (22 bits, as far as they lie above 2^-24), three in bf16 (all 24. With two, 16 bits,
+  // one output in 300 rounded to its other neighbour; 1 - e^-t was off by 2^-17). None of a weight's operands is
+  // 0: times an infinite V that would be NaN.
+  template <bool WHOLE = false, typename F>
   __device__ __forceinline__ void step(const SR& x, const u32x4 (&qr)[QT][NJ], float c, bool some, F in) {
     f32x4 sc[QT][2];  // [qt][tt][r]: key 16 tt + 4 g + r, row 16 qt + l16
 #pragma unroll
@@ -291,7 +293,7 @@ struct RowState {
           for (int r = 0; r < 4; ++r)
             if (!in(tt, r)) sc[qt][tt][r] = -INFINITY;
     }
-    u32x4 pb[QT], rest[QT];
+    u32x4 pb[QT], rest[QT], last[QT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       const float m0 = fmaxf(fmaxf(sc[qt][0][0], sc[qt][0][1]), fmaxf(sc[qt][0][2], sc[qt][0][3]));
@@ -315,17 +317,24 @@ struct RowState {
           sc[qt][tt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qt][tt][r], c, -level[qt]));
       const f32x4 s2 = sc[qt][0] + sc[qt][1];
       l[qt] += (s2[0] + s2[1]) + (s2[2] + s2[3]);
-      if constexpr (!F32 && BOTH) {
+      if constexpr (!F32 && WHOLE) {
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
           for (int r = 0; r < 4; r += 2) {
-            const float a = sc[qt][tt][r], b = sc[qt][tt][r + 1];
-            const uint32_t cut = cut2<BF16>(a, b);
-            pb[qt][2 * tt + r / 2] = cut;
-            rest[qt][2 * tt + r / 2] =
-                pack2<BF16>(fmaxf(a - low_half<BF16>(cut), fminf(a, LEAST<BF16>)),
-                            fmaxf(b - high_half<BF16>(cut), fminf(b, LEAST<BF16>)));
+            const int at = 2 * tt + r / 2;
+            float a = sc[qt][tt][r], b = sc[qt][tt][r + 1];
+            const float a0 = fminf(a, LEAST<BF16>), b0 = fminf(b, LEAST<BF16>);
+            pb[qt][at] = cut2<BF16>(a, b);
+            a = fmaxf(a - low_half<BF16>(pb[qt][at]), a0);
+            b = fmaxf(b - high_half<BF16>(pb[qt][at]), b0);
+            if constexpr (BF16) {
+              rest[qt][at] = cut2<true>(a, b);
+              last[qt][at] = cut2<true>(fmaxf(a - low_half<true>(rest[qt][at]), a0),
+                                        fmaxf(b - high_half<true>(rest[qt][at]), b0));
+            } else {
+              rest[qt][at] = pack2<false>(a, b);
+            }
           }
       } else if constexpr (!F32) {
         pb[qt] = u32x4{pack2<BF16>(sc[qt][0][0], sc[qt][0][1]), pack2<BF16>(sc[qt][0][2], sc[qt][0][3]),
@@ -353,7 +362,8 @@ struct RowState {
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
           o[qt][dt] = mfma16<BF16>(vo, pb[qt], o[qt][dt]);
-          if constexpr (BOTH) o[qt][dt] = mfma16<BF16>(vo, rest[qt], o[qt][dt]);
+          if constexpr (WHOLE) o[qt][dt] = mfma16<BF16>(vo, rest[qt], o[qt][dt]);
+          if constexpr (WHOLE && BF16) o[qt][dt] = mfma16<BF16>(vo, last[qt], o[qt][dt]);
         }
       }
     }

@@ -5,9 +5,9 @@
 //  1. The contexts of all units, cut into pieces of 128 keys, make one list of which each
 //     workgroup takes an equal stretch. Every wave walks its own 32-key steps, K and V straight
 //     from the pages into matrix operands (S^T = K Q^T, online softmax in the log2 domain,
-//     O^T += V^T P^T; maxima, sums and O in fp32; P as two 16-bit operands, its upper bits and
-//     the rest, so that bf16 outputs are as near as their own rounding, 1.7e-3 in place of
-//     1.9e-3 in norm; the second product costs 0.3 us of 10 at 600 keys and nothing that shows at
+//     O^T += V^T P^T; maxima, sums and O in fp32; P as 16-bit operands of its upper bits and of what
+//     those leave, two in fp16 and three in bf16, so that only the output is rounded; each further
+//     product costs some 0.4 us of 10 at 600 keys, 1 % where pages are of 8 and nothing that shows at other
 //     long contexts; fp32 on the fp32 matrix instructions). A part that is all of a unit
 //     is finished there; of the others one partial (level, row sum, O) is left per row.
 //  2. join_kernel, one wave per row, merges the partials. Where one workgroup a unit does

@@ -571,8 +571,8 @@ cab_status_t cab_verify_drafts(const void* logits, const void* draft_logits, cab
  * all -inf) have NaN for both; finite scores below -1e30 / scale weigh nothing. What is behind a length or in no page of the sequence is
  * not read. q, out: [B, H, 1, D], out is q itself or shares no memory with the
  * inputs; D 64 or 128; H % H_kv == 0; 16-byte aligned rows; place strides
- * in [0, 2^25] bytes. bf16, fp16 (P as two 16-bit operands, its upper bits and the rest; sums in fp32) or
- * fp32. workspace: cab_paged_attn_workspace_bytes() bytes (may be 0), 16-byte aligned,
+ * in [0, 2^25] bytes. bf16, fp16 (P as 16-bit operands of its upper bits and of what those leave, three in bf16: all 24 bits,
+ * two in fp16: 22; sums in fp32) or fp32. workspace: cab_paged_attn_workspace_bytes() bytes (may be 0), 16-byte aligned,
  * overwritten.
  *
  * cab_adjust_logits prepares logits [B, T, V] (strides {b, t}, last dim
