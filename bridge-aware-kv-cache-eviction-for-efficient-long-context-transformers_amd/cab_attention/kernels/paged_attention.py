@@ -57,7 +57,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     Rows behind a length, and pages that are not the sequence's, are not read. A sequence that
     sees no row has output 0 and log-sum-exp -inf. One whose scores have no softmax (a NaN or
-    +inf among them, or all -inf) has NaN for both. Scores, weights and sums are held in fp32 (weights for
+    +inf among them, or all -inf; ``q k^T`` past fp32's range is infinite) has NaN for both. Scores, weights and sums are held in fp32 (weights for
     the product with 16-bit values: 24 bits with bf16, 22 with fp16); the output is rounded once.
     Returns the output ``[B, H, 1, D]``, with ``return_lse`` also the fp32 natural-log
     log-sum-exp ``[B, H, 1]``.

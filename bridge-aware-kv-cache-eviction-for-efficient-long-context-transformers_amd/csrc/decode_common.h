@@ -233,35 +233,42 @@ __device__ __forceinline__ float high_half(uint32_t x) {
   return BF16 ? __uint_as_float(x & 0xffff0000u) : f16_to_f32(static_cast<uint16_t>(x >> 16));
 }
 template <bool BF16> constexpr float LEAST = BF16 ? 0x1p-126f : 0x1p-24f;
+// What whole weights are multiplied by as operands (in fp16 they keep 11 bits to 1.9e-9 so, not to 6e-5).
+template <bool BF16> constexpr float WEIGHT = BF16 ? 1.f : 0x1p15f;
+
+// The maximum of no scores. WHOLE: no finite score lies below it.
+template <bool WHOLE> constexpr float NO_SCORE = WHOLE ? -0x1.fffffep127f : M_EMPTY;
 
 // QT tiles of 16 query rows and what they have seen, of one wave (l16 = lane % 16: a
-// tile's row, g = lane / 16).
-template <cab_dtype_t DT, int HD, int QT>
+// tile's row, g = lane / 16). WHOLE: weights are 2^((s - m) c) for the maximum m, with the difference
+// formed first, whatever the scores' size, where else they are relative to a rounded level, which for scores
+// of 2^31 and more can be more than 2^128 away from them; and the second product takes them in all their digits.
+template <cab_dtype_t DT, int HD, int QT, bool WHOLE = false>
 struct RowState {
   static constexpr bool F32 = DT == CAB_F32, BF16 = DT == CAB_BF16;
   static constexpr int NDT = HD / 16;
   using SR = StepRegs<DT, HD>;
   static constexpr int NJ = SR::NJ;
   f32x4 o[QT][NDT];
-  float l[QT], m[QT], level[QT];  // l: of this lane's keys alone
+  float l[QT], m[QT], level[WHOLE ? 1 : QT];  // l: of this lane's keys alone
 
   __device__ __forceinline__ void clear(float c) {
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       l[qt] = 0.f;
-      m[qt] = M_EMPTY;
-      level[qt] = level_of<DT>(M_EMPTY, c);
+      m[qt] = NO_SCORE<WHOLE>;
+      if constexpr (!WHOLE) level[qt] = level_of<DT>(M_EMPTY, c);
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt) o[qt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
   }
 
   // 32 keys; with `some`, of those alone for which in(tt, r) (key 16 tt + 4 g + r). WHOLE: 16-bit weights
-  // as operands of their upper bits and of what those leave, so that only the output's rounding is
+  // (in fp16 times 2^15) as operands of their upper bits and of what those leave, so that only the output's rounding is
   // left: two in fp16 (22 bits, as far as they lie above 2^-24), three in bf16 (all 24. With two, 16 bits,
   // one output in 300 rounded to its other neighbour; 1 - e^-t was off by 2^-17). None of a weight's operands is
   // 0: times an infinite V that would be NaN.
-  template <bool WHOLE = false, typename F>
+  template <typename F>
   __device__ __forceinline__ void step(const SR& x, const u32x4 (&qr)[QT][NJ], float c, bool some, F in) {
     f32x4 sc[QT][2];  // [qt][tt][r]: key 16 tt + 4 g + r, row 16 qt + l16
 #pragma unroll
@@ -302,19 +309,20 @@ struct RowState {
       colmax2(mx, mdup);
       if (__builtin_amdgcn_ballot_w64(mx > m[qt]) != 0) {
         const float mn = fmaxf(mx, m[qt]);
-        const float upto = level_of<DT>(mn, c);
-        const float alpha = relevel<DT>(m[qt], level[qt], mn, upto, c);
+        const float upto = WHOLE ? 0.f : level_of<DT>(mn, c);
+        const float alpha = WHOLE ? __builtin_amdgcn_exp2f((m[qt] - mn) * c) : relevel<DT>(m[qt], level[qt], mn, upto, c);
         l[qt] *= alpha;
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) o[qt][dt] *= alpha;
         m[qt] = mn;
-        level[qt] = upto;
+        if constexpr (!WHOLE) level[qt] = upto;
       }
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          sc[qt][tt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qt][tt][r], c, -level[qt]));
+          sc[qt][tt][r] = __builtin_amdgcn_exp2f(WHOLE ? (sc[qt][tt][r] - m[qt]) * c
+                                                       : __builtin_fmaf(sc[qt][tt][r], c, -level[qt]));
       const f32x4 s2 = sc[qt][0] + sc[qt][1];
       l[qt] += (s2[0] + s2[1]) + (s2[2] + s2[3]);
       if constexpr (!F32 && WHOLE) {
@@ -323,7 +331,7 @@ struct RowState {
 #pragma unroll
           for (int r = 0; r < 4; r += 2) {
             const int at = 2 * tt + r / 2;
-            float a = sc[qt][tt][r], b = sc[qt][tt][r + 1];
+            float a = sc[qt][tt][r] * WEIGHT<BF16>, b = sc[qt][tt][r + 1] * WEIGHT<BF16>;
             const float a0 = fminf(a, LEAST<BF16>), b0 = fminf(b, LEAST<BF16>);
             pb[qt][at] = cut2<BF16>(a, b);
             a = fmaxf(a - low_half<BF16>(pb[qt][at]), a0);
@@ -372,8 +380,8 @@ struct RowState {
 
 // Merge of four waves' rows: common maximum, then the scaled O^T and sums in wave order.
 // value(qt, e, y) gets values e = 64 dt + lane of a tile's O^T, sums(qt, level, sum) a row's level
-// and sum (threads 0 .. 15: the row). sum() is there for both.
-template <cab_dtype_t DT, int HD, int QT>
+// (WHOLE: its maximum) and sum (threads 0 .. 15: the row). sum() is there for both.
+template <cab_dtype_t DT, int HD, int QT, bool WHOLE = false>
 struct RowMerge {
   static constexpr int NDT = HD / 16;
   f32x4 o[4][NDT * 64];  // one query tile's O^T per wave
@@ -384,7 +392,7 @@ struct RowMerge {
   }
 
   template <typename V, typename S>
-  __device__ __forceinline__ void run(RowState<DT, HD, QT>& x, int w, int lane, float c, V value, S sums) {
+  __device__ __forceinline__ void run(RowState<DT, HD, QT, WHOLE>& x, int w, int lane, float c, V value, S sums) {
     const int l16 = lane & 15, g = lane >> 4;
     __syncthreads();  // (the last part's merge has been read)
 #pragma unroll
@@ -397,11 +405,13 @@ struct RowMerge {
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       const float mm = fmaxf(fmaxf(m[0][qt][l16], m[1][qt][l16]), fmaxf(m[2][qt][l16], m[3][qt][l16]));
-      const float upto = level_of<DT>(mm, c);
-      const float f = relevel<DT>(x.m[qt], x.level[qt], mm, upto, c);
+      const float upto = WHOLE ? mm : level_of<DT>(mm, c);
+      const float f = WHOLE ? __builtin_amdgcn_exp2f((x.m[qt] - mm) * c)
+                            : relevel<DT>(x.m[qt], x.level[qt], mm, upto, c);
+      const float fo = WHOLE && DT == CAB_F16 ? f * (1.f / WEIGHT<false>) : f;
       if (g == 0) l[w][qt][l16] = x.l[qt] * f;
 #pragma unroll
-      for (int dt = 0; dt < NDT; ++dt) o[w][dt * 64 + lane] = x.o[qt][dt] * f;
+      for (int dt = 0; dt < NDT; ++dt) o[w][dt * 64 + lane] = x.o[qt][dt] * fo;
       __syncthreads();
       for (int e = threadIdx.x; e < NDT * 64; e += 256)
         value(qt, e, (o[0][e] + o[1][e]) + (o[2][e] + o[3][e]));

@@ -4,12 +4,12 @@
 //
 //  1. The contexts of all units, cut into pieces of 128 keys, make one list of which each
 //     workgroup takes an equal stretch. Every wave walks its own 32-key steps, K and V straight
-//     from the pages into matrix operands (S^T = K Q^T, online softmax in the log2 domain,
+//     from the pages into matrix operands (S^T = K Q^T, online softmax, weights 2^((s - m) c),
 //     O^T += V^T P^T; maxima, sums and O in fp32; P as 16-bit operands of its upper bits and of what
 //     those leave, two in fp16 and three in bf16, so that only the output is rounded; each further
 //     product costs some 0.4 us of 10 at 600 keys, 1 % where pages are of 8 and nothing that shows at other
 //     long contexts; fp32 on the fp32 matrix instructions). A part that is all of a unit
-//     is finished there; of the others one partial (level, row sum, O) is left per row.
+//     is finished there; of the others one partial (maximum, row sum, O) is left per row.
 //  2. join_kernel, one wave per row, merges the partials. Where one workgroup a unit does
 //     (paged_plan), there are none and it is not launched.
 //
@@ -56,7 +56,7 @@ struct PagedArgs {
   float* lse;     // [B, H], may be null
   // Partials; workgroup x's of unit u is number x + u.
   float* po;  // [number][group][D]
-  float* pm;  // [number][group] level of the maximum score
+  float* pm;  // [number][group] the maximum score
   float* pl;  // [number][group] row sums, NO_KEY where none was seen
 };
 
@@ -68,10 +68,10 @@ __device__ __forceinline__ uint32_t divided(uint32_t x, uint64_t magic) {
 // The bits of a row's log-sum-exp: -inf with no key seen; NaN where keys are seen but have no
 // softmax (a score of NaN or +inf, or all -inf: the sum is NaN or 0). Bits, tested and stored as
 // such, because this file is compiled with -fno-honor-nans.
-__device__ __forceinline__ uint32_t lse_bits(bool any, float level, float sum) {
+__device__ __forceinline__ uint32_t lse_bits(bool any, float m, float sum, float c) {
   int32_t bits = __builtin_bit_cast(int32_t, sum);
   asm("" : "+v"(bits));  // (or the test is made one of floats)
-  const float x = (level + __log2f(sum)) * 0.69314718055994531f;
+  const float x = __builtin_fmaf(m, c, __log2f(sum)) * 0.69314718055994531f;
   const uint32_t y = bits > 0 && bits <= 0x7f800000 ? __builtin_bit_cast(uint32_t, x) : 0x7fc00000u;
   return any ? y : 0xff800000u;
 }
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void paged_kernel(Paged
   // (Two register sets spill with 32 rows of 128 in 16 bits, and gain nothing in fp32 but for 16 rows
   // of 64: 8 x 4 heads of 5000 keys 28.0 -> 26.2 us.)
   constexpr bool ONE_SET = F32 ? QT * HD > 64 : QT * HD > 128;
-  __shared__ RowMerge<DT, HD, QT> merge;
+  __shared__ RowMerge<DT, HD, QT, true> merge;
   __shared__ int seen_by[4];
 
   const int row0 = blockIdx.y * (16 * QT);
@@ -112,7 +112,7 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void paged_kernel(Paged
         if (r < a.group) qr[qt][j] = *reinterpret_cast<const u32x4*>(qp + 64 * j + 16 * g);
       }
     }
-    RowState<DT, HD, QT> rows;
+    RowState<DT, HD, QT, true> rows;
     rows.clear(c);
     int seen = 0;
 
@@ -201,7 +201,7 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void paged_kernel(Paged
     auto compute = [&](const Step& s) __attribute__((always_inline)) {
       const uint64_t some = __builtin_amdgcn_ballot_w64(s.in != 255u);
       seen |= static_cast<int>(__builtin_amdgcn_ballot_w64(s.in != 0) != 0);
-      rows.template step<true>(s.x, qr, c, some != 0, [&](int tt, int r) { return (s.in >> (4 * tt + r) & 1u) != 0; });
+      rows.step(s.x, qr, c, some != 0, [&](int tt, int r) { return (s.in >> (4 * tt + r) & 1u) != 0; });
     };
 
     int page, place;
@@ -262,16 +262,16 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void paged_kernel(Paged
             }
           }
         },
-        [&](int qt, float level, float sum) {
+        [&](int qt, float m, float sum) {
           const int row = row0 + 16 * qt + static_cast<int>(threadIdx.x);
           if (row >= a.group) return;
           const bool any = (seen_by[0] | seen_by[1] | seen_by[2] | seen_by[3]) != 0;
           if (!whole) {
-            a.pm[part * a.group + row] = any ? level : -INFINITY;
+            a.pm[part * a.group + row] = any ? m : -INFINITY;
             a.pl[part * a.group + row] = any ? sum : NO_KEY;
           } else if (a.lse) {
             const int64_t at = static_cast<int64_t>(b) * a.H + static_cast<int64_t>(hk) * a.group + row;
-            reinterpret_cast<uint32_t*>(a.lse)[at] = lse_bits(any, level, sum);
+            reinterpret_cast<uint32_t*>(a.lse)[at] = lse_bits(any, m, sum, c);
           }
         });
     __syncthreads();  // (seen_by and the sums have been read)
@@ -314,7 +314,7 @@ __global__ __launch_bounds__(256) void join_kernel(PagedArgs a) {
   const int parts = pieces ? (start + pieces - 1) / cut.per - first + 1 : 0;
   if (parts == 1) return;  // (finished by the workgroup that had all of it)
   const int64_t row = (static_cast<int64_t>(first) + b * a.Hkv + hk) * a.group + (h - hk * a.group);
-  // (whether a key was seen goes by bits: levels may be NaN, and comparisons of those say anything)
+  // (whether a key was seen goes by bits: sums may be NaN, and comparisons of those say anything)
   float m = -INFINITY;
   bool some = false;
   for (int x = lane; x < parts; x += 64) {
@@ -330,7 +330,7 @@ __global__ __launch_bounds__(256) void join_kernel(PagedArgs a) {
 #pragma unroll 4
     for (int x = grp; x < parts; x += G) {
       const int64_t y = row + static_cast<int64_t>(x) * a.group;
-      const float f = __builtin_amdgcn_exp2f(a.pm[y] - m);
+      const float f = __builtin_amdgcn_exp2f((a.pm[y] - m) * a.c);
       l += a.pl[y] * f;
       const f32x4* po = reinterpret_cast<const f32x4*>(a.po + y * HD) + 2 * at;
       const f32x4 y0 = po[0], y1 = po[1];
@@ -377,7 +377,7 @@ __global__ __launch_bounds__(256) void join_kernel(PagedArgs a) {
     *reinterpret_cast<u32x4*>(op) = u32x4{pack2<BF16>(o[0], o[1]), pack2<BF16>(o[2], o[3]),
                                           pack2<BF16>(o[4], o[5]), pack2<BF16>(o[6], o[7])};
   }
-  if (at == 0 && a.lse) reinterpret_cast<uint32_t*>(a.lse)[id] = lse_bits(any, m, l);
+  if (at == 0 && a.lse) reinterpret_cast<uint32_t*>(a.lse)[id] = lse_bits(any, m, l, a.c);
 }
 
 struct PagedPlan {
