@@ -215,8 +215,7 @@ __device__ __forceinline__ f32x4 mfma4(float a, float b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-// Two weights' upper 16 bits (rounded towards 0), as fp32 again, and the least rest that is no zero
-// (times the largest V it is 4 in bf16, 2^-8 in fp16, whose weights go up to 2^15).
+// Two weights' upper 16 bits (rounded towards 0), as fp32 again, and the least operand that is no zero.
 template <bool BF16>
 __device__ __forceinline__ uint32_t cut2(float lo, float hi) {
   if constexpr (BF16)
@@ -263,12 +262,28 @@ struct RowState {
     }
   }
 
+  // Whether a sum of this wave's is NaN (or some are infinities of both signs). By its bits: comparisons
+  // may not tell.
+  __device__ __forceinline__ bool not_a_number() const {
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) y += o[qt][dt];
+    const float t = (y[0] + y[1]) + (y[2] + y[3]);
+    uint32_t bits = __float_as_uint(t);
+    asm("" : "+v"(bits));
+    return __builtin_amdgcn_ballot_w64((bits & 0x7fffffffu) > 0x7f800000u) != 0;
+  }
+
   // 32 keys; with `some`, of those alone for which in(tt, r) (key 16 tt + 4 g + r). WHOLE: 16-bit weights
-  // (in fp16 times 2^15) as operands of their upper bits and of what those leave, so that only the output's rounding is
-  // left: two in fp16 (22 bits, as far as they lie above 2^-24), three in bf16 (all 24. With two, 16 bits,
-  // one output in 300 rounded to its other neighbour; 1 - e^-t was off by 2^-17). None of a weight's operands is
-  // 0: times an infinite V that would be NaN.
-  template <typename F>
+  // (in fp16 times 2^15) as operands of their upper bits and of what those leave, so that only the
+  // output's rounding is left: two in fp16 (22 bits, as far as they lie above 2^-24), three in bf16 (all 24. With
+  // two, 16 bits, one output in 300 rounded to its other neighbour; 1 - e^-t was off by 2^-17). An operand of 0
+  // times an infinite V is NaN, so weights that are not 0 have none that is: in bf16 they are 2^-126 at the
+  // least. fp16's least is 2^-24, which many keys would add up: there it is with NONE_0 alone, for a second walk
+  // over rows whose sums became NaN.
+  template <bool NONE_0 = false, typename F>
   __device__ __forceinline__ void step(const SR& x, const u32x4 (&qr)[QT][NJ], float c, bool some, F in) {
     f32x4 sc[QT][2];  // [qt][tt][r]: key 16 tt + 4 g + r, row 16 qt + l16
 #pragma unroll
@@ -331,17 +346,28 @@ struct RowState {
 #pragma unroll
           for (int r = 0; r < 4; r += 2) {
             const int at = 2 * tt + r / 2;
-            float a = sc[qt][tt][r] * WEIGHT<BF16>, b = sc[qt][tt][r + 1] * WEIGHT<BF16>;
-            const float a0 = fminf(a, LEAST<BF16>), b0 = fminf(b, LEAST<BF16>);
-            pb[qt][at] = cut2<BF16>(a, b);
-            a = fmaxf(a - low_half<BF16>(pb[qt][at]), a0);
-            b = fmaxf(b - high_half<BF16>(pb[qt][at]), b0);
+            float x[2] = {sc[qt][tt][r] * WEIGHT<BF16>, sc[qt][tt][r + 1] * WEIGHT<BF16>};
+            const float least[2] = {x[0] > 0.f ? LEAST<BF16> : x[0], x[1] > 0.f ? LEAST<BF16> : x[1]};
+            auto keep = [&]() {
+              if constexpr (NONE_0 || BF16) {
+                x[0] = fmaxf(x[0], least[0]);
+                x[1] = fmaxf(x[1], least[1]);
+              }
+            };
+            auto less = [&](uint32_t cut) {
+              x[0] -= low_half<BF16>(cut);
+              x[1] -= high_half<BF16>(cut);
+              keep();
+            };
+            if constexpr (!BF16) keep();
+            pb[qt][at] = cut2<BF16>(x[0], x[1]);
+            less(pb[qt][at]);
             if constexpr (BF16) {
-              rest[qt][at] = cut2<true>(a, b);
-              last[qt][at] = cut2<true>(fmaxf(a - low_half<true>(rest[qt][at]), a0),
-                                        fmaxf(b - high_half<true>(rest[qt][at]), b0));
+              rest[qt][at] = cut2<true>(x[0], x[1]);
+              less(rest[qt][at]);
+              last[qt][at] = cut2<true>(x[0], x[1]);
             } else {
-              rest[qt][at] = pack2<false>(a, b);
+              rest[qt][at] = pack2<false>(x[0], x[1]);
             }
           }
       } else if constexpr (!F32) {

@@ -113,7 +113,6 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void paged_kernel(Paged
       }
     }
     RowState<DT, HD, QT, true> rows;
-    rows.clear(c);
     int seen = 0;
 
     const int end = min((len + STEP - 1) / STEP, 4 * (piece + pieces));
@@ -198,43 +197,52 @@ __global__ __launch_bounds__(256, DT == CAB_F32 ? 1 : 2) void paged_kernel(Paged
         }
       }
     };
-    auto compute = [&](const Step& s) __attribute__((always_inline)) {
+    auto compute = [&](const Step& s, auto none_0) __attribute__((always_inline)) {
       const uint64_t some = __builtin_amdgcn_ballot_w64(s.in != 255u);
       seen |= static_cast<int>(__builtin_amdgcn_ballot_w64(s.in != 0) != 0);
-      rows.step(s.x, qr, c, some != 0, [&](int tt, int r) { return (s.in >> (4 * tt + r) & 1u) != 0; });
+      rows.template step<decltype(none_0)::value>(
+          s.x, qr, c, some != 0, [&](int tt, int r) { return (s.in >> (4 * tt + r) & 1u) != 0; });
     };
 
-    int page, place;
-    look_up(begin, page, place);
-    if constexpr (ONE_SET) {
-      Step x;
-      int n = 0;
-      for (int step = begin; step < end; step += 4) {
-        load(step, n, page, place, x);
-        if (++n == kept) {
-          n = 0;
-          look_up(step + 4, page, place);
+    auto walk = [&](auto none_0) __attribute__((always_inline)) {
+      rows.clear(c);
+      seen = 0;
+      int page, place;
+      look_up(begin, page, place);
+      if constexpr (ONE_SET || decltype(none_0)::value) {
+        Step x;
+        int n = 0;
+        for (int step = begin; step < end; step += 4) {
+          load(step, n, page, place, x);
+          if (++n == kept) {
+            n = 0;
+            look_up(step + 4, page, place);
+          }
+          compute(x, none_0);
         }
-        compute(x);
+      } else {
+        // Two register sets: a step's loads are in flight while the one before it is computed.
+        Step x, y;
+        int n = 1;
+        if (begin < end) load(begin, 0, page, place, x);
+        for (int step = begin; step < end; step += 8) {
+          if (step + 4 < end) load(step + 4, n, page, place, y);
+          if (++n == kept) {
+            n = 0;
+            look_up(step + 8, page, place);
+          }
+          compute(x, none_0);
+          if (step + 4 < end) {
+            if (step + 8 < end) load(step + 8, n, page, place, x);
+            ++n;
+            compute(y, none_0);
+          }
+        }
       }
-    } else {
-      // Two register sets: a step's loads are in flight while the one before it is computed.
-      Step x, y;
-      int n = 1;
-      if (begin < end) load(begin, 0, page, place, x);
-      for (int step = begin; step < end; step += 8) {
-        if (step + 4 < end) load(step + 4, n, page, place, y);
-        if (++n == kept) {
-          n = 0;
-          look_up(step + 8, page, place);
-        }
-        compute(x);
-        if (step + 4 < end) {
-          if (step + 8 < end) load(step + 8, n, page, place, x);
-          ++n;
-          compute(y);
-        }
-      }
+    };
+    walk(std::false_type{});
+    if constexpr (DT == CAB_F16) {  // (an infinite V times an operand of 0)
+      if (__builtin_expect(rows.not_a_number(), 0)) walk(std::true_type{});
     }
 
     if (lane == 0) seen_by[w] = seen;  // (read behind the merge's barriers, written before its first)
