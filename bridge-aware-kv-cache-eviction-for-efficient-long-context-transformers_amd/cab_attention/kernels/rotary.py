@@ -157,7 +157,7 @@ class Rotary(torch.nn.Module):
     into belong to that pass's stream, whatever the operator.
 
     The frequencies are a buffer that goes to the module's device and is no part of its
-    state dict.
+    state dict; they are formed anew where it is (``to_empty`` after a start on the meta device).
     """
 
     def __init__(self, head_dim: int, rotary_dim: Optional[int] = None, base: float = 10000.0,
@@ -174,8 +174,26 @@ class Rotary(torch.nn.Module):
         self.interleaved = bool(interleaved)
         self.scaling = dict(scaling) if scaling else None
         self.frequencies, self.amplitude = _frequencies(self.rotary_dim, self.base, self.scaling)
-        self.register_buffer("turns", torch.tensor([_turns(x) for x in self.frequencies], dtype=torch.int64),
-                             persistent=False)
+        self.register_buffer("turns", self._formed(), persistent=False)
+
+    def _formed(self) -> torch.Tensor:
+        return torch.tensor([_turns(x) for x in self.frequencies], dtype=torch.int64)
+
+    def reset_parameters(self) -> None:
+        """Forms the buffer's values anew, where it lies."""
+        with torch.device("cpu"):
+            turns = self._formed()
+        with torch.no_grad():
+            self.turns.copy_(turns)
+
+    def _apply(self, fn, *args, **kwargs):
+        """(a buffer that is made anew, by ``to_empty`` say, would hold whatever the memory did: no state dict has
+        its values)"""
+        before = self.turns
+        super()._apply(fn, *args, **kwargs)
+        if self.turns is not before and not self.turns.is_meta and self.turns.dtype is torch.int64:
+            self.reset_parameters()
+        return self
 
     def extra_repr(self) -> str:
         return (f"head_dim={self.head_dim}, rotary_dim={self.rotary_dim}, base={self.base}, "
