@@ -109,7 +109,10 @@ class _Turned(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         # (changed in place before the backward pass: an error, not other angles)
         ctx.save_for_backward(turns, positions)
-        return tuple(_turn(plan, turns, positions, inverse, [x.detach() for x in tensors]))
+        outs = tuple(_turn(plan, turns, positions, inverse, [x.detach() for x in tensors]))
+        # (a frozen key's turned form is frozen too)
+        ctx.mark_non_differentiable(*[y for y, need in zip(outs, ctx.needs_input_grad[4:]) if not need])
+        return outs
 
     @staticmethod
     def backward(ctx, *grads):
