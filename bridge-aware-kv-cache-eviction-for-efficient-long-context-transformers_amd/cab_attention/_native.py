@@ -232,6 +232,13 @@ def aligned_rows(t: torch.Tensor) -> torch.Tensor:
     return t if rows_aligned(t) else t.clone()
 
 
+def empty_rows_like(t: torch.Tensor) -> torch.Tensor:
+    """``torch.empty_like``, but contiguous where that would lay values of a row apart (rows that
+    overlap, at a stride of one value, make it do so)."""
+    out = torch.empty_like(t)
+    return out if out.stride(-1) == 1 else torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
 # Looked up once: a decode step asks addressable() per layer.
 _is_compiling = torch.compiler.is_compiling

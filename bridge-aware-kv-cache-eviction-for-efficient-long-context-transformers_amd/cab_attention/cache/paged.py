@@ -95,7 +95,7 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
             raise TypeError("q and k dtypes differ")
         if q.stride(3) != 1:
             q = q.contiguous()
-        H, out = q.shape[1], torch.empty_like(q)
+        H, out = q.shape[1], nat.empty_rows_like(q)
         q_strides, out_strides = nat.stride_array(q.stride()), nat.stride_array(out.stride())
     if k.stride(3) != 1:
         k = k.contiguous()

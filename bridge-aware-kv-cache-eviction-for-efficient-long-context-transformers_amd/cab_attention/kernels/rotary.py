@@ -83,7 +83,7 @@ def _plain(fn: str, *tensors: torch.Tensor) -> None:
 def _turn(plan: tuple, turns: torch.Tensor, positions, inverse: bool, tensors):
     """plan: (rotary_dim, interleaved, amplitude)."""
     tensors = [x if x.stride(3) == 1 else x.contiguous() for x in tensors]
-    outs = [torch.empty_like(x) for x in tensors]
+    outs = [nat.empty_rows_like(x) for x in tensors]
     n = len(tensors)
     B, _, N, D = tensors[0].shape
     array = ctypes.c_void_p * n
@@ -150,7 +150,7 @@ class Rotary(torch.nn.Module):
             those below ``low`` (1) go by ``1 / factor``, interpolated over the turns between.
 
     ``rotary(q, k, positions)`` turns two tensors ``[B, H, N, D]`` (heads of their own; bf16,
-    fp16 or fp32; any strides) in one launch and returns them in the same layout;
+    fp16 or fp32; any strides) in one launch and returns them in the same layout (contiguous where rows overlap);
     ``rotary(q, positions=..)`` one. positions: int32 ``[N]`` or ``[B, N]`` on the device (int64 is
     converted), any value; ``None``: 0 .. N - 1. Angles are within 2e-9 radians for
     every position (64-bit fixed point, no table); the products are formed in fp32 and rounded once. ``B * N < 2**24``.

@@ -1,0 +1,35 @@
+"""Rotary, append_paged and paged_attention on layouts at the edge of "any strides": windows that slide over one
+row, rows of one value, dims of one place with strides of no meaning."""
+
+import pytest
+import torch
+
+from cab_attention.cache import append_paged
+from cab_attention.kernels import Rotary
+
+pytestmark = pytest.mark.gpu
+
+
+def rand(shape, seed, dt=torch.bfloat16):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(shape, generator=g).to(dt)
+
+
+def test_windows_that_slide_over_a_row(cuda):
+    """Rows at a stride of one value, fewer than a head's values: an output cannot be laid out like them."""
+    rot = Rotary(64).to(cuda)
+    x = rand(70, 1).to(cuda).unfold(0, 64, 1)[None, None]  # [1, 1, 7, 64]
+    flat = x.contiguous()
+    assert torch.equal(rot(x), rot(flat))
+    both = rot(x, x)
+    assert torch.equal(both[0], rot(flat)) and torch.equal(both[1], rot(flat))
+    leaf = flat.clone().requires_grad_()
+    (got,) = torch.autograd.grad(rot(leaf), leaf, x)
+    (want,) = torch.autograd.grad(rot(leaf), leaf, flat)
+    assert torch.equal(got, want)
+    pools = [torch.zeros((2, 1, 16, 64), dtype=torch.bfloat16, device=cuda) for _ in range(4)]
+    table, n = torch.tensor([[1]], dtype=torch.int32, device=cuda), torch.zeros(1, dtype=torch.int32, device=cuda)
+    a = append_paged(x, x, *pools[:2], table, n, rotary=rot, q=x)
+    b = append_paged(flat, flat, *pools[2:], table, n, rotary=rot, q=flat)
+    assert torch.equal(a, b) and torch.equal(a, rot(flat))
+    assert all(torch.equal(y, z) for y, z in zip(pools[:2], pools[2:])) and pools[0].any()
