@@ -390,7 +390,7 @@ extern "C" cab_status_t cab_paged_append(
   for (int t = H == 0 ? 1 : 0; t < 3; ++t) {
     CAB_REQUIRE((reinterpret_cast<uintptr_t>(src[t]) | reinterpret_cast<uintptr_t>(dst[t])) % es == 0,
                 CAB_ESHAPE, "%s: pointers not aligned to their elements", fn);
-    CAB_REQUIRE(ss[t][3] == 1 && ds[t][3] == 1, CAB_ESHAPE, "%s: last-dim stride must be 1", fn);
+    CAB_REQUIRE(D == 1 || (ss[t][3] == 1 && ds[t][3] == 1), CAB_ESHAPE, "%s: last-dim stride must be 1", fn);
     CAB_REQUIRE(RowLayout(ds[t], t == 0 ? q_size : page_sizes, D).apart, CAB_ESHAPE,
                 "%s: rows of %s overlap", fn, t == 0 ? "q_out" : "the pages");
     a.t[t].src = static_cast<const char*>(src[t]);

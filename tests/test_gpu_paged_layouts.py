@@ -33,3 +33,20 @@ def test_windows_that_slide_over_a_row(cuda):
     b = append_paged(flat, flat, *pools[2:], table, n, rotary=rot, q=flat)
     assert torch.equal(a, b) and torch.equal(a, rot(flat))
     assert all(torch.equal(y, z) for y, z in zip(pools[:2], pools[2:])) and pools[0].any()
+
+
+def test_rows_of_one_value(cuda):
+    """D = 1: the last stride has no meaning."""
+    wide = rand((2, 3, 5, 7), 1).to(cuda)
+    k, v = wide[..., ::7], wide[..., 3::7]
+    assert k.shape == v.shape == (2, 3, 5, 1) and k.stride(3) == 7
+    room = torch.zeros((6, 3, 4, 5), dtype=torch.bfloat16, device=cuda)
+    pools, others = [room[..., 1::5], room[..., 3::5]], [torch.zeros((6, 3, 4, 1), dtype=torch.bfloat16, device=cuda) for _ in range(2)]
+    table = torch.tensor([[4, 0], [2, 5]], dtype=torch.int32, device=cuda)
+    n = torch.tensor([1, 3], dtype=torch.int32, device=cuda)
+    append_paged(k, v, *pools, table, n)
+    append_paged(k.clone(memory_format=torch.contiguous_format), v.clone(memory_format=torch.contiguous_format),
+                 *others, table, n)
+    for x, y in zip(pools, others):
+        assert torch.equal(x, y) and x.any()
+    assert not room[..., [0, 2, 4]].any()
