@@ -492,18 +492,19 @@ extern "C" cab_status_t cab_paged_attn_fwd(
   const int64_t es = static_cast<int64_t>(dtype_size(dtype));
   const void* ptrs[4] = {q, out, k_pages, v_pages};
   const int64_t* strides[4] = {q_strides, o_strides, k_strides, v_strides};
+  const int64_t sizes[4][3] = {{B, H, 1}, {B, H, 1}, {pages, H_kv, page_size}, {pages, H_kv, page_size}};
   for (int t = 0; t < 4; ++t) {
-    const int dims = t < 2 ? 2 : 3;
     CAB_REQUIRE(strides[t][3] == 1, CAB_ESHAPE, "%s: last-dim stride must be 1", fn);
     CAB_REQUIRE(reinterpret_cast<uintptr_t>(ptrs[t]) % 16 == 0, CAB_ESHAPE,
                 "%s: pointers must be 16-byte aligned", fn);
-    for (int d = 0; d < dims; ++d)
-      CAB_REQUIRE(strides[t][d] * es % 16 == 0, CAB_ESHAPE, "%s: rows must be 16-byte aligned", fn);
+    for (int d = 0; d < 3; ++d)  // (the stride of one place has no meaning)
+      CAB_REQUIRE(sizes[t][d] <= 1 || strides[t][d] * es % 16 == 0, CAB_ESHAPE,
+                  "%s: rows must be 16-byte aligned", fn);
   }
   // 16 rows of K and of V are addressed by 32-bit offsets.
   const int64_t lim = int64_t{1} << 25;
-  CAB_REQUIRE(k_strides[2] >= 0 && k_strides[2] * es <= lim && v_strides[2] >= 0 &&
-                  v_strides[2] * es <= lim,
+  CAB_REQUIRE(page_size == 1 || (k_strides[2] >= 0 && k_strides[2] * es <= lim && v_strides[2] >= 0 &&
+                                 v_strides[2] * es <= lim),
               CAB_ESHAPE, "%s: place strides of the pages must be in [0, 2^25] bytes", fn);
   const int64_t out_size[3] = {B, H, 1};
   const int64_t os3[3] = {o_strides[0], o_strides[1], 0}, qs3[3] = {q_strides[0], q_strides[1], 0};

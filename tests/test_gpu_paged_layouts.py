@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from cab_attention.cache import append_paged
-from cab_attention.kernels import Rotary
+from cab_attention.kernels import Rotary, paged_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +50,19 @@ def test_rows_of_one_value(cuda):
     for x, y in zip(pools, others):
         assert torch.equal(x, y) and x.any()
     assert not room[..., [0, 2, 4]].any()
+
+
+def test_dims_of_one_place(cuda):
+    """One head, one page, one place a page, at strides off every boundary."""
+    q = rand((1, 2, 1, 64), 1).to(cuda)
+    k, v = (rand(64 * 40, s).to(cuda) for s in (2, 3))
+    odd = lambda x: x.as_strided((3, 1, 1, 64), (64, 3, 1 << 27, 1))
+    even = lambda x: x[:192].view(3, 1, 1, 64)
+    table = torch.tensor([[2, 0, 1]], dtype=torch.int32, device=cuda)
+    n = torch.tensor([3], dtype=torch.int32, device=cuda)
+    want = paged_attention(q, even(k), even(v), table, n)
+    assert torch.equal(paged_attention(q, odd(k), odd(v), table, n), want)
+    one = lambda x: x[:1024].as_strided((1, 1, 16, 64), (5, 3, 64, 1))
+    flat = lambda x: x[:1024].view(1, 1, 16, 64)
+    want = paged_attention(q, flat(k), flat(v), table[:, 1:2], n)
+    assert torch.equal(paged_attention(q, one(k), one(v), table[:, 1:2], n), want)
