@@ -222,19 +222,22 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(AdjustArgs a) {
   }
   lds_barrier();
 
-  // x / r as x times 1 / r; in fp32 the remainder corrects the product's rounding (it is no number
-  // where x or the product is not finite), in 16 bits that is far below the result's own. Penalties
-  // whose inverse is of no use: divided.
-  const float inverse = 1.f / r;
+  // x / r as x times 1 / r in two parts, the first one rounded down: so the quotient is rounded once, and in 16
+  // bits it is the fp32 one's value, where x times a rounded 1 / r was the neighbour's for a 60th of all x at
+  // r = 1.2. Where nothing is divided the second part is the least number, which no sum shows, since an
+  // infinity times 0 is none. Penalties whose inverse is of no use: divided.
+  constexpr float NEXT_TO_0 = 0x1p-149f;
   const bool usual = r > 1e-30f && r < 1e30f;
+  float inverse = 1.f / r, rest = __builtin_fmaf(-r, inverse, 1.f);
+  if (rest < 0.f) {
+    inverse = __uint_as_float(__float_as_uint(inverse) - 1);
+    rest = __builtin_fmaf(-r, inverse, 1.f);
+  }
+  rest = fmaxf(rest * inverse, NEXT_TO_0);
   auto penalised = [&](float x, uint32_t word) {
     const uint32_t c = PLACES == HALVES ? word & 0xffffu : word, n = c & (GIVEN<PLACES> - 1);
     const float factor = c ? (x > 0.f ? inverse : r) : 1.f;
-    float y = x * factor;
-    if constexpr (DT == CAB_F32) {
-      const float rest = __builtin_fmaf(-y, r, x);
-      if (c && x > 0.f && __builtin_fabsf(rest) < INFINITY) y = __builtin_fmaf(rest, inverse, y);
-    }
+    float y = __builtin_fmaf(x, factor, x * (c && x > 0.f ? rest : NEXT_TO_0));
     if (!usual && c) y = x > 0.f ? x / r : x * r;
     const float off = f * static_cast<float>(n) + p;
     return y - (n ? off : 0.f);
