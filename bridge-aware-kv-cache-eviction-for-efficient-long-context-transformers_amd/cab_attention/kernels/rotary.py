@@ -150,10 +150,12 @@ class Rotary(torch.nn.Module):
             those below ``low`` (1) go by ``1 / factor``, interpolated over the turns between.
 
     ``rotary(q, k, positions)`` turns two tensors ``[B, H, N, D]`` (heads of their own; bf16,
-    fp16 or fp32; any strides) in one launch and returns them in the same layout (contiguous where rows overlap);
-    ``rotary(q, positions=..)`` one. positions: int32 ``[N]`` or ``[B, N]`` on the device (int64 is
-    converted), any value; ``None``: 0 .. N - 1. Angles are within 2e-9 radians for
-    every position (64-bit fixed point, no table); the products are formed in fp32 and rounded once. ``B * N < 2**24``.
+    fp16 or fp32; any strides) in one launch and returns them in the same layout (contiguous
+    where rows overlap); ``rotary(q, positions=..)`` one. positions: int32 ``[N]`` or ``[B, N]`` on the
+    device, any value (int64 is converted: past 32 bits the nearest one); ``None``: 0 .. N - 1. Angles are
+    reduced to a turn within 2e-9 radians at every position (64-bit fixed point, no table), and what is left
+    after quarter turns, up to pi / 4, is held in fp32 (1.5e-7 in all); the products are formed in fp32 and
+    rounded once. ``B * N < 2**24``.
 
     Gradients of any order are recorded. A backward pass that is captured into a graph takes
     them with ``torch.autograd.grad``: leaves that an eager pass has accumulated gradients
