@@ -52,13 +52,15 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         lengths: int32 ``[B]`` on the device, the rows a sequence sees, its own token's
             included (see ``cache.append_paged``). Values outside ``[0, M S]`` count as the
             nearest one inside.
-        scale: defaults to ``1/sqrt(D)``.
+        scale: defaults to ``1/sqrt(D)``; positive, and below 2.3e38.
         out: where the output goes, like q; q itself, or memory of none of the inputs.
 
     Rows behind a length, and pages that are not the sequence's, are not read. A sequence that
     sees no row has output 0 and log-sum-exp -inf. One whose scores have no softmax (a NaN or
-    +inf among them, or all -inf; ``q k^T`` past fp32's range is infinite) has NaN for both. Scores, weights and sums are held in fp32 (weights for
-    the product with 16-bit values: 24 bits with bf16, 22 with fp16); the output is rounded once.
+    +inf among them, or all -inf; ``q k^T`` past fp32's range is infinite) has NaN for both. Scores,
+    weights, their sum and the sum of weights times values are held in fp32, relative to the largest
+    weight (below 2^-126 of it a weight is 0; for the product with 16-bit values weights have 24 bits in
+    bf16, 22 in fp16); the output is rounded once.
     Returns the output ``[B, H, 1, D]``, with ``return_lse`` also the fp32 natural-log
     log-sum-exp ``[B, H, 1]``.
     """

@@ -487,7 +487,8 @@ extern "C" cab_status_t cab_paged_attn_fwd(
   CAB_REQUIRE(q && out && q_strides && k_strides && v_strides && o_strides && lengths, CAB_EINVAL,
               "%s: null argument", fn);
   CAB_REQUIRE(none || (k_pages && v_pages && table), CAB_EINVAL, "%s: null argument", fn);
-  CAB_REQUIRE(std::isfinite(scale) && scale > 0.f, CAB_EINVAL, "%s: scale must be positive", fn);
+  const float c = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
+  CAB_REQUIRE(std::isfinite(c) && c > 0.f, CAB_EINVAL, "%s: scale must be positive, and below 2.3e38", fn);
   CAB_REQUIRE(table_stride == 0 || table_stride >= columns, CAB_ESHAPE, "%s: bad table stride", fn);
   const int64_t es = static_cast<int64_t>(dtype_size(dtype));
   const void* ptrs[4] = {q, out, k_pages, v_pages};
@@ -553,7 +554,7 @@ extern "C" cab_status_t cab_paged_attn_fwd(
   a.group = static_cast<int32_t>(H / H_kv);
   a.H = static_cast<int32_t>(H);
   a.direct = pl.direct;
-  a.c = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
+  a.c = c;
   a.out = static_cast<char*>(out);
   a.lse = lse;
   char* ws = static_cast<char*>(workspace);

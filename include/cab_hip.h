@@ -570,7 +570,7 @@ cab_status_t cab_verify_drafts(const void* logits, const void* draft_logits, cab
  * scaled scores. With no such row: 0 and -inf. Rows whose scores have no softmax (NaN or +inf among them, or
  * all -inf) have NaN for both; q . k past fp32 counts as infinite, finite ones of any size as they are. What is behind a length or in no page of the sequence is
  * not read. q, out: [B, H, 1, D], out is q itself or shares no memory with the
- * inputs; D 64 or 128; H % H_kv == 0; 16-byte aligned rows; place strides
+ * inputs; 0 < scale < 2.3e38; D 64 or 128; H % H_kv == 0; 16-byte aligned rows; place strides
  * in [0, 2^25] bytes. bf16, fp16 (P as 16-bit operands of its upper bits and of what those leave, three in bf16: all 24 bits,
  * two in fp16: 22; sums in fp32) or fp32. workspace: cab_paged_attn_workspace_bytes() bytes (may be 0), 16-byte aligned,
  * overwritten.
