@@ -7,8 +7,9 @@
 //
 // Bound: HBM, each row read and written once, and beside it the vector instructions of counting
 // and of the values that are asked something (64 sequences of 128000 tokens, bf16, histories of
-// 8192: 12.3 us, 10.8 without biases and mask, 6.4 with nothing to do; a copy's rate: 6.9; trees of
-// 26 x 50001 fp32, four of them, 12.4). A workgroup takes a stretch of the vocabulary of
+// 8192, new logits in every call: 13.0 us in a graph of calls, 13.7 in a trace; over the same logits 12.5, of which
+// 11.1 without biases and mask, 6.4 with nothing to do; a copy's rate: 6.9; four trees of 26 x 50001, fp32, 12.7,
+// bf16 12.3). A workgroup takes a stretch of the vocabulary of
 // one sequence and counts the history's tokens that fall into it in LDS (whole numbers: the order
 // of the atomics does not show). In a tree the counts stay as they are from node to node,
 // and only the tokens of a node's line are added and taken off again. The history is read again
@@ -373,8 +374,9 @@ extern "C" cab_status_t cab_adjust_logits(
   const bool tree = drafts != nullptr, with_bias = biases > 0;
   // The longest stretch that leaves a workgroup a CU, and as many groups of a tree's nodes, each of
   // which counts the history anew, as make three of them. (us, with 4 for both -> so: 8 rows of
-  // 128000, histories of 8000, 7.5 -> 5.2; trees of 26 x 50001 10.0 -> 8.4; 4 x 64 x 32000 22.8 -> 17.1;
-  // 8 x 32 x 128000 35.8 -> 32.7; two groups a CU there 34.6, 4 x 26 x 50001 14.0 -> 15.6.)
+  // 128000, histories of 8000, bf16, 7.9 -> 5.3; a tree of 26 x 50001, fp32, 8.3 -> 6.7, four 13.5 -> 12.6; four of
+  // 64 x 32000, fp32, 15.2 -> 15.7, bf16 13.6 -> 13.7; eight of 32 x 128000, bf16, 30.5 -> 33.5. Two groups: four of
+  // 26 x 50001 14.3, the last 34.4; four on these stretches: 12.7, 30.4.)
   // (in a tree the T nodes of a line are counted too)
   const int places = !with_bias ? NO_PLACES
                      : history_len + (tree ? T : 0) < HALF && biases < HALF ? HALVES : WORDS;

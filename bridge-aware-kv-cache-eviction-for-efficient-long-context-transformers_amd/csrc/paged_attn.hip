@@ -18,15 +18,15 @@
 // scalars, so that no load waits for the table and addresses are a scalar base and a fixed
 // offset a lane. Of other sizes the blocks are of 8, 4, 2 or 1 keys, which divide the size, and
 // the lanes that load a key's parts fetch its block's page from the lane that holds it (a
-// look-up of 32 keys a step, one step ahead: 100 keys in pages of 24 6.8 us, of which 5.5 are left;
-// 16 sequences of up to 32768 in pages of 8 260, 243).
+// look-up of 32 keys a step, one step ahead: 100 keys in pages of 24 6.8 us, of which 5.1 are left;
+// 16 sequences of up to 32768 in pages of 8 260, 248).
 // Rows past the length or without a page are not read: zeros take their place, scores -inf.
 //
 // Bound: HBM (K and V, read once); short caches: the latency of a start, a few steps and a merge.
-// Measured, D = 128: 16 sequences of up to 32768 keys, 32 heads on 8, bf16, pages of 16, 203 + 4.8 us
+// Measured, D = 128: 16 sequences of up to 32768 keys, 32 heads on 8, bf16, pages of 16, 205 + 4.6 us
 // (contexts + join; 6.6 TB/s of K and V; with pages in order, or of 64, the same within 4 %); one of 128000
-// keys, 28 heads on 4, fp16, 45 + 5.4; one of 600, 10.6, alone. fp32, D = 64, pages of 24: 3 x 12 heads of up to
-// 5003 keys 17.9 + 4.3.
+// keys, 28 heads on 4, fp16, 46 + 5.3; one of 600, bf16, 10.7 in a graph, alone. fp32, D = 64, pages of 24: 3 x 12
+// heads of up to 5003 keys 16.5 + 4.1.
 #include "decode_common.h"
 #include "row_layout.h"
 
@@ -403,9 +403,12 @@ constexpr int WGS = 256;
 constexpr int64_t MANY_UNITS = 512;
 // Places a sequence up to which a workgroup does a unit alone, without partials and join: of 16 bits,
 // of fp32 (as values of a row's length, whose matrix instructions take seven times as long), and where there
-// is a unit a CU (us, list -> alone: 16 bits, D = 128, 8 units of 608 keys 10.7 -> 9.8, 128 of 1024 18.8 -> 20.2,
-// 256 of up to 1024 28.7 -> 24.8, 1024 of up to 1024 86 -> 81, of up to 4096 256 -> 274; fp32, 8 units, D = 128, 200
-// keys 13.7 -> 13.5, 400 14.8 -> 20.1; D = 64, 400 10.6 both; 256 units, D = 128, of up to 1000 55 -> 51).
+// is a unit a CU (us, list -> alone: bf16, D = 128, 8 units of 608 keys 10.8 -> 10.6, 640 10.9 -> 11.0, 704 10.8 ->
+// 11.7; 32 of 640 11.6 -> 15.1; 128 of 640 19.1 -> 15.8, 768 17.2 -> 18.5; D = 64, 8 units of 640 9.3 -> 8.3, 768
+// 9.4 -> 9.2, 1024 9.8 -> 14.6; 32 of 640 10.1 -> 11.2; 128 of 768 14.6 -> 13.7, 1024 15.1 -> 17.2; a unit a CU,
+// D = 128, 1024 28.6 -> 25.5, 1536 38.7 -> 35.6, D = 64, 1024 19.6 -> 18.3, 1536 24.5 -> 25.1; 1024 units of up to 1024 86
+// -> 81, of up to 4096 256 -> 274; fp32, 8 units, D = 128, 200 keys 12.3 -> 11.2, 256 13.3 -> 13.6, 320 14.0 -> 17.5;
+// D = 64, 400 11.1 -> 10.6, 512 10.9 -> 11.4; 256 units, D = 128, of 1024 56 -> 53).
 constexpr int64_t BRIEF = 640, BRIEF_VALUES = 25600, BRIEF_FILLED = 1024;
 
 PagedPlan paged_plan(cab_dtype_t dtype, int64_t B, int64_t H, int64_t Hkv, int64_t most, int64_t D) {

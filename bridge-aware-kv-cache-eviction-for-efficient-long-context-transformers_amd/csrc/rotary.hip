@@ -14,7 +14,7 @@
 // Bound: HBM, each row read and written once. A workgroup takes 2 tokens (1 where there are few),
 // forms their angles once for all heads (through LDS) and streams the heads: 16 bytes of
 // both of a pair's halves a lane, neighbouring lanes along the row, then tokens, then heads; one
-// head in flight a thread, many waves. Measured, bf16, D = 128: 40 heads of 16384 tokens 63 us, 5.3 TB/s (4 tokens
+// head in flight a thread, many waves. Measured, bf16, D = 128: 40 heads of 16384 tokens 62 us, 5.4 TB/s (4 tokens
 // and 4 heads in flight 75, 4 and 2 70, 2 and 1 67, so with non-temporal stores 63, loads too 62);
 // 8000 tokens into pages, 32 + 8 + 8 heads, 43 us (51); one token of 16 sequences 3.6 us in a graph.
 #include "attn_common.h"
